@@ -13,8 +13,8 @@ Operators (package cudalm_w4a16, modules paged_kv and draft):
   verify   acceptance of drafted tokens against the target's probabilities
            and the token that follows the accepted ones
 
-Layouts: keys [pages, kv heads, D/8, page size, 8], values [pages, kv heads,
-page size/8, D, 8], weights [pages, kv heads, page size] in fp32. Head shapes
+Layouts: keys [pages, kv heads, page size, D], values [pages, kv heads, page
+size/8, D, 8], weights [pages, kv heads, page size] in fp32. Head shapes
 are those of the 24-layer hybrid decoder (8 query heads on 2 key-value heads
 of 256) and generic ones; the vocabulary is its LM head's.
 """
@@ -183,10 +183,10 @@ def _int32(values):
     return torch.tensor(values, dtype=torch.int32, device="cuda")
 
 
-def _tables(gen, lens, page, width=None, skip=0, pages=None):
+def _tables(gen, lens, page, skip=0):
     """Page numbers of every sequence, in random order, -1 past its end."""
     need = _int32([-(-n // page) for n in lens])
-    width = width or max(-(-n // page) for n in lens)
+    width = max(-(-n // page) for n in lens)
     total = int(sum(-(-n // page) for n in lens))
     at = torch.arange(width, device="cuda")[None, :] < need[:, None]
     t = torch.full((len(lens), width), -1, dtype=torch.int32, device="cuda")
@@ -207,7 +207,7 @@ def prepare(case, seed):
         kept = [min(n, case["keep"]) for n in lens]
         st["dst"], more = _tables(gen, kept, page, skip=total)
         pages = total + more
-    st["k"] = _randn(gen, pages, kv, D // 8, page, 8, dtype=dtype)
+    st["k"] = _randn(gen, pages, kv, page, D, dtype=dtype)
     st["v"] = _randn(gen, pages, kv, page // 8, D, 8, dtype=dtype)
     st["w"] = None
     if kind == "evict":  # a heavy tail: few tokens draw most of the attention
@@ -249,7 +249,7 @@ def _prepare_verify(case, gen):
 def _dense(st, cache, keys):
     """[B, kv heads, width * page, D] of a cache through the tables, in fp32."""
     x = cache[st["tables"].clamp(min=0).long()]  # [B, width, kv, ...]
-    x = x.permute(0, 2, 1, 4, 3, 5) if keys else x.permute(0, 2, 1, 3, 5, 4)
+    x = x.permute(0, 2, 1, 3, 4) if keys else x.permute(0, 2, 1, 3, 5, 4)
     return x.reshape(x.shape[0], x.shape[1], -1, st["D"]).float()
 
 
@@ -313,8 +313,7 @@ def _plain_append(st):
     b = torch.repeat_interleave(torch.arange(st["B"], device="cuda"), new, output_size=st["nk"].shape[0])
     t = st["lens"].long()[b] - new[b] + torch.arange(b.shape[0], device="cuda") - cu[b]
     at, off = st["tables"][b, t // st["page"]].long(), t % st["page"]
-    T, kv, D = st["nk"].shape
-    st["k"][at, :, :, off] = st["nk"].view(T, kv, D // 8, 8)
+    st["k"][at, :, off] = st["nk"]
     st["v"][at, :, off // 8, :, off % 8] = st["nv"]
     if st["w"] is None:
         return [st["k"], st["v"]]
@@ -323,7 +322,7 @@ def _plain_append(st):
 
 
 def _plain_evict(st):
-    B, kv, D, page, keep = st["B"], st["kv"], st["D"], st["page"], st["keep"]
+    B, kv, page, keep = st["B"], st["kv"], st["page"], st["keep"]
     n = st["lens"].long()[:, None, None]
     w = st["w"][st["tables"].clamp(min=0).long()].permute(0, 2, 1, 3).reshape(B, kv, -1)
     t = torch.arange(w.shape[2], device="cuda")
@@ -340,7 +339,7 @@ def _plain_evict(st):
     src = kept[b, h, j]
     at, off = st["tables"][b, src // page].long(), src % page
     to, place = st["dst"][b, j // page].long(), j % page
-    st["k"][to, h, :, place] = st["k"][at, h, :, off]
+    st["k"][to, h, place] = st["k"][at, h, off]
     st["v"][to, h, place // 8, :, place % 8] = st["v"][at, h, off // 8, :, off % 8]
     st["w"][to, h, place] = st["w"][at, h, off]
     wide = torch.full((B, kv, keep), -1, dtype=torch.int32, device="cuda")
@@ -441,7 +440,7 @@ def exact(case, seed):
         if case["window"] > 0:
             hidden = hidden | ((p - t >= case["window"]) & (t >= case["sinks"]))
         for h in range(kv):
-            keys = st["k"][ids, h].double().transpose(1, 2).reshape(-1, D)[:length]
+            keys = st["k"][ids, h].double().reshape(-1, D)[:length]
             values = st["v"][ids, h].double().transpose(2, 3).reshape(-1, D)[:length]
             received = torch.zeros(length, dtype=torch.float64, device="cuda")
             for g in range(h * (H // kv), (h + 1) * (H // kv)):
