@@ -1,0 +1,90 @@
+"""Verification of drafted tokens (include/cudalm_draft.h). The reference
+decodes one token per step and has no counterpart."""
+from __future__ import annotations
+
+import ctypes
+
+from . import _I, _P, _SZ, _check, _lib, _stream
+from .paged_kv import _workspace
+
+_L = ctypes.c_int64
+
+_SIGS = {
+    "cudalm_draft_verify_workspace_bytes": ([_I, _I, _I], _SZ),
+    "cudalm_draft_verify": ([_P, _L, _P, _L, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _SZ, _P], _I),
+}
+for _name, (_args, _ret) in _SIGS.items():
+    _fn = getattr(_lib, _name)
+    _fn.argtypes = _args
+    _fn.restype = _ret
+
+EXPORTED_SYMBOLS = tuple(_SIGS)
+
+_types = None
+
+
+def _need(ok, what):
+    if not ok:
+        raise ValueError("draft: " + what)
+
+
+def _probs(p, B, rows, V, like, name):
+    """Row stride of probabilities [B, rows, V]."""
+    if rows == 0:
+        return V
+    _need(tuple(p.shape) == (B, rows, V) and p.dtype == like.dtype and p.device == like.device and
+          p.stride(2) == 1 and (B == 1 or p.stride(0) == rows * p.stride(1)),
+          f"{name} is [{B}, {rows}, {V}] of the target's type, rows contiguous and equally spaced")
+    return p.stride(1) if rows > 1 or B == 1 else p.stride(0)
+
+
+def verify(target, draft_probs, tokens, u_accept, u_next, counts=None, out=None, accepted=None,
+           workspace=None, stream=None):
+    """target [B, G + 1, V] and draft_probs [B, G, V] (None: the draft was
+    certain) hold probabilities in float32, bfloat16 or float16; tokens [B, G]
+    int32 are the drafted ones, counts [B] int32 how many are valid (None: G),
+    u_accept [B, G] and u_next [B] float32 random numbers of [0, 1). Returns
+    (out [B, G + 1] int32: the accepted tokens, the next one, -1 after it;
+    accepted [B] int32)."""
+    global _types
+    import torch
+
+    if _types is None:
+        _types = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    _need(target.dim() == 3 and target.device.type == "cuda" and target.dtype in _types,
+          "target is [B, G + 1, V] in float32, bfloat16 or float16 on the GPU")
+    B, G, V = target.shape
+    G -= 1
+    device = target.device
+    _need(B >= 1 and G >= 0 and V >= 1, "target has a row per drafted token and one more")
+    ts = _probs(target, B, G + 1, V, target, "target")
+    ds, dp = 0, None
+    if draft_probs is not None:
+        ds = _probs(draft_probs, B, G, V, target, "draft_probs")
+        dp = draft_probs.data_ptr()
+    for t, shape, dtype, name in ((tokens, (B, G), torch.int32, "tokens"),
+                                  (u_accept, (B, G), torch.float32, "u_accept"),
+                                  (u_next, (B,), torch.float32, "u_next")):
+        _need(tuple(t.shape) == shape and t.dtype == dtype and t.is_contiguous() and
+              t.device == device, f"{name} is a contiguous {dtype} tensor {list(shape)}")
+    if counts is not None:
+        _need(tuple(counts.shape) == (B,) and counts.dtype == torch.int32 and
+              counts.is_contiguous() and counts.device == device,
+              "counts is a contiguous int32 tensor [B]")
+    if out is None:
+        out = torch.empty(B, G + 1, dtype=torch.int32, device=device)
+    if accepted is None:
+        accepted = torch.empty(B, dtype=torch.int32, device=device)
+    for t, shape, name in ((out, (B, G + 1), "out"), (accepted, (B,), "accepted")):
+        _need(tuple(t.shape) == shape and t.dtype == torch.int32 and t.is_contiguous() and
+              t.device == device, f"{name} is a contiguous int32 tensor {list(shape)}")
+    need = 0
+    if workspace is None:
+        need = _lib.cudalm_draft_verify_workspace_bytes(B, G, V)
+    at, size, held = _workspace(need, workspace, device, stream)
+    rc = _lib.cudalm_draft_verify(target.data_ptr(), ts, dp, ds, _types[target.dtype],
+                                  tokens.data_ptr(), None if counts is None else counts.data_ptr(),
+                                  u_accept.data_ptr(), u_next.data_ptr(), out.data_ptr(),
+                                  accepted.data_ptr(), B, G, V, at, size, _stream(stream))
+    _check(rc, "cudalm_draft_verify")
+    return out, accepted
