@@ -38,20 +38,21 @@ struct PrefillArgs {
   long long token_stride, head_stride;
   float scale_log2;
   int tokens, heads, group, units, splits, least, window, sinks;
+  int negate;  // scale is negative: queries are negated and it is taken positive
 };
 
-// 16 bytes per lane from memory to LDS: lane i's land at dst + 16 i. The
-// compiler's builtin for it makes every later LDS read wait for all such loads,
-// the next tile's among them; here loads_landed() does the waiting.
-__device__ __forceinline__ void load_lds16(const uint16_t* src, uint16_t* dst) {
+// 16 bytes per lane from base (wave-uniform) + offset to LDS: lane i's land at
+// dst + 16 i. The compiler's builtin for it makes every later LDS read wait for
+// all such loads, the next tile's among them; here loads_landed() does the waiting.
+__device__ __forceinline__ void load_lds16(const uint16_t* base, uint32_t offset, uint16_t* dst) {
   const uint32_t at = __builtin_amdgcn_readfirstlane(
       static_cast<uint32_t>(reinterpret_cast<uintptr_t>(dst)));
   uint32_t saved;  // m0 holds the LDS address for the instruction
   asm volatile(
-      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\t"
+      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\t"
       "s_mov_b32 m0, %0"
       : "=&s"(saved)
-      : "s"(at), "v"(src)
+      : "s"(at), "v"(offset), "s"(base)
       : "memory");
 }
 
@@ -62,10 +63,12 @@ __device__ __forceinline__ int swap_bits_2_3(int r) {
   return (r & ~12) | ((r & 4) << 1) | ((r & 8) >> 1);
 }
 
-template <typename T, int D, int NW, int KT>
-__global__ __launch_bounds__(64 * NW, 2) void paged_prefill_kernel(const PrefillArgs a) {
+// NQ: tiles of 32 rows per wave; KT: tokens per step.
+template <typename T, int D, int NQ, int NW, int KT, int WPS>
+__global__ __launch_bounds__(64 * NW, WPS) void paged_prefill_kernel(const PrefillArgs a) {
   constexpr int kShift = KT == 64 ? 6 : 5;
   constexpr int KK = D / 16, DT = D / 32, ST = KT / 32;
+  constexpr int kRows = 32 * NQ * NW;  // of a workgroup
   constexpr int C = D / 8;             // 16-byte chunks of a key row
   constexpr int kLoads = KT * D / 512; // 1 KB loads of a tile of keys (of values)
   constexpr int kTileElems = KT * D;
@@ -77,197 +80,96 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_prefill_kernel(const Prefill
   const int hs = blockIdx.x % (a.kv.kv_heads * a.splits);
   const int unit = a.units - 1 - static_cast<int>(blockIdx.x) / (a.kv.kv_heads * a.splits);
   const int h = hs % a.kv.kv_heads, split = hs / a.kv.kv_heads;
-  const int b = sequence_of(a.cu, a.kv.batch, unit, a.group, 32 * NW, 1);
+  const int b = sequence_of(a.cu, a.kv.batch, unit, a.group, kRows, 1);
   if (b < 0) return;
   const int begin_row = load_uniform(a.cu + b), new_tokens = load_uniform(a.cu + b + 1) - begin_row;
   if (begin_row < 0 || new_tokens < 1 || begin_row + new_tokens > a.tokens) return;
-  const int row0 = (unit - (begin_row * a.group / (32 * NW) + b)) * 32 * NW;
+  const int row0 = (unit - (begin_row * a.group / kRows + b)) * kRows;
   const int rows = new_tokens * a.group;
   if (row0 >= rows) return;
   const int length = a.kv.uniform_length(b), first = length - new_tokens;
 
-  // this lane's row, and the positions of the workgroup's first and last
-  const int row = row0 + wave * 32 + n;
-  const bool real = row < rows;
-  const int j = (real ? row : rows - 1) / a.group;
-  const int pos = real ? first + j : -1;
-  const int wg_first = first + row0 / a.group;
-  const int wg_last = first + (row0 + 32 * NW - 1 < rows ? row0 + 32 * NW - 1 : rows - 1) / a.group;
+  // this lane's rows, and the positions of the wave's and the workgroup's
+  int pos[NQ];
+  long long out_row[NQ];
+  bool real[NQ];
+  u32x4_t qf[NQ][KK];
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    const int row = row0 + (wave * NQ + x) * 32 + n;
+    real[x] = row < rows;
+    const int j = (real[x] ? row : rows - 1) / a.group;
+    pos[x] = real[x] ? first + j : -1;
+    const long long token = static_cast<long long>(begin_row) + j;
+    const int head = h * a.group + (real[x] ? row - j * a.group : 0);
+    out_row[x] = token * a.heads + head;
+    const uint16_t* qp = a.q + token * a.token_stride + head * a.head_stride + 8 * half;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      qf[x][kk] = *reinterpret_cast<const u32x4_t*>(qp + 16 * kk);
+      if (a.negate) qf[x][kk] ^= 0x80008000u;
+    }
+  }
+  const int wave_row = row0 + wave * NQ * 32;
+  auto position = [&](int row) { return first + (row < rows ? row : rows - 1) / a.group; };
+  const int wave_first = position(wave_row), wave_last = position(wave_row + 32 * NQ - 1);
+  const int wg_first = position(row0), wg_last = position(row0 + kRows - 1);
   const PagedTiles tiles(length, wg_first, wg_last, a.window, a.sinks, kShift);
   const int per = tiles_per_split(tiles.count, a.splits, a.least, 1);
   const int begin = split * per, end = begin + per < tiles.count ? begin + per : tiles.count;
 
-  const long long token = static_cast<long long>(begin_row) + j;
-  const int head = h * a.group + (real ? row - j * a.group : 0);
-  const long long out_row = token * a.heads + head;
-
-  u32x4_t qf[KK];
-  {
-    const uint16_t* qp = a.q + token * a.token_stride + head * a.head_stride + 8 * half;
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const u32x4_t*>(qp + 16 * kk);
-  }
-  f32x16_t o[DT];
-  float m = kLowest, l = 0;
+  f32x16_t o[NQ][DT];
+  float m[NQ], l[NQ];
 
   const int P = 1 << a.kv.page_shift;
   const size_t page_elems = static_cast<size_t>(P) * D * a.kv.kv_heads;
   const size_t head_elems = static_cast<size_t>(P) * D * h;
-  // what this lane loads of a 1 KB piece of keys: row and chunk
-  const int piece_row = lane / C, piece_slot = lane % C;
+  // A wave loads 1 KB pieces wave, wave + 4, .. of a tile's keys and values.
+  // Key row r of piece 4 x + wave is r0 + x kStep: its low three bits, and with them
+  // the exchange of its chunks, are the same for every x, and its token is that of r0
+  // plus a number that all lanes share. So one offset per lane serves all loads.
+  static_assert(NW == 4 && KT == 32, "");
+  constexpr int kStep = 2048 / D;
+  const int r0 = wave * (512 / D) + lane / C;
+  const uint32_t k_lane = 2 * (swap_bits_2_3(r0) % 16 * D + 8 * ((lane % C) ^ (r0 & 7)));
+  const int v_piece = wave * 64;  // in channels of the tile's groups of eight tokens
+  const uint32_t v_lane = 16 * (v_piece % D + lane);
 
-  // A tile's pages, and whether every row of the workgroup sees all of it.
-  int t0 = 0, page0 = -1, page1 = -1, page2 = -1, page3 = -1;  // of 16 tokens each
+  // A tile's place and its pages, of 16 tokens each; a bit for each absent one.
+  int t0 = 0, page0 = 0, page1 = 0;
+  uint32_t absent = 0;
   auto look_up = [&](int i) {
     t0 = tiles.tile(i) << kShift;
-    const int s = a.kv.page_shift;
-    page0 = a.kv.uniform_page(b, t0 >> s);
-    page1 = a.kv.uniform_page(b, (t0 + 16) >> s);
-    page2 = KT > 32 ? a.kv.uniform_page(b, (t0 + 32) >> s) : page0;
-    page3 = KT > 32 ? a.kv.uniform_page(b, (t0 + 48) >> s) : page0;
-    return page0 >= 0 && page1 >= 0 && page2 >= 0 && page3 >= 0 && t0 + KT - 1 <= wg_first && row0 + 32 * NW <= rows &&
-           (a.window <= 0 || t0 > wg_last - a.window || t0 + KT - 1 < a.sinks);
+    page0 = a.kv.uniform_page(b, t0 >> a.kv.page_shift);
+    page1 = a.kv.uniform_page(b, (t0 + 16) >> a.kv.page_shift);
+    absent = (page0 < 0) | (page1 < 0) << 1;
   };
   auto fetch = [&](int buf) {
     // absent pages are hidden below; any page will do
-    const int g0 = max(page0, 0), g1 = max(page1, 0), g2 = max(page2, 0), g3 = max(page3, 0);
-    uint16_t* kd = lds + buf * 2 * kTileElems;
+    const size_t at0 = max(page0, 0) * page_elems + head_elems + static_cast<size_t>(t0 & (P - 1)) * D;
+    const size_t at1 =
+        max(page1, 0) * page_elems + head_elems + static_cast<size_t>((t0 + 16) & (P - 1)) * D;
+    uint16_t* kd = lds + buf * 2 * kTileElems + wave * 512;
     uint16_t* vd = kd + kTileElems;
 #pragma unroll
     for (int x = 0; x < kLoads / NW; ++x) {
-      const int piece = x * NW + wave;
-      {
-        const int r = piece * (64 / C) + piece_row;
-        const int tok = swap_bits_2_3(r);
-        // (rows of a piece are tokens of the same 16)
-        const int x16 = (piece * (64 / C)) >> 4;
-        const int pg = x16 < 2 ? (x16 ? g1 : g0) : x16 == 2 ? g2 : g3;
-        const uint16_t* src = a.k + pg * page_elems + head_elems +
-                              static_cast<size_t>((t0 + tok) & (P - 1)) * D +
-                              8 * (piece_slot ^ (r & 7));
-        load_lds16(src, kd + piece * 512);
-      }
-      {
-        const int g = piece * 64 / D;  // group of eight tokens
-        const int x16 = g >> 1;
-        const int pg = x16 < 2 ? (x16 ? g1 : g0) : x16 == 2 ? g2 : g3;
-        const uint16_t* src = a.v + pg * page_elems + head_elems +
-                              static_cast<size_t>((t0 + 8 * g) & (P - 1)) * D +
-                              8 * (piece * 64 % D + lane);
-        load_lds16(src, vd + piece * 512);
-      }
+      // rows of the piece: tokens of 16-token half r / 16, bit 3 of r is bit 2 of the token
+      const int r = x * kStep + wave * (512 / D), g = x * (2048 / (8 * D)) + v_piece / D;
+      load_lds16(a.k + (r & 16 ? at1 : at0) + (D == 256 ? (x & 1) * 4 * D : 0), k_lane, kd + x * 2048);
+      load_lds16(a.v + (g & 2 ? at1 : at0) + (g & 1) * 8 * D, v_lane, vd + x * 2048);
     }
   };
-
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) o[dt][e] = 0;
-  // One tile of keys and values against the wave's rows.
-  uint32_t seen[ST];  // which of a lane's 16 scores (of 32 tokens) its row sees
-  auto step = [&](auto masked, const uint16_t* kt, const uint16_t* vt) {
-    constexpr bool kMasked = decltype(masked)::value;
-    f32x16_t s[ST];
-#pragma unroll
-    for (int st = 0; st < ST; ++st) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[st][e] = 0;
-      const int r = 32 * st + n;
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(
-            kt + r * D + 8 * ((2 * kk + half) ^ (r & 7)));
-        s[st] = T::mfma32(kf, qf[kk], s[st]);
-      }
-    }
-#pragma unroll
-    for (int st = 0; st < ST; ++st) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        s[st][e] *= a.scale_log2;
-        if (kMasked) s[st][e] = (seen[st] >> e) & 1 ? s[st][e] : -__builtin_inff();
-      }
-    }
-    float top = s[0][0];
-#pragma unroll
-    for (int st = 0; st < ST; ++st)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) top = fmaxf(top, s[st][e]);
-    top = fmaxf(top, __shfl_xor(top, 32));
-    // The maximum may lag by up to 2^8 (as in the decode kernel).
-    if (__any(top > m + 8.0f)) {
-      const float next = fmaxf(m, top), r = exp2_fast(m - next);
-      l *= r;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[dt][e] *= r;
-      m = next;
-    }
-    u32x4_t pf[2 * ST];
-    float sum = 0;
-#pragma unroll
-    for (int st = 0; st < ST; ++st)
-#pragma unroll
-      for (int e = 0; e < 16; e += 2) {
-        const float p0 = exp2_fast(s[st][e] - m), p1 = exp2_fast(s[st][e + 1] - m);
-        sum += p0 + p1;
-        // rounded to the values' type, as the matrix unit takes them
-        pf[2 * st + e / 8][e % 8 / 2] = T::pack(p0, p1);
-      }
-    l += sum;
-#pragma unroll
-    for (int x = 0; x < 2 * ST; ++x)
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        const u32x4_t vf =
-            *reinterpret_cast<const u32x4_t*>(vt + ((2 * x + half) * D + 32 * dt + n) * 8);
-        o[dt] = T::mfma32(vf, pf[x], o[dt]);
-      }
-  };
-
-  // Tiles that every row sees whole, the next one on its way meanwhile.
-  int i = begin, buf = 0;
-  while (i < end && !look_up(i)) ++i;
-  if (i < end) fetch(0);
-  while (i < end) {
-    loads_landed();
-    __syncthreads();  // this tile has landed for all waves; the other buffer is free
-    do ++i;
-    while (i < end && !look_up(i));
-    if (i < end) fetch(buf ^ 1);
-    step(std::false_type{}, lds + buf * 2 * kTileElems, lds + (buf * 2 + 1) * kTileElems);
-    buf ^= 1;
-  }
-  // The others: at the diagonal, the ends of the window and the sinks, and
-  // where pages are absent.
-#pragma unroll 1
-  for (i = begin; i < end; ++i) {
-    if (look_up(i)) continue;
-    __syncthreads();
-    fetch(0);
-    const uint32_t absent = (page0 < 0) | (page1 < 0) << 1 | (page2 < 0) << 2 | (page3 < 0) << 3;
-#pragma unroll
-    for (int st = 0; st < ST; ++st) {
-      seen[st] = 0;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int t = 32 * st + 16 * (e >> 3) + 8 * half + (e & 7);
-        seen[st] |= paged_sees(t0 + t, pos, a.window, a.sinks) ? 1u << e : 0u;
-      }
-      const uint32_t gone = absent >> (2 * st);
-      seen[st] &= ~((gone & 1 ? 0x00FFu : 0u) | (gone & 2 ? 0xFF00u : 0u));
-    }
-    loads_landed();
-    __syncthreads();
-    // Values that no row sees may be anything: clear them. Look whether the
-    // others are finite.
-    u32x4_t* vt = reinterpret_cast<u32x4_t*>(lds + kTileElems);
-    uint32_t special = 0;
+  // Zero weights times Inf or NaN are NaN. So in a tile that some row sees only
+  // part of, values past the end or of absent pages (which may be anything) are
+  // cleared, and Inf and NaN among the others taken out; the rows that do see
+  // those get them at the end.
+  uint32_t special = 0;
+  auto clean = [&](u32x4_t* vt, int t0, uint32_t absent) {
+#pragma unroll 2
     for (int u = threadIdx.x; u < KT / 8 * D; u += 64 * NW) {
       const int g = u / D, t = t0 + 8 * g;
-      u32x4_t w = vt[u];
       const bool gone = (absent >> (g >> 1)) & 1;
+      u32x4_t w = vt[u];
       if (gone || t + 8 > length) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -276,68 +178,209 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_prefill_kernel(const Prefill
         }
         vt[u] = w;
       }
-      special |= special_bits<T>(w);
+      const uint32_t bad = special_bits<T>(w);
+      special |= bad;
+      if (bad) vt[u] = finite_part<T>(w);
     }
-    if (lane == 0) votes[wave] = 0;
-    if (__any(special != 0) && lane == 0) votes[wave] = 1;
-    __syncthreads();
-    special = 0;
+  };
+
+  // One tile of keys and values against the wave's rows.
+  auto step = [&](bool whole, int t0, uint32_t absent, const uint16_t* kt, const uint16_t* vt) {
+    f32x16_t s[NQ][ST];
 #pragma unroll
-    for (int w = 0; w < NW; ++w) special |= votes[w];
-    if (special) {
-      for (int u = threadIdx.x; u < KT / 8 * D; u += 64 * NW) vt[u] = finite_part<T>(vt[u]);
-      __syncthreads();
-    }
-    step(std::true_type{}, lds, lds + kTileElems);
-    if (special) {
-      __syncthreads();
-      fetch(0);
-      loads_landed();
-      __syncthreads();
+    for (int st = 0; st < ST; ++st) {
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
+      for (int x = 0; x < NQ; ++x)
 #pragma unroll
-        for (int flip = 0; flip < 2; ++flip) {
-          f32x16_t count;
+        for (int e = 0; e < 16; ++e) s[x][st][e] = 0;
+      const int r = 32 * st + n;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) count[e] = 0;
+      for (int kk = 0; kk < KK; ++kk) {
+        const u32x4_t kf =
+            *reinterpret_cast<const u32x4_t*>(kt + r * D + 8 * ((2 * kk + half) ^ (r & 7)));
 #pragma unroll
-          for (int x = 0; x < 2 * ST; ++x)
-            count = T::mfma32(special_part<T>(vt[(2 * x + half) * D + 32 * dt + n], flip - 1),
-                              seen_operand<T>(seen[x / 2] >> (8 * (x & 1))), count);
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            o[dt][e] += count[e] > 0 ? (flip ? -__builtin_inff() : __builtin_inff()) : 0.0f;
-          asm volatile("" ::: "memory");  // one at a time: few registers over speed here
-          __builtin_amdgcn_sched_barrier(0);
-        }
+        for (int x = 0; x < NQ; ++x) s[x][st] = T::mfma32(kf, qf[x][kk], s[x][st]);
       }
     }
-  }
-  l += __shfl_xor(l, 32);
-  if (!real) return;
-  if (a.part_o) {
-    const size_t at = static_cast<size_t>(split) * a.tokens * a.heads + out_row;
-    if (half == 0) a.part_ml[2 * at] = m, a.part_ml[2 * at + 1] = l;
-    if (begin >= end) return;
-    float* p = a.part_o + at * D + 4 * half;
+    if (!whole) {
+      // Token t0 + 8 half + i is seen from pos if 0 <= pos - that < window.
+      const uint32_t reach = a.window > 0 ? a.window : 0x7FFFFFFF;
+      const bool sinks = t0 < a.sinks;
+#pragma unroll
+      for (int x = 0; x < NQ; ++x) {
+        const int back = pos[x] - t0 - 8 * half;
+        const int sunk = sinks ? min(a.sinks - t0 - 8 * half, back + 1) : -1;
+#pragma unroll
+        for (int st = 0; st < ST; ++st)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int i = 32 * st + 16 * (e >> 3) + (e & 7);
+            bool sees = static_cast<uint32_t>(back - i) < reach || i < sunk;
+            s[x][st][e] = sees ? s[x][st][e] : -__builtin_inff();
+          }
+      }
+      if (absent) {
+#pragma unroll
+        for (int st = 0; st < ST; ++st)
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+            if ((absent >> (2 * st + y)) & 1)
+#pragma unroll
+              for (int x = 0; x < NQ; ++x)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[x][st][8 * y + e] = -__builtin_inff();
+      }
+    }
+    u32x4_t pf[NQ][2 * ST];
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+      float top = s[x][0][0];
+#pragma unroll
+      for (int st = 0; st < ST; ++st)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, s[x][st][e]);
+      top = fmaxf(top, __shfl_xor(top, 32)) * a.scale_log2;
+      // The maximum may lag by up to 2^8 (as in the decode kernel).
+      if (__any(top > m[x] + 8.0f)) {
+        const float next = fmaxf(m[x], top), r = exp2_fast(m[x] - next);
+        l[x] *= r;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[x][dt][e] *= r;
+        m[x] = next;
+      }
+      float sum = 0;
+#pragma unroll
+      for (int st = 0; st < ST; ++st)
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+          const float p0 = exp2_fast(__builtin_fmaf(s[x][st][e], a.scale_log2, -m[x]));
+          const float p1 = exp2_fast(__builtin_fmaf(s[x][st][e + 1], a.scale_log2, -m[x]));
+          sum += p0 + p1;
+          // rounded to the values' type, as the matrix unit takes them
+          pf[x][2 * st + e / 8][e % 8 / 2] = T::pack(p0, p1);
+        }
+      l[x] += sum;
+    }
+#pragma unroll
+    for (int y = 0; y < 2 * ST; ++y)
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const u32x4_t vf =
+            *reinterpret_cast<const u32x4_t*>(vt + ((2 * y + half) * D + 32 * dt + n) * 8);
+#pragma unroll
+        for (int x = 0; x < NQ; ++x) o[x][dt] = T::mfma32(vf, pf[x][y], o[x][dt]);
+      }
+  };
+
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    m[x] = kLowest;
+    l[x] = 0;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-        *reinterpret_cast<f32x4_t*>(p + 32 * dt + 8 * x) =
-            f32x4_t{o[dt][4 * x], o[dt][4 * x + 1], o[dt][4 * x + 2], o[dt][4 * x + 3]};
-    return;
+      for (int e = 0; e < 16; ++e) o[x][dt][e] = 0;
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  uint16_t* y = a.out + out_row * D + 4 * half;
+  // every row from position `from` to `to` sees all of the tile looked up
+  auto seen_whole = [&](int from, int to) {
+    return !absent && t0 + KT - 1 <= from &&
+           (a.window <= 0 || t0 > to - a.window || t0 + KT - 1 < a.sinks);
+  };
+  const bool wg_full = row0 + kRows <= rows, wave_full = wave_row + 32 * NQ <= rows;
+  int buf = 0;
+  if (begin < end) {
+    look_up(begin);
+    fetch(0);
+  }
+#pragma unroll 1
+  for (int i = begin; i < end; ++i) {
+    uint16_t* kt = lds + buf * 2 * kTileElems;
+    uint16_t* vt = kt + kTileElems;
+    const int here = t0;
+    const uint32_t gone = absent;
+    const bool whole = wave_full && seen_whole(wave_first, wave_last);
+    const bool wg_whole = wg_full && seen_whole(wg_first, wg_last);
+    loads_landed();
+    __syncthreads();  // this tile has landed for all waves; the other buffer is free
+    buf ^= 1;
+    if (i + 1 < end) {
+      look_up(i + 1);
+      fetch(buf);
+    }
+    if (!wg_whole) {
+      clean(reinterpret_cast<u32x4_t*>(vt), here, gone);
+      __syncthreads();
+    }
+    if (here <= wave_last) step(whole, here, gone, kt, vt);  // not above the wave's rows
+  }
+  // Inf or NaN for the sums of channels 32 dt .. whose rows see such a value in a
+  // tile that was cleaned of it: how many tokens hold +Inf or NaN, -Inf or NaN.
+  auto add_special = [&](f32x16_t& r, int x, int dt) {
+    f32x16_t up, down;
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
+    for (int e = 0; e < 16; ++e) up[e] = down[e] = 0;
+#pragma unroll 1
+    for (int i = begin; i < end; ++i) {
+      look_up(i);
+      if (wg_full && seen_whole(wg_first, wg_last)) continue;
+#pragma unroll 1
+      for (int y = 0; y < KT / 16; ++y) {
+        const int t = t0 + 16 * y + 8 * half;
+        const int page = a.kv.page(b, t >> a.kv.page_shift);
+        uint32_t seen = 0;
+        u32x4_t w = {0, 0, 0, 0};
+        if (page >= 0) {
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
-      *reinterpret_cast<u32x2_t*>(y + 32 * dt + 8 * x) =
-          u32x2_t{T::pack(o[dt][4 * x] * inv, o[dt][4 * x + 1] * inv),
-                  T::pack(o[dt][4 * x + 2] * inv, o[dt][4 * x + 3] * inv)};
+          for (int e = 0; e < 8; ++e)
+            seen |= paged_sees(t + e, pos[x], a.window, a.sinks) ? 1u << e : 0u;
+          w = *reinterpret_cast<const u32x4_t*>(a.v + page * page_elems + head_elems +
+                                                static_cast<size_t>(t & (P - 1)) * D +
+                                                8 * (32 * dt + n));
+        }
+        const u32x4_t ones = seen_operand<T>(seen);
+        up = T::mfma32(special_part<T>(w, ~0u), ones, up);
+        down = T::mfma32(special_part<T>(w, 0), ones, down);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      r[e] += (up[e] > 0 ? __builtin_inff() : 0.0f) + (down[e] > 0 ? -__builtin_inff() : 0.0f);
+  };
+  votes[wave] = __any(special != 0);
+  __syncthreads();
+  special = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) special |= votes[w];
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    l[x] += __shfl_xor(l[x], 32);
+    const float inv = l[x] == 0.0f ? 0.0f : 1.0f / l[x];
+    const size_t at = static_cast<size_t>(split) * a.tokens * a.heads + out_row[x];
+    if (a.part_o && real[x] && half == 0) a.part_ml[2 * at] = m[x], a.part_ml[2 * at + 1] = l[x];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      f32x16_t r = o[x][dt];
+      if (special) add_special(r, x, dt);
+      if (!real[x]) continue;
+      if (a.part_o) {
+        if (begin >= end) continue;  // the join goes by l
+        float* p = a.part_o + at * D + 32 * dt + 4 * half;
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          *reinterpret_cast<f32x4_t*>(p + 8 * y) =
+              f32x4_t{r[4 * y], r[4 * y + 1], r[4 * y + 2], r[4 * y + 3]};
+      } else {
+        uint16_t* out = a.out + out_row[x] * D + 32 * dt + 4 * half;
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          *reinterpret_cast<u32x2_t*>(out + 8 * y) =
+              u32x2_t{T::pack(r[4 * y] * inv, r[4 * y + 1] * inv),
+                      T::pack(r[4 * y + 2] * inv, r[4 * y + 3] * inv)};
+      }
+    }
+  }
 }
 
 // One wave per (token, head): the join of the splits' partial sums.
@@ -373,16 +416,12 @@ __global__ __launch_bounds__(256) void paged_prefill_join_kernel(const PrefillAr
   }
 }
 
+// Rows of a workgroup: 4 waves of one or two tiles of 32.
 constexpr int kWaves = 4;
-
-template <int D>
-constexpr int tile_tokens() {
-  return D == 256 ? 32 : 64;
-}
 
 struct PrefillPlan {
   long long units;
-  int splits, least;
+  int nq, splits, least;
   size_t o_bytes, ml_bytes;
   size_t bytes() const { return o_bytes + ml_bytes; }
 };
@@ -390,12 +429,14 @@ struct PrefillPlan {
 PrefillPlan plan_of(const cudalm_paged_kv* kv, const cudalm_paged_query* q, int tokens) {
   PrefillPlan p;
   const int group = q->heads / kv->kv_heads;
-  const int kt = kv->head_dim == 256 ? 32 : 64;
-  p.units = static_cast<long long>(tokens) * group / (32 * kWaves) + kv->batch;
+  constexpr int kt = 32;
+  p.nq = kv->head_dim == 256 ? 1 : 2;
+  const int wg_rows = 32 * p.nq * kWaves;
+  p.units = static_cast<long long>(tokens) * group / wg_rows + kv->batch;
   const int len = expected_len(kv, q->max_len), window = window_of(q);
   long long tiles = (len + kt - 1) / kt;
   if (window > 0) {
-    const long long near = (static_cast<long long>(window) + 32 * kWaves / group + kt) / kt + 1 +
+    const long long near = (static_cast<long long>(window) + wg_rows / group + kt) / kt + 1 +
                            (sinks_of(q) + kt - 1) / kt;
     tiles = near < tiles ? near : tiles;
   }
@@ -405,35 +446,42 @@ PrefillPlan plan_of(const cudalm_paged_kv* kv, const cudalm_paged_query* q, int 
   want = want < most ? want : most;
   want = want < 16 ? want : 16;
   p.splits = static_cast<int>(want < 1 ? 1 : want);
-  p.least = static_cast<int>((tiles + p.splits - 1) / p.splits);
-  if (p.least < 1) p.least = 1;
-  // a shorter range of tiles (rows early in a chunk) still uses all splits
-  p.least = p.least < 4 ? p.least : 4;
+  p.least = 4;
   const size_t parts = static_cast<size_t>(p.splits) * tokens * q->heads;
   p.o_bytes = p.splits > 1 ? parts * kv->head_dim * 4 : 0;
   p.ml_bytes = p.splits > 1 ? parts * 8 : 0;
   return p;
 }
 
-template <typename T, int D>
-int launch(const PrefillArgs& a, hipStream_t stream) {
-  constexpr int KT = tile_tokens<D>();
-  auto kernel = paged_prefill_kernel<T, D, kWaves, KT>;
+template <typename T, int D, int NQ>
+int launch_nq(const PrefillArgs& a, hipStream_t stream) {
+  constexpr int KT = 32;
+  auto kernel = paged_prefill_kernel<T, D, NQ, kWaves, KT, 2>;
   constexpr size_t kLds = 4 * KT * D * 2 + 4 * kWaves;
   if (!allow_lds(kernel, kLds)) return CUDALM_W4A16_ELAUNCH;
   const unsigned grid = static_cast<unsigned>(a.units) * a.kv.kv_heads * a.splits;
   kernel<<<grid, 64 * kWaves, kLds, stream>>>(a);
-  if (a.splits > 1) {
-    if (const int rc = launch_status()) return rc;
-    const long long rows = static_cast<long long>(a.tokens) * a.heads;
-    paged_prefill_join_kernel<T, D><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, stream>>>(a);
-  }
+  return launch_status();
+}
+
+template <typename T, int D>
+int launch(const PrefillArgs& a, int nq, hipStream_t stream) {
+  int rc;
+  if constexpr (D == 256)
+    rc = launch_nq<T, D, 1>(a, stream);
+  else
+    rc = nq == 1 ? launch_nq<T, D, 1>(a, stream) : launch_nq<T, D, 2>(a, stream);
+  if (rc || a.splits == 1) return rc;
+  const long long rows = static_cast<long long>(a.tokens) * a.heads;
+  paged_prefill_join_kernel<T, D><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, stream>>>(a);
   return launch_status();
 }
 
 template <typename T>
-int launch_d(int D, const PrefillArgs& a, hipStream_t stream) {
-  return D == 64 ? launch<T, 64>(a, stream) : D == 128 ? launch<T, 128>(a, stream) : launch<T, 256>(a, stream);
+int launch_d(int D, const PrefillArgs& a, int nq, hipStream_t stream) {
+  return D == 64    ? launch<T, 64>(a, nq, stream)
+         : D == 128 ? launch<T, 128>(a, nq, stream)
+                    : launch<T, 256>(a, nq, stream);
 }
 
 int check(const cudalm_paged_kv* kv, const cudalm_paged_query* q, int tokens) {
@@ -446,11 +494,14 @@ int check(const cudalm_paged_kv* kv, const cudalm_paged_query* q, int tokens) {
   return CUDALM_W4A16_OK;
 }
 
+template <typename T, int D>
+int regs_of_dim() {
+  return regs_of(paged_prefill_kernel<T, D, D == 256 ? 1 : 2, kWaves, 32, 2>);
+}
+
 template <typename T>
 int regs_of_type(int D) {
-  return D == 64    ? regs_of(paged_prefill_kernel<T, 64, kWaves, tile_tokens<64>()>)
-         : D == 128 ? regs_of(paged_prefill_kernel<T, 128, kWaves, tile_tokens<128>()>)
-                    : regs_of(paged_prefill_kernel<T, 256, kWaves, tile_tokens<256>()>);
+  return D == 64 ? regs_of_dim<T, 64>() : D == 128 ? regs_of_dim<T, 128>() : regs_of_dim<T, 256>();
 }
 
 }  // namespace
@@ -495,7 +546,8 @@ extern "C" int cudalm_paged_prefill(const cudalm_paged_kv* kv, const cudalm_page
   a.cu = cu_new;
   a.token_stride = q->token_stride;
   a.head_stride = q->head_stride;
-  a.scale_log2 = q->scale * kLog2e;
+  a.negate = q->scale < 0;
+  a.scale_log2 = (a.negate ? -q->scale : q->scale) * kLog2e;
   a.tokens = tokens;
   a.heads = q->heads;
   a.group = q->heads / kv->kv_heads;
@@ -504,6 +556,6 @@ extern "C" int cudalm_paged_prefill(const cudalm_paged_kv* kv, const cudalm_page
   a.least = p.least;
   a.window = window_of(q);
   a.sinks = sinks_of(q);
-  return kv->type == CUDALM_PAGED_BF16 ? launch_d<PagedBf16>(kv->head_dim, a, stream)
-                                       : launch_d<PagedF16>(kv->head_dim, a, stream);
+  return kv->type == CUDALM_PAGED_BF16 ? launch_d<PagedBf16>(kv->head_dim, a, p.nq, stream)
+                                       : launch_d<PagedF16>(kv->head_dim, a, p.nq, stream);
 }
