@@ -19,12 +19,16 @@
 // many rows, would meet in the same banks.
 
 #include <cstdint>
-#include <type_traits>
 
 #include "paged_device.h"
 
 namespace cudalm_hip {
 namespace {
+
+constexpr int kWaves = 4;           // of a workgroup, 32 rows each
+constexpr int kRows = 32 * kWaves;
+constexpr int kTile = 32;           // tokens per step
+constexpr int kTileShift = 5;
 
 struct PrefillArgs {
   PagedView kv;
@@ -63,12 +67,9 @@ __device__ __forceinline__ int swap_bits_2_3(int r) {
   return (r & ~12) | ((r & 4) << 1) | ((r & 8) >> 1);
 }
 
-// NQ: tiles of 32 rows per wave; KT: tokens per step.
-template <typename T, int D, int NQ, int NW, int KT, int WPS>
-__global__ __launch_bounds__(64 * NW, WPS) void paged_prefill_kernel(const PrefillArgs a) {
-  constexpr int kShift = KT == 64 ? 6 : 5;
-  constexpr int KK = D / 16, DT = D / 32, ST = KT / 32;
-  constexpr int kRows = 32 * NQ * NW;  // of a workgroup
+template <typename T, int D>
+__global__ __launch_bounds__(64 * kWaves, 2) void paged_prefill_kernel(const PrefillArgs a) {
+  constexpr int KT = kTile, KK = D / 16, DT = D / 32;
   constexpr int C = D / 8;             // 16-byte chunks of a key row
   constexpr int kLoads = KT * D / 512; // 1 KB loads of a tile of keys (of values)
   constexpr int kTileElems = KT * D;
@@ -89,37 +90,32 @@ __global__ __launch_bounds__(64 * NW, WPS) void paged_prefill_kernel(const Prefi
   if (row0 >= rows) return;
   const int length = a.kv.uniform_length(b), first = length - new_tokens;
 
-  // this lane's rows, and the positions of the wave's and the workgroup's
-  int pos[NQ];
-  long long out_row[NQ];
-  bool real[NQ];
-  u32x4_t qf[NQ][KK];
-#pragma unroll
-  for (int x = 0; x < NQ; ++x) {
-    const int row = row0 + (wave * NQ + x) * 32 + n;
-    real[x] = row < rows;
-    const int j = (real[x] ? row : rows - 1) / a.group;
-    pos[x] = real[x] ? first + j : -1;
-    const long long token = static_cast<long long>(begin_row) + j;
-    const int head = h * a.group + (real[x] ? row - j * a.group : 0);
-    out_row[x] = token * a.heads + head;
+  // this lane's row, and the positions of the wave's and the workgroup's first and last
+  const int wave_row = row0 + 32 * wave, row = wave_row + n;
+  const bool real = row < rows;
+  const int j = (real ? row : rows - 1) / a.group;
+  const int pos = real ? first + j : -1;
+  const long long token = static_cast<long long>(begin_row) + j;
+  const int head = h * a.group + (real ? row - j * a.group : 0);
+  const long long out_row = token * a.heads + head;
+  u32x4_t qf[KK];
+  {
     const uint16_t* qp = a.q + token * a.token_stride + head * a.head_stride + 8 * half;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
-      qf[x][kk] = *reinterpret_cast<const u32x4_t*>(qp + 16 * kk);
-      if (a.negate) qf[x][kk] ^= 0x80008000u;
+      qf[kk] = *reinterpret_cast<const u32x4_t*>(qp + 16 * kk);
+      if (a.negate) qf[kk] ^= 0x80008000u;
     }
   }
-  const int wave_row = row0 + wave * NQ * 32;
   auto position = [&](int row) { return first + (row < rows ? row : rows - 1) / a.group; };
-  const int wave_first = position(wave_row), wave_last = position(wave_row + 32 * NQ - 1);
+  const int wave_first = position(wave_row), wave_last = position(wave_row + 31);
   const int wg_first = position(row0), wg_last = position(row0 + kRows - 1);
-  const PagedTiles tiles(length, wg_first, wg_last, a.window, a.sinks, kShift);
+  const PagedTiles tiles(length, wg_first, wg_last, a.window, a.sinks, kTileShift);
   const int per = tiles_per_split(tiles.count, a.splits, a.least, 1);
   const int begin = split * per, end = begin + per < tiles.count ? begin + per : tiles.count;
 
-  f32x16_t o[NQ][DT];
-  float m[NQ], l[NQ];
+  f32x16_t o[DT];
+  float m = kLowest, l = 0;
 
   const int P = 1 << a.kv.page_shift;
   const size_t page_elems = static_cast<size_t>(P) * D * a.kv.kv_heads;
@@ -128,7 +124,6 @@ __global__ __launch_bounds__(64 * NW, WPS) void paged_prefill_kernel(const Prefi
   // Key row r of piece 4 x + wave is r0 + x kStep: its low three bits, and with them
   // the exchange of its chunks, are the same for every x, and its token is that of r0
   // plus a number that all lanes share. So one offset per lane serves all loads.
-  static_assert(NW == 4 && KT == 32, "");
   constexpr int kStep = 2048 / D;
   const int r0 = wave * (512 / D) + lane / C;
   const uint32_t k_lane = 2 * (swap_bits_2_3(r0) % 16 * D + 8 * ((lane % C) ^ (r0 & 7)));
@@ -139,7 +134,7 @@ __global__ __launch_bounds__(64 * NW, WPS) void paged_prefill_kernel(const Prefi
   int t0 = 0, page0 = 0, page1 = 0;
   uint32_t absent = 0;
   auto look_up = [&](int i) {
-    t0 = tiles.tile(i) << kShift;
+    t0 = tiles.tile(i) << kTileShift;
     page0 = a.kv.uniform_page(b, t0 >> a.kv.page_shift);
     page1 = a.kv.uniform_page(b, (t0 + 16) >> a.kv.page_shift);
     absent = (page0 < 0) | (page1 < 0) << 1;
@@ -152,7 +147,7 @@ __global__ __launch_bounds__(64 * NW, WPS) void paged_prefill_kernel(const Prefi
     uint16_t* kd = lds + buf * 2 * kTileElems + wave * 512;
     uint16_t* vd = kd + kTileElems;
 #pragma unroll
-    for (int x = 0; x < kLoads / NW; ++x) {
+    for (int x = 0; x < kLoads / kWaves; ++x) {
       // rows of the piece: tokens of 16-token half r / 16, bit 3 of r is bit 2 of the token
       const int r = x * kStep + wave * (512 / D), g = x * (2048 / (8 * D)) + v_piece / D;
       load_lds16(a.k + (r & 16 ? at1 : at0) + (D == 256 ? (x & 1) * 4 * D : 0), k_lane, kd + x * 2048);
@@ -166,7 +161,7 @@ __global__ __launch_bounds__(64 * NW, WPS) void paged_prefill_kernel(const Prefi
   uint32_t special = 0;
   auto clean = [&](u32x4_t* vt, int t0, uint32_t absent) {
 #pragma unroll 2
-    for (int u = threadIdx.x; u < KT / 8 * D; u += 64 * NW) {
+    for (int u = threadIdx.x; u < KT / 8 * D; u += 64 * kWaves) {
       const int g = u / D, t = t0 + 8 * g;
       const bool gone = (absent >> (g >> 1)) & 1;
       u32x4_t w = vt[u];
@@ -186,109 +181,71 @@ __global__ __launch_bounds__(64 * NW, WPS) void paged_prefill_kernel(const Prefi
 
   // One tile of keys and values against the wave's rows.
   auto step = [&](bool whole, int t0, uint32_t absent, const uint16_t* kt, const uint16_t* vt) {
-    f32x16_t s[NQ][ST];
+    f32x16_t s;
 #pragma unroll
-    for (int st = 0; st < ST; ++st) {
+    for (int e = 0; e < 16; ++e) s[e] = 0;
 #pragma unroll
-      for (int x = 0; x < NQ; ++x)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[x][st][e] = 0;
-      const int r = 32 * st + n;
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        const u32x4_t kf =
-            *reinterpret_cast<const u32x4_t*>(kt + r * D + 8 * ((2 * kk + half) ^ (r & 7)));
-#pragma unroll
-        for (int x = 0; x < NQ; ++x) s[x][st] = T::mfma32(kf, qf[x][kk], s[x][st]);
-      }
-    }
+    for (int kk = 0; kk < KK; ++kk)
+      s = T::mfma32(*reinterpret_cast<const u32x4_t*>(kt + n * D + 8 * ((2 * kk + half) ^ (n & 7))),
+                    qf[kk], s);
+    // s[e] is the score of token t0 + 16 (e / 8) + 8 half + e % 8
     if (!whole) {
-      // Token t0 + 8 half + i is seen from pos if 0 <= pos - that < window.
+      // token t is seen from p if 0 <= p - t < window, or if t is a sink up to p
       const uint32_t reach = a.window > 0 ? a.window : 0x7FFFFFFF;
-      const bool sinks = t0 < a.sinks;
+      const int back = pos - t0 - 8 * half;
+      const int sunk = t0 < a.sinks ? min(a.sinks - t0 - 8 * half, back + 1) : -1;
 #pragma unroll
-      for (int x = 0; x < NQ; ++x) {
-        const int back = pos[x] - t0 - 8 * half;
-        const int sunk = sinks ? min(a.sinks - t0 - 8 * half, back + 1) : -1;
-#pragma unroll
-        for (int st = 0; st < ST; ++st)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int i = 32 * st + 16 * (e >> 3) + (e & 7);
-            bool sees = static_cast<uint32_t>(back - i) < reach || i < sunk;
-            s[x][st][e] = sees ? s[x][st][e] : -__builtin_inff();
-          }
-      }
-      if (absent) {
-#pragma unroll
-        for (int st = 0; st < ST; ++st)
-#pragma unroll
-          for (int y = 0; y < 2; ++y)
-            if ((absent >> (2 * st + y)) & 1)
-#pragma unroll
-              for (int x = 0; x < NQ; ++x)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) s[x][st][8 * y + e] = -__builtin_inff();
+      for (int e = 0; e < 16; ++e) {
+        const int i = 16 * (e >> 3) + (e & 7);
+        const bool sees = (static_cast<uint32_t>(back - i) < reach || i < sunk) &&
+                          !((absent >> (e >> 3)) & 1);
+        s[e] = sees ? s[e] : -__builtin_inff();
       }
     }
-    u32x4_t pf[NQ][2 * ST];
+    float top = s[0];
 #pragma unroll
-    for (int x = 0; x < NQ; ++x) {
-      float top = s[x][0][0];
+    for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
+    top = fmaxf(top, __shfl_xor(top, 32)) * a.scale_log2;
+    // The maximum may lag by up to 2^8 (as in the decode kernel).
+    if (__any(top > m + 8.0f)) {
+      const float next = fmaxf(m, top), r = exp2_fast(m - next);
+      l *= r;
 #pragma unroll
-      for (int st = 0; st < ST; ++st)
+      for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) top = fmaxf(top, s[x][st][e]);
-      top = fmaxf(top, __shfl_xor(top, 32)) * a.scale_log2;
-      // The maximum may lag by up to 2^8 (as in the decode kernel).
-      if (__any(top > m[x] + 8.0f)) {
-        const float next = fmaxf(m[x], top), r = exp2_fast(m[x] - next);
-        l[x] *= r;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[x][dt][e] *= r;
-        m[x] = next;
-      }
-      float sum = 0;
-#pragma unroll
-      for (int st = 0; st < ST; ++st)
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          const float p0 = exp2_fast(__builtin_fmaf(s[x][st][e], a.scale_log2, -m[x]));
-          const float p1 = exp2_fast(__builtin_fmaf(s[x][st][e + 1], a.scale_log2, -m[x]));
-          sum += p0 + p1;
-          // rounded to the values' type, as the matrix unit takes them
-          pf[x][2 * st + e / 8][e % 8 / 2] = T::pack(p0, p1);
-        }
-      l[x] += sum;
+        for (int e = 0; e < 16; ++e) o[dt][e] *= r;
+      m = next;
     }
+    u32x4_t pf[2];
+    float sum = 0;
 #pragma unroll
-    for (int y = 0; y < 2 * ST; ++y)
+    for (int e = 0; e < 16; e += 2) {
+      const float p0 = exp2_fast(__builtin_fmaf(s[e], a.scale_log2, -m));
+      const float p1 = exp2_fast(__builtin_fmaf(s[e + 1], a.scale_log2, -m));
+      sum += p0 + p1;
+      // rounded to the values' type, as the matrix unit takes them
+      pf[e / 8][e % 8 / 2] = T::pack(p0, p1);
+    }
+    l += sum;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        const u32x4_t vf =
-            *reinterpret_cast<const u32x4_t*>(vt + ((2 * y + half) * D + 32 * dt + n) * 8);
+    for (int y = 0; y < 2; ++y)
 #pragma unroll
-        for (int x = 0; x < NQ; ++x) o[x][dt] = T::mfma32(vf, pf[x][y], o[x][dt]);
-      }
+      for (int dt = 0; dt < DT; ++dt)
+        o[dt] = T::mfma32(
+            *reinterpret_cast<const u32x4_t*>(vt + ((2 * y + half) * D + 32 * dt + n) * 8), pf[y],
+            o[dt]);
   };
 
 #pragma unroll
-  for (int x = 0; x < NQ; ++x) {
-    m[x] = kLowest;
-    l[x] = 0;
+  for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) o[x][dt][e] = 0;
-  }
+    for (int e = 0; e < 16; ++e) o[dt][e] = 0;
   // every row from position `from` to `to` sees all of the tile looked up
   auto seen_whole = [&](int from, int to) {
     return !absent && t0 + KT - 1 <= from &&
            (a.window <= 0 || t0 > to - a.window || t0 + KT - 1 < a.sinks);
   };
-  const bool wg_full = row0 + kRows <= rows, wave_full = wave_row + 32 * NQ <= rows;
+  const bool wg_full = row0 + kRows <= rows, wave_full = wave_row + 32 <= rows;
   int buf = 0;
   if (begin < end) {
     look_up(begin);
@@ -317,7 +274,7 @@ __global__ __launch_bounds__(64 * NW, WPS) void paged_prefill_kernel(const Prefi
   }
   // Inf or NaN for the sums of channels 32 dt .. whose rows see such a value in a
   // tile that was cleaned of it: how many tokens hold +Inf or NaN, -Inf or NaN.
-  auto add_special = [&](f32x16_t& r, int x, int dt) {
+  auto add_special = [&](f32x16_t& r, int dt) {
     f32x16_t up, down;
 #pragma unroll
     for (int e = 0; e < 16; ++e) up[e] = down[e] = 0;
@@ -334,7 +291,7 @@ __global__ __launch_bounds__(64 * NW, WPS) void paged_prefill_kernel(const Prefi
         if (page >= 0) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            seen |= paged_sees(t + e, pos[x], a.window, a.sinks) ? 1u << e : 0u;
+            seen |= paged_sees(t + e, pos, a.window, a.sinks) ? 1u << e : 0u;
           w = *reinterpret_cast<const u32x4_t*>(a.v + page * page_elems + head_elems +
                                                 static_cast<size_t>(t & (P - 1)) * D +
                                                 8 * (32 * dt + n));
@@ -352,33 +309,30 @@ __global__ __launch_bounds__(64 * NW, WPS) void paged_prefill_kernel(const Prefi
   __syncthreads();
   special = 0;
 #pragma unroll
-  for (int w = 0; w < NW; ++w) special |= votes[w];
+  for (int w = 0; w < kWaves; ++w) special |= votes[w];
+  l += __shfl_xor(l, 32);
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const size_t at = static_cast<size_t>(split) * a.tokens * a.heads + out_row;
+  if (a.part_o && real && half == 0) a.part_ml[2 * at] = m, a.part_ml[2 * at + 1] = l;
 #pragma unroll
-  for (int x = 0; x < NQ; ++x) {
-    l[x] += __shfl_xor(l[x], 32);
-    const float inv = l[x] == 0.0f ? 0.0f : 1.0f / l[x];
-    const size_t at = static_cast<size_t>(split) * a.tokens * a.heads + out_row[x];
-    if (a.part_o && real[x] && half == 0) a.part_ml[2 * at] = m[x], a.part_ml[2 * at + 1] = l[x];
+  for (int dt = 0; dt < DT; ++dt) {
+    f32x16_t r = o[dt];
+    if (special) add_special(r, dt);
+    if (!real) continue;
+    if (a.part_o) {
+      if (begin >= end) continue;  // the join goes by l
+      float* p = a.part_o + at * D + 32 * dt + 4 * half;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      f32x16_t r = o[x][dt];
-      if (special) add_special(r, x, dt);
-      if (!real[x]) continue;
-      if (a.part_o) {
-        if (begin >= end) continue;  // the join goes by l
-        float* p = a.part_o + at * D + 32 * dt + 4 * half;
+      for (int y = 0; y < 4; ++y)
+        *reinterpret_cast<f32x4_t*>(p + 8 * y) =
+            f32x4_t{r[4 * y], r[4 * y + 1], r[4 * y + 2], r[4 * y + 3]};
+    } else {
+      uint16_t* out = a.out + out_row * D + 32 * dt + 4 * half;
 #pragma unroll
-        for (int y = 0; y < 4; ++y)
-          *reinterpret_cast<f32x4_t*>(p + 8 * y) =
-              f32x4_t{r[4 * y], r[4 * y + 1], r[4 * y + 2], r[4 * y + 3]};
-      } else {
-        uint16_t* out = a.out + out_row[x] * D + 32 * dt + 4 * half;
-#pragma unroll
-        for (int y = 0; y < 4; ++y)
-          *reinterpret_cast<u32x2_t*>(out + 8 * y) =
-              u32x2_t{T::pack(r[4 * y] * inv, r[4 * y + 1] * inv),
-                      T::pack(r[4 * y + 2] * inv, r[4 * y + 3] * inv)};
-      }
+      for (int y = 0; y < 4; ++y)
+        *reinterpret_cast<u32x2_t*>(out + 8 * y) =
+            u32x2_t{T::pack(r[4 * y] * inv, r[4 * y + 1] * inv),
+                    T::pack(r[4 * y + 2] * inv, r[4 * y + 3] * inv)};
     }
   }
 }
@@ -416,12 +370,9 @@ __global__ __launch_bounds__(256) void paged_prefill_join_kernel(const PrefillAr
   }
 }
 
-// Rows of a workgroup: 4 waves of one or two tiles of 32.
-constexpr int kWaves = 4;
-
 struct PrefillPlan {
   long long units;
-  int nq, splits, least;
+  int splits, least;
   size_t o_bytes, ml_bytes;
   size_t bytes() const { return o_bytes + ml_bytes; }
 };
@@ -429,15 +380,12 @@ struct PrefillPlan {
 PrefillPlan plan_of(const cudalm_paged_kv* kv, const cudalm_paged_query* q, int tokens) {
   PrefillPlan p;
   const int group = q->heads / kv->kv_heads;
-  constexpr int kt = 32;
-  p.nq = kv->head_dim == 256 ? 1 : 2;
-  const int wg_rows = 32 * p.nq * kWaves;
-  p.units = static_cast<long long>(tokens) * group / wg_rows + kv->batch;
+  p.units = static_cast<long long>(tokens) * group / kRows + kv->batch;
   const int len = expected_len(kv, q->max_len), window = window_of(q);
-  long long tiles = (len + kt - 1) / kt;
+  long long tiles = (len + kTile - 1) / kTile;
   if (window > 0) {
-    const long long near = (static_cast<long long>(window) + wg_rows / group + kt) / kt + 1 +
-                           (sinks_of(q) + kt - 1) / kt;
+    const long long near = (static_cast<long long>(window) + kRows / group + kTile) / kTile + 1 +
+                           (sinks_of(q) + kTile - 1) / kTile;
     tiles = near < tiles ? near : tiles;
   }
   const long long groups = p.units * kv->kv_heads;
@@ -453,35 +401,26 @@ PrefillPlan plan_of(const cudalm_paged_kv* kv, const cudalm_paged_query* q, int 
   return p;
 }
 
-template <typename T, int D, int NQ>
-int launch_nq(const PrefillArgs& a, hipStream_t stream) {
-  constexpr int KT = 32;
-  auto kernel = paged_prefill_kernel<T, D, NQ, kWaves, KT, 2>;
-  constexpr size_t kLds = 4 * KT * D * 2 + 4 * kWaves;
+template <typename T, int D>
+int launch(const PrefillArgs& a, hipStream_t stream) {
+  auto kernel = paged_prefill_kernel<T, D>;
+  constexpr size_t kLds = 4 * kTile * D * 2 + 4 * kWaves;
   if (!allow_lds(kernel, kLds)) return CUDALM_W4A16_ELAUNCH;
   const unsigned grid = static_cast<unsigned>(a.units) * a.kv.kv_heads * a.splits;
   kernel<<<grid, 64 * kWaves, kLds, stream>>>(a);
-  return launch_status();
-}
-
-template <typename T, int D>
-int launch(const PrefillArgs& a, int nq, hipStream_t stream) {
-  int rc;
-  if constexpr (D == 256)
-    rc = launch_nq<T, D, 1>(a, stream);
-  else
-    rc = nq == 1 ? launch_nq<T, D, 1>(a, stream) : launch_nq<T, D, 2>(a, stream);
-  if (rc || a.splits == 1) return rc;
-  const long long rows = static_cast<long long>(a.tokens) * a.heads;
-  paged_prefill_join_kernel<T, D><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, stream>>>(a);
+  if (a.splits > 1) {
+    if (const int rc = launch_status()) return rc;
+    const long long rows = static_cast<long long>(a.tokens) * a.heads;
+    paged_prefill_join_kernel<T, D><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, stream>>>(a);
+  }
   return launch_status();
 }
 
 template <typename T>
-int launch_d(int D, const PrefillArgs& a, int nq, hipStream_t stream) {
-  return D == 64    ? launch<T, 64>(a, nq, stream)
-         : D == 128 ? launch<T, 128>(a, nq, stream)
-                    : launch<T, 256>(a, nq, stream);
+int launch_d(int D, const PrefillArgs& a, hipStream_t stream) {
+  return D == 64    ? launch<T, 64>(a, stream)
+         : D == 128 ? launch<T, 128>(a, stream)
+                    : launch<T, 256>(a, stream);
 }
 
 int check(const cudalm_paged_kv* kv, const cudalm_paged_query* q, int tokens) {
@@ -494,14 +433,11 @@ int check(const cudalm_paged_kv* kv, const cudalm_paged_query* q, int tokens) {
   return CUDALM_W4A16_OK;
 }
 
-template <typename T, int D>
-int regs_of_dim() {
-  return regs_of(paged_prefill_kernel<T, D, D == 256 ? 1 : 2, kWaves, 32, 2>);
-}
-
 template <typename T>
 int regs_of_type(int D) {
-  return D == 64 ? regs_of_dim<T, 64>() : D == 128 ? regs_of_dim<T, 128>() : regs_of_dim<T, 256>();
+  return D == 64    ? regs_of(paged_prefill_kernel<T, 64>)
+         : D == 128 ? regs_of(paged_prefill_kernel<T, 128>)
+                    : regs_of(paged_prefill_kernel<T, 256>);
 }
 
 }  // namespace
@@ -556,6 +492,6 @@ extern "C" int cudalm_paged_prefill(const cudalm_paged_kv* kv, const cudalm_page
   a.least = p.least;
   a.window = window_of(q);
   a.sinks = sinks_of(q);
-  return kv->type == CUDALM_PAGED_BF16 ? launch_d<PagedBf16>(kv->head_dim, a, p.nq, stream)
-                                       : launch_d<PagedF16>(kv->head_dim, a, p.nq, stream);
+  return kv->type == CUDALM_PAGED_BF16 ? launch_d<PagedBf16>(kv->head_dim, a, stream)
+                                       : launch_d<PagedF16>(kv->head_dim, a, stream);
 }
