@@ -46,17 +46,17 @@ struct PrefillArgs {
 };
 
 // 16 bytes per lane from base (wave-uniform) + offset to LDS: lane i's land at
-// dst + 16 i. The compiler's builtin for it makes every later LDS read wait for
-// all such loads, the next tile's among them; here loads_landed() does the waiting.
-__device__ __forceinline__ void load_lds16(const uint16_t* base, uint32_t offset, uint16_t* dst) {
-  const uint32_t at = __builtin_amdgcn_readfirstlane(
-      static_cast<uint32_t>(reinterpret_cast<uintptr_t>(dst)));
+// dst + 16 i. Two loads at a time. The compiler's builtin for it makes every later
+// LDS read wait for all such loads, the next tile's among them; here loads_landed()
+// does the waiting.
+__device__ __forceinline__ void load_lds16(const uint16_t* base0, uint32_t offset0, uint32_t dst0,
+                                           const uint16_t* base1, uint32_t offset1, uint32_t dst1) {
   uint32_t saved;  // m0 holds the LDS address for the instruction
   asm volatile(
       "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\t"
-      "s_mov_b32 m0, %0"
+      "s_mov_b32 m0, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %5, %6\n\ts_mov_b32 m0, %0"
       : "=&s"(saved)
-      : "s"(at), "v"(offset), "s"(base)
+      : "s"(dst0), "v"(offset0), "s"(base0), "s"(dst1), "v"(offset1), "s"(base1)
       : "memory");
 }
 
@@ -67,8 +67,15 @@ __device__ __forceinline__ int swap_bits_2_3(int r) {
   return (r & ~12) | ((r & 4) << 1) | ((r & 8) >> 1);
 }
 
+// Key row r has chunk c at place c ^ chunk_exchange(r): 16 rows of 64 channels lie in
+// eight lines of 64 banks, two to a line, wider ones in one line or more each.
+template <int D>
+__device__ __forceinline__ int chunk_exchange(int r) {
+  return D == 64 ? (r >> 1) & 7 : r & 15;
+}
+
 template <typename T, int D>
-__global__ __launch_bounds__(64 * kWaves, 2) void paged_prefill_kernel(const PrefillArgs a) {
+__global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : D == 128 ? 3 : 4) void paged_prefill_kernel(const PrefillArgs a) {
   constexpr int KT = kTile, KK = D / 16, DT = D / 32;
   constexpr int C = D / 8;             // 16-byte chunks of a key row
   constexpr int kLoads = KT * D / 512; // 1 KB loads of a tile of keys (of values)
@@ -121,37 +128,63 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_prefill_kernel(const Pre
   const size_t page_elems = static_cast<size_t>(P) * D * a.kv.kv_heads;
   const size_t head_elems = static_cast<size_t>(P) * D * h;
   // A wave loads 1 KB pieces wave, wave + 4, .. of a tile's keys and values.
-  // Key row r of piece 4 x + wave is r0 + x kStep: its low three bits, and with them
-  // the exchange of its chunks, are the same for every x, and its token is that of r0
-  // plus a number that all lanes share. So one offset per lane serves all loads.
+  // Key row r of piece 4 x + wave is r0 + x kStep: its token is that of r0 plus a number
+  // that all lanes share, and the exchange of its chunks is the same for every x (but
+  // for chunk bit 3 where D = 256). So one or two offsets per lane serve all loads.
   constexpr int kStep = 2048 / D;
   const int r0 = wave * (512 / D) + lane / C;
-  const uint32_t k_lane = 2 * (swap_bits_2_3(r0) % 16 * D + 8 * ((lane % C) ^ (r0 & 7)));
+  const uint32_t k_lane =
+      2 * (swap_bits_2_3(r0) % 16 * D + 8 * ((lane % C) ^ chunk_exchange<D>(r0)));
   const int v_piece = wave * 64;  // in channels of the tile's groups of eight tokens
   const uint32_t v_lane = 16 * (v_piece % D + lane);
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)) + wave * 1024;
 
-  // A tile's place and its pages, of 16 tokens each; a bit for each absent one.
-  int t0 = 0, page0 = 0, page1 = 0;
-  uint32_t absent = 0;
-  auto look_up = [&](int i) {
-    t0 = tiles.tile(i) << kTileShift;
-    page0 = a.kv.uniform_page(b, t0 >> a.kv.page_shift);
-    page1 = a.kv.uniform_page(b, (t0 + 16) >> a.kv.page_shift);
-    absent = (page0 < 0) | (page1 < 0) << 1;
+  // every row from position `from` to `to` sees all of the tile at t
+  auto seen_whole = [&](int t, int from, int to) {
+    return t + KT - 1 <= from && (a.window <= 0 || t > to - a.window || t + KT - 1 < a.sinks);
   };
-  auto fetch = [&](int buf) {
+  const bool wg_full = row0 + kRows <= rows, wave_full = wave_row + 32 <= rows;
+  // Places, pages and visibility of the next 32 tiles: lanes 2 i and 2 i + 1 hold the
+  // halves of tile i, masks a bit each. One vector load of the table per 32 tiles,
+  // and no scalar load in the loop.
+  uint64_t half_at = 0;  // of the half's first key, and value, in its cache
+  uint64_t absent_bits = 0, whole_bits = 0, wg_whole_bits = 0;
+  int t0 = 0;
+  auto look_ahead = [&](int i) {
+    const int t = (tiles.tile(i + lane / 2) << kTileShift) + 16 * (lane & 1);
+    int page = -1;
+    if (i + lane / 2 < end) page = a.kv.page(b, t >> a.kv.page_shift);
     // absent pages are hidden below; any page will do
-    const size_t at0 = max(page0, 0) * page_elems + head_elems + static_cast<size_t>(t0 & (P - 1)) * D;
-    const size_t at1 =
-        max(page1, 0) * page_elems + head_elems + static_cast<size_t>((t0 + 16) & (P - 1)) * D;
-    uint16_t* kd = lds + buf * 2 * kTileElems + wave * 512;
-    uint16_t* vd = kd + kTileElems;
+    half_at = max(page, 0) * page_elems + head_elems + static_cast<uint64_t>(t & (P - 1)) * D;
+    absent_bits = __ballot(page < 0);
+    const int first_token = t - 16 * (lane & 1);
+    whole_bits = __ballot(wave_full && seen_whole(first_token, wave_first, wave_last));
+    wg_whole_bits = __ballot(wg_full && seen_whole(first_token, wg_first, wg_last));
+  };
+  auto half_place = [&](int x) {
+    return static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(half_at), x)) |
+           static_cast<uint64_t>(
+               static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(half_at >> 32), x)))
+               << 32;
+  };
+  uint32_t absent = 0;  // of the tile fetched last: a bit for each half
+  bool whole = false, wg_whole = false;
+  auto fetch = [&](int i, int buf) {
+    const int x = 2 * ((i - begin) & 31);
+    if (x == 0) look_ahead(i);
+    t0 = tiles.tile(i) << kTileShift;
+    absent = static_cast<uint32_t>(absent_bits >> x) & 3;
+    whole = !absent && ((whole_bits >> x) & 1);
+    wg_whole = !absent && ((wg_whole_bits >> x) & 1);
+    const uint64_t at0 = half_place(x), at1 = half_place(x + 1);
+    const uint32_t kd = lds0 + buf * 4 * kTileElems, vd = kd + 2 * kTileElems;
 #pragma unroll
-    for (int x = 0; x < kLoads / kWaves; ++x) {
+    for (int y = 0; y < kLoads / kWaves; ++y) {
       // rows of the piece: tokens of 16-token half r / 16, bit 3 of r is bit 2 of the token
-      const int r = x * kStep + wave * (512 / D), g = x * (2048 / (8 * D)) + v_piece / D;
-      load_lds16(a.k + (r & 16 ? at1 : at0) + (D == 256 ? (x & 1) * 4 * D : 0), k_lane, kd + x * 2048);
-      load_lds16(a.v + (g & 2 ? at1 : at0) + (g & 1) * 8 * D, v_lane, vd + x * 2048);
+      const int r = y * kStep + wave * (512 / D), g = y * (2048 / (8 * D)) + v_piece / D;
+      const bool odd = D == 256 && (y & 1);
+      load_lds16(a.k + (r & 16 ? at1 : at0) + (odd ? 4 * D : 0), odd ? k_lane ^ 128 : k_lane,
+                 kd + y * 4096, a.v + (g & 2 ? at1 : at0) + (g & 1) * 8 * D, v_lane, vd + y * 4096);
     }
   };
   // Zero weights times Inf or NaN are NaN. So in a tile that some row sees only
@@ -180,14 +213,25 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_prefill_kernel(const Pre
   };
 
   // One tile of keys and values against the wave's rows.
+  constexpr int kAhead = D == 256 ? 3 : 4;
   auto step = [&](bool whole, int t0, uint32_t absent, const uint16_t* kt, const uint16_t* vt) {
+    __builtin_amdgcn_s_setprio(1);
     f32x16_t s;
 #pragma unroll
     for (int e = 0; e < 16; ++e) s[e] = 0;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk)
-      s = T::mfma32(*reinterpret_cast<const u32x4_t*>(kt + n * D + 8 * ((2 * kk + half) ^ (n & 7))),
+      s = T::mfma32(*reinterpret_cast<const u32x4_t*>(
+                        kt + n * D + 8 * ((2 * kk + half) ^ chunk_exchange<D>(n))),
                     qf[kk], s);
+    __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+    for (int kk = 0; kk < KK - kAhead; ++kk) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+    __builtin_amdgcn_s_setprio(0);
     // s[e] is the score of token t0 + 16 (e / 8) + 8 half + e % 8
     if (!whole) {
       // token t is seen from p if 0 <= p - t < window, or if t is a sink up to p
@@ -218,6 +262,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_prefill_kernel(const Pre
     }
     u32x4_t pf[2];
     float sum = 0;
+    const u32x4_t* vp = reinterpret_cast<const u32x4_t*>(vt) + half * D + n;
+    constexpr int kFirst = D == 256 ? 3 : 1;  // value operands that load during the exponentials
+    u32x4_t vf[kFirst];
+#pragma unroll
+    for (int x = 0; x < kFirst; ++x) vf[x] = vp[(x / DT) * 2 * D + 32 * (x % DT)];
 #pragma unroll
     for (int e = 0; e < 16; e += 2) {
       const float p0 = exp2_fast(__builtin_fmaf(s[e], a.scale_log2, -m));
@@ -227,64 +276,60 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_prefill_kernel(const Pre
       pf[e / 8][e % 8 / 2] = T::pack(p0, p1);
     }
     l += sum;
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-    for (int y = 0; y < 2; ++y)
+    for (int x = 0; x < 2 * DT; ++x) {
+      const u32x4_t w = vf[x % kFirst];
+      if (x + kFirst < 2 * DT) vf[x % kFirst] = vp[((x + kFirst) / DT) * 2 * D + 32 * ((x + kFirst) % DT)];
+      o[x % DT] = T::mfma32(w, pf[x / DT], o[x % DT]);
+    }
+    if (D == 256) {
+      __builtin_amdgcn_sched_group_barrier(0x100, kFirst, 0);
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-        o[dt] = T::mfma32(
-            *reinterpret_cast<const u32x4_t*>(vt + ((2 * y + half) * D + 32 * dt + n) * 8), pf[y],
-            o[dt]);
+      for (int x = 0; x < 2 * DT - kFirst; ++x) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, kFirst, 0);
+    }
+    __builtin_amdgcn_s_setprio(0);
   };
 
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[dt][e] = 0;
-  // every row from position `from` to `to` sees all of the tile looked up
-  auto seen_whole = [&](int from, int to) {
-    return !absent && t0 + KT - 1 <= from &&
-           (a.window <= 0 || t0 > to - a.window || t0 + KT - 1 < a.sinks);
-  };
-  const bool wg_full = row0 + kRows <= rows, wave_full = wave_row + 32 <= rows;
   int buf = 0;
-  if (begin < end) {
-    look_up(begin);
-    fetch(0);
-  }
+  if (begin < end) fetch(begin, 0);
 #pragma unroll 1
   for (int i = begin; i < end; ++i) {
     uint16_t* kt = lds + buf * 2 * kTileElems;
     uint16_t* vt = kt + kTileElems;
     const int here = t0;
     const uint32_t gone = absent;
-    const bool whole = wave_full && seen_whole(wave_first, wave_last);
-    const bool wg_whole = wg_full && seen_whole(wg_first, wg_last);
+    const bool seen = whole, wg_seen = wg_whole;
     loads_landed();
     __syncthreads();  // this tile has landed for all waves; the other buffer is free
     buf ^= 1;
-    if (i + 1 < end) {
-      look_up(i + 1);
-      fetch(buf);
-    }
-    if (!wg_whole) {
+    if (i + 1 < end) fetch(i + 1, buf);
+    if (!wg_seen) {
       clean(reinterpret_cast<u32x4_t*>(vt), here, gone);
       __syncthreads();
     }
-    if (here <= wave_last) step(whole, here, gone, kt, vt);  // not above the wave's rows
+    if (here <= wave_last) step(seen, here, gone, kt, vt);  // not above the wave's rows
   }
-  // Inf or NaN for the sums of channels 32 dt .. whose rows see such a value in a
-  // tile that was cleaned of it: how many tokens hold +Inf or NaN, -Inf or NaN.
+  // Inf or NaN for the sums of channels 32 dt .. whose rows see such a value (in
+  // tiles that were not cleaned of it they have it already): how many tokens hold +Inf or NaN, -Inf or NaN.
   auto add_special = [&](f32x16_t& r, int dt) {
     f32x16_t up, down;
 #pragma unroll
     for (int e = 0; e < 16; ++e) up[e] = down[e] = 0;
 #pragma unroll 1
     for (int i = begin; i < end; ++i) {
-      look_up(i);
-      if (wg_full && seen_whole(wg_first, wg_last)) continue;
+      const int place = tiles.tile(i) << kTileShift;
 #pragma unroll 1
       for (int y = 0; y < KT / 16; ++y) {
-        const int t = t0 + 16 * y + 8 * half;
+        const int t = place + 16 * y + 8 * half;
         const int page = a.kv.page(b, t >> a.kv.page_shift);
         uint32_t seen = 0;
         u32x4_t w = {0, 0, 0, 0};
@@ -388,9 +433,9 @@ PrefillPlan plan_of(const cudalm_paged_kv* kv, const cudalm_paged_query* q, int 
                            (sinks_of(q) + kTile - 1) / kTile;
     tiles = near < tiles ? near : tiles;
   }
-  const long long groups = p.units * kv->kv_heads;
-  long long want = 2LL * cu_count() / groups;
+  const long long groups = (static_cast<long long>(tokens) * group + kRows - 1) / kRows * kv->kv_heads;
   const long long most = tiles / 4;
+  long long want = 2LL * cu_count() / groups;
   want = want < most ? want : most;
   want = want < 16 ? want : 16;
   p.splits = static_cast<int>(want < 1 ? 1 : want);
