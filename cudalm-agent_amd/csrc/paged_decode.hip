@@ -16,7 +16,13 @@
 // goes through LDS before the end.
 //
 // A workgroup of four waves takes RT tiles of 16 rows and 4 / RT slices of the
-// tokens of its split; slices are joined in LDS, splits by a second kernel.
+// tokens, which it joins in LDS. A call's tiles of 32 tokens, those of all
+// sequences and heads in a row, are cut into as many equal ranges as workgroups
+// run at once: sequences of any mix of lengths keep all of them busy to the end.
+// A range may end inside a sequence; such parts go to the workspace and a second
+// kernel joins them. Where parts of a tile per slice are too few to fill the chip,
+// every sequence gets as many workgroups as the longest needs, with no search for
+// the ranges' places.
 
 #include <cstdint>
 
@@ -28,332 +34,479 @@ namespace {
 constexpr int kTile = 32;      // tokens per step of a wave
 constexpr int kTileShift = 5;
 
+// (sequence, head, 64 rows) in this order are the segments of a call.
 struct DecodeArgs {
   PagedView kv;
   const uint16_t* k;
   const uint16_t* v;
   const uint16_t* q;
   void* out;
-  float* part_o;    // [bh][splits][rows][D], NULL: one split, straight to out
-  float* part_ml;   // [bh][splits][rows][2]
+  float* part_o;    // [parts][part_rows][D], part 2 w + x being workgroup w's ..
+  float* part_ml;   // [parts][part_rows][2] .. or, with fixed splits, w itself
   float* final_ml;  // [bh][rows][2] or NULL
   float* scores;    // [bh][rows][score_pitch] (times scale log2 e) or NULL
   long long token_stride, head_stride;
   float scale_log2;
-  int new_tokens, group, rows, splits, least, window, sinks, score_pitch;
+  int new_tokens, group, rows, zrows, part_rows, groups, splits, least, window, sinks, score_pitch;
+
+  __device__ __forceinline__ PagedTiles tiles_of(int length) const {
+    return PagedTiles(length, length - new_tokens, length - 1, window, sinks, kTileShift);
+  }
+  // Tiles of sequence b's segments; one where there are none, for its zeros.
+  __device__ __forceinline__ int count_of(int b) const {
+    const int n = tiles_of(kv.length(b)).count;
+    return n > 0 ? n : 1;
+  }
 };
 
-template <typename T, int D, int RT>
+// 16 bytes; `once`: nothing else of the call reads them, so the caches need not keep
+// them (64 sequences of up to 3000 tokens, 8 heads of 128: 103 us without, 93 with).
+template <bool once>
+__device__ __forceinline__ u32x4_t load_once(const uint16_t* p) {
+  const u32x4_t* q = reinterpret_cast<const u32x4_t*>(p);
+  return once ? __builtin_nontemporal_load(q) : *q;
+}
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Sum of v over the wave's lanes.
+__device__ __forceinline__ int wave_sum(int v) {
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) v += __shfl_xor(v, x);
+  return uniform(v);
+}
+
+// Where the segments lie in the row of all tiles (fewer than 2^31): 64 sequences at a
+// time, a lane each.
+struct Segments {
+  int block, base;  // first sequence of the 64, tiles before it
+  int count, end;   // this lane's sequence: tiles of a segment, end of its last one
+
+  // Tiles of sequences 0 .. batch - 1.
+  static __device__ __forceinline__ int total(const DecodeArgs& a, int batch, int lane) {
+    int all = 0;
+    for (int b = lane; b < batch; b += 64) all += a.count_of(b);
+    return wave_sum(all) * a.kv.kv_heads * a.zrows;
+  }
+  __device__ __forceinline__ void load(const DecodeArgs& a, int lane) {
+    count = block + lane < a.kv.batch ? a.count_of(block + lane) : 0;
+    end = count * a.kv.kv_heads * a.zrows;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) {
+      const int o = __shfl_up(end, x);
+      if (lane >= x) end += o;
+    }
+  }
+  // The sequence of tile g (not before the block, and before the last), its tiles per
+  // segment and the place of its first one.
+  __device__ __forceinline__ int find(const DecodeArgs& a, int lane, int g, int* tiles, int* first) {
+    for (;;) {
+      const uint64_t after = __ballot(base + end > g);
+      if (after) {
+        const int x = __builtin_ctzll(after);
+        *tiles = __builtin_amdgcn_readlane(count, x);
+        *first = base + __builtin_amdgcn_readlane(end, x) - *tiles * a.kv.kv_heads * a.zrows;
+        return block + x;
+      }
+      base += __builtin_amdgcn_readlane(end, 63);
+      block += 64;
+      load(a, lane);
+    }
+  }
+};
+
+// Tiles per workgroup.
+__device__ __forceinline__ int tiles_per_group(const DecodeArgs& a, int total) {
+  const int r = uniform((total + a.groups - 1) / a.groups);
+  return r > a.least ? r : a.least;
+}
+
+// RANGES: equal ranges of all tiles, else fixed splits.
+template <typename T, int D, int RT, bool RANGES>
 __global__ __launch_bounds__(256, 2) void paged_decode_kernel(const DecodeArgs a) {
   constexpr int KK = D / 32, DT = D / 16, SL = 4 / RT;
   constexpr int kPitch = D + 4;
-  __shared__ float obuf[2][16 * kPitch];
+  // Each wave's queries in the order of its operands (registers are for what is on
+  // its way from memory), later the sums of two waves.
+  union Shared {
+    u32x4_t q[4][KK][64];
+    float o[2][16 * kPitch];
+  };
+  __shared__ Shared shared;
   __shared__ float mlbuf[4][2][16];
+  __shared__ uint32_t badbuf[4];
   const int wave = wave_id(), lane = threadIdx.x & 63;
   const int n = lane & 15, quarter = lane >> 4;
   const int rt = wave % RT, slice = wave / RT;
 
-  int id = blockIdx.x;
-  const int split = id % a.splits;
-  id /= a.splits;
-  const int bh = id % (a.kv.batch * a.kv.kv_heads), zr = id / (a.kv.batch * a.kv.kv_heads);
-  const int b = bh / a.kv.kv_heads, h = bh % a.kv.kv_heads;
-
-  const int length = a.kv.uniform_length(b), first = length - a.new_tokens;
-  const PagedTiles tiles(length, first, length - 1, a.window, a.sinks, kTileShift);
-  const int per = tiles_per_split(tiles.count, a.splits, a.least, SL);
-  const int begin = split * per, end = begin + per < tiles.count ? begin + per : tiles.count;
-  if (a.part_o && begin >= end) return;  // the join knows how many splits there are
-
-  // this lane's row
-  const int row = (zr * RT + rt) * 16 + n;
-  const bool real = row < a.rows;
-  const int j = row / a.group;
-  const int pos = real ? first + j : -1;
-
-  u32x4_t qf[KK];
-  {
-    const uint16_t* qp = a.q +
-                         (static_cast<long long>(b) * a.new_tokens + (real ? j : 0)) * a.token_stride +
-                         (static_cast<long long>(h) * a.group + (real ? row - j * a.group : 0)) *
-                             a.head_stride +
-                         8 * quarter;
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      qf[kk] = *reinterpret_cast<const u32x4_t*>(qp + 32 * kk);
-      if (!real) qf[kk] = u32x4_t{0, 0, 0, 0};
-    }
-  }
-
-  f32x4_t o[DT];
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4_t{0, 0, 0, 0};
-  float m = kLowest, l = 0;
-
   const int P = 1 << a.kv.page_shift;
   const size_t page_elems = (static_cast<size_t>(P) * D) * a.kv.kv_heads;
-  const size_t head_elems = static_cast<size_t>(P) * D * h;
   const int ktok = 8 * (n >> 2) + (n & 3);  // token of K row n in half 0
-  u32x4_t kf[2][KK], vf[DT];
 
-  // The pages of a tile's two halves, and whether every row sees all of it.
-  int t0 = 0, pa = -1, pb = -1;
-  auto look_up = [&](int i) {
-    t0 = tiles.tile(i) << kTileShift;
-    pa = a.kv.uniform_page(b, t0 >> a.kv.page_shift);
-    pb = a.kv.uniform_page(b, (t0 + 16) >> a.kv.page_shift);
-    return pa >= 0 && pb >= 0 && t0 + kTile - 1 <= first &&
-           (a.window <= 0 || t0 > length - 1 - a.window || t0 + kTile - 1 < a.sinks);
-  };
-  auto load_k = [&]() {
-    const int pg = n < 8 ? pa : pb;
-    const uint16_t* kp = a.k + (pg < 0 ? 0 : pg) * page_elems + head_elems +
-                         static_cast<size_t>((t0 + ktok) & (P - 1)) * D + 8 * quarter;
+  // tiles [begin, end) of a segment with `all` of them; `slot` of the workspace
+  auto part = [&](int b, int hz, int begin, int end, int all, int slot) {
+    const int h = hz / a.zrows, zr = hz % a.zrows;
+    const int length = a.kv.uniform_length(b), first = length - a.new_tokens;
+    const PagedTiles tiles = a.tiles_of(length);
+    // this lane's row
+    const int row = (zr * RT + rt) * 16 + n;
+    const bool real = row < a.rows;
+    const int j = row / a.group;
+    const int pos = real ? first + j : -1;
+    {
+      const uint16_t* qp =
+          a.q +
+          (static_cast<long long>(b) * a.new_tokens + (real ? j : 0)) * a.token_stride +
+          (static_cast<long long>(h) * a.group + (real ? row - j * a.group : 0)) * a.head_stride +
+          8 * quarter;
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk)
-#pragma unroll
-      for (int f = 0; f < 2; ++f)
-        kf[f][kk] = *reinterpret_cast<const u32x4_t*>(kp + 4 * f * D + 32 * kk);
-  };
-  auto load_v = [&]() {
-    const int pg = quarter < 2 ? pa : pb;
-    const uint16_t* vp = a.v + (pg < 0 ? 0 : pg) * page_elems + head_elems +
-                         static_cast<size_t>((t0 + 8 * quarter) & (P - 1)) * D + 8 * n;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) vf[dt] = *reinterpret_cast<const u32x4_t*>(vp + 128 * dt);
-  };
-  float t[8];  // this lane's scores: its row, tokens 8 quarter .. 8 quarter + 7
-  auto scores = [&]() {
-    f32x4_t s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      s0 = T::mfma(kf[0][kk], qf[kk], s0);
-      s1 = T::mfma(kf[1][kk], qf[kk], s1);
+      for (int kk = 0; kk < KK; ++kk) {
+        u32x4_t v = *reinterpret_cast<const u32x4_t*>(qp + 32 * kk);
+        if (!real) v = u32x4_t{0, 0, 0, 0};
+        shared.q[wave][kk][lane] = v;
+      }
+      wave_lds_sync();
     }
+    const size_t head_elems = static_cast<size_t>(P) * D * h;
+    f32x4_t o[DT];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      t[e] = s0[e] * a.scale_log2;
-      t[4 + e] = s1[e] * a.scale_log2;
+    for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4_t{0, 0, 0, 0};
+    float m = kLowest, l = 0;
+    uint32_t bad = 0;
+    u32x4_t kf[2][KK], vf[DT];
+
+    // The next 32 tiles of this wave: lanes 2 i and 2 i + 1 hold the halves of tile i.
+    int tile = 0;            // first token
+    uint64_t half_at = 0;    // of the half's first key, and value, in its cache
+    auto place = [&](int x) {
+      return static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(half_at), x)) |
+             static_cast<uint64_t>(static_cast<uint32_t>(
+                 __builtin_amdgcn_readlane(static_cast<uint32_t>(half_at >> 32), x)))
+                 << 32;
+    };
+    auto load_k = [&](int x) {
+      const uint64_t at0 = place(x), at1 = place(x + 1), at = n < 8 ? at0 : at1;
+      const uint16_t* kp = a.k + at + static_cast<uint32_t>((ktok & 15) * D + 8 * quarter);
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+        for (int f = 0; f < 2; ++f)
+          kf[f][kk] = load_once<RT == 1>(kp + 4 * f * D + 32 * kk);
+    };
+    auto load_v = [&](int x) {
+      const uint64_t at0 = place(x), at1 = place(x + 1), at = quarter < 2 ? at0 : at1;
+      const uint16_t* vp = a.v + at + static_cast<uint32_t>(8 * (quarter & 1) * D + 8 * n);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) vf[dt] = load_once<RT == 1>(vp + 128 * dt);
+    };
+    float t[8];  // this lane's scores: its row, tokens 8 quarter .. 8 quarter + 7
+    auto scores = [&]() {
+      f32x4_t s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
+      asm volatile("" ::: "memory");  // the queries stay in LDS between tiles
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        const u32x4_t qf = shared.q[wave][kk][lane];
+        s0 = T::mfma(kf[0][kk], qf, s0);
+        s1 = T::mfma(kf[1][kk], qf, s1);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        t[e] = s0[e] * a.scale_log2;
+        t[4 + e] = s1[e] * a.scale_log2;
+      }
+    };
+    auto keep_scores = [&](int t0) {
+      if (!a.scores || !real || t0 + kTile > a.score_pitch) return;
+      float* sp = a.scores +
+                  (static_cast<size_t>(b * a.kv.kv_heads + h) * a.rows + row) * a.score_pitch + t0 +
+                  8 * quarter;
+      *reinterpret_cast<f32x4_t*>(sp) = f32x4_t{t[0], t[1], t[2], t[3]};
+      *reinterpret_cast<f32x4_t*>(sp + 4) = f32x4_t{t[4], t[5], t[6], t[7]};
+    };
+    u32x4_t pf;
+    auto softmax = [&]() {
+      float top = t[0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) top = fmaxf(top, t[e]);
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      // The maximum may lag by up to 2^8: weights stay below 256, which neither
+      // fp32 sums nor 16-bit weights mind, and most tiles rescale nothing.
+      if (__any(top > m + 8.0f)) {
+        const float next = fmaxf(m, top), r = exp2_fast(m - next);
+        l *= r;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt] *= r;
+        m = next;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float p0 = exp2_fast(t[e] - m), p1 = exp2_fast(t[e + 1] - m);
+        l += p0 + p1;
+        // The weights are rounded to the values' type, as the matrix unit takes
+        // them; their sum l is that of the unrounded ones.
+        pf[e / 2] = T::pack(p0, p1);
+      }
+    };
+
+#pragma unroll 1
+    for (int c = begin + slice; c < end; c += 32 * SL) {
+      const int mine = c + SL * (lane >> 1);
+      tile = tiles.tile(mine) << kTileShift;
+      const int half_t = tile + 16 * (lane & 1);
+      int page = -1;
+      if (mine < end) page = a.kv.page(b, half_t >> a.kv.page_shift);
+      half_at = static_cast<uint64_t>(page < 0 ? 0 : page) * page_elems + head_elems +
+                static_cast<uint64_t>(half_t & (P - 1)) * D;
+      const uint64_t here = __ballot(page >= 0);
+      const int last = (end - c + SL - 1) / SL < 32 ? (end - c + SL - 1) / SL : 32;
+      // The next tile's keys load while this one's weights are made, its values
+      // while the scores are. Every tile is masked, and Inf and NaN taken out of its
+      // values: a wave has far more time per tile than that takes (below).
+      load_k(0);
+#pragma unroll 1
+      for (int x = 0; x < last; ++x) {
+        load_v(2 * x);
+        const int t0 = __builtin_amdgcn_readlane(tile, 2 * x);
+        scores();
+        if (x + 1 < last) load_k(2 * x + 2);
+        const bool has = (here >> (2 * x + (quarter >> 1))) & 1;
+        uint32_t sees = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const bool one = has && paged_sees(t0 + 8 * quarter + e, pos, a.window, a.sinks);
+          sees |= one ? 1u << e : 0u;
+          t[e] = one ? t[e] : -__builtin_inff();
+        }
+        keep_scores(t0);
+        softmax();
+        // Zero weights times Inf or NaN are NaN: values of tokens that no row here
+        // sees, which may be anything, are cleared, and Inf and NaN taken out of the
+        // others; the rows that do see those get them at the end.
+        uint32_t some = sees;
+#pragma unroll
+        for (int y = 1; y < 16; y <<= 1) some |= __shfl_xor(static_cast<int>(some), y);
+        uint32_t keep[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          keep[w] = ((some >> (2 * w)) & 1 ? 0xFFFFu : 0u) | ((some >> (2 * w + 1)) & 1 ? 0xFFFF0000u : 0u);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) vf[dt][w] &= keep[w];
+          bad |= special_bits<T>(vf[dt]);
+          o[dt] = T::mfma(finite_part<T>(vf[dt]), pf, o[dt]);
+        }
+      }
     }
-  };
-  auto keep_scores = [&](int tile0) {
-    if (!a.scores || !real || tile0 + kTile > a.score_pitch) return;
-    float* sp = a.scores + (static_cast<size_t>(bh) * a.rows + row) * a.score_pitch + tile0 +
-                8 * quarter;
-    *reinterpret_cast<f32x4_t*>(sp) = f32x4_t{t[0], t[1], t[2], t[3]};
-    *reinterpret_cast<f32x4_t*>(sp + 4) = f32x4_t{t[4], t[5], t[6], t[7]};
-  };
-  u32x4_t pf;
-  auto softmax = [&]() {
-    float top = t[0];
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    // join the slices: the upper half of the waves hands its sums down
+    if (SL > 1) {
+      if (quarter == 0) mlbuf[wave][0][n] = m, mlbuf[wave][1][n] = l;
+      badbuf[wave] = __any(bad != 0);
+      __syncthreads();
+      float top = m;
 #pragma unroll
-    for (int e = 1; e < 8; ++e) top = fmaxf(top, t[e]);
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
-    // The maximum may lag by up to 2^8: weights stay below 256, which neither
-    // fp32 sums nor 16-bit weights mind, and most tiles rescale nothing.
-    if (__any(top > m + 8.0f)) {
-      const float next = fmaxf(m, top), r = exp2_fast(m - next);
-      l *= r;
+      for (int s = 0; s < SL; ++s) top = fmaxf(top, mlbuf[s * RT + rt][0][n]);
+      l = 0;
+#pragma unroll
+      for (int s = 0; s < SL; ++s)
+        l += mlbuf[s * RT + rt][1][n] * exp2_fast(mlbuf[s * RT + rt][0][n] - top);
+      const float r = exp2_fast(m - top);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) o[dt] *= r;
-      m = next;
-    }
+      m = top;
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      const float p0 = exp2_fast(t[e] - m), p1 = exp2_fast(t[e + 1] - m);
-      l += p0 + p1;
-      // The weights are rounded to the values' type, as the matrix unit takes
-      // them; their sum l is that of the unrounded ones.
-      pf[e / 2] = T::pack(p0, p1);
+      for (int half = SL / 2; half > 0; half >>= 1) {
+        if (slice >= half && slice < 2 * half) {
+          float* p = shared.o[(slice - half) * RT + rt] + n * kPitch + 4 * quarter;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4_t*>(p + 16 * dt) = o[dt];
+        }
+        __syncthreads();
+        if (slice < half) {
+          const float* p = shared.o[slice * RT + rt] + n * kPitch + 4 * quarter;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) o[dt] += *reinterpret_cast<const f32x4_t*>(p + 16 * dt);
+        }
+        __syncthreads();
+      }
+    }
+    // to the workspace, or the output if the segment is all here
+    const bool whole = begin == 0 && end == all;
+    const int heads = a.group * a.kv.kv_heads;
+    float* part_o = nullptr;
+    uint16_t* out = nullptr;
+    if (whole) {
+      const size_t to = (static_cast<size_t>(b) * a.new_tokens + j) * heads + h * a.group + row - j * a.group;
+      out = static_cast<uint16_t*>(a.out) + to * D + 4 * quarter;
+    } else {
+      part_o = a.part_o + (static_cast<size_t>(slot) * a.part_rows + rt * 16 + n) * D + 4 * quarter;
+    }
+    if (slice == 0 && real) {
+      if (!whole) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4_t*>(part_o + 16 * dt) = o[dt];
+        if (quarter == 0) {
+          float* ml = a.part_ml + 2 * (static_cast<size_t>(slot) * a.part_rows + rt * 16 + n);
+          ml[0] = m, ml[1] = l;
+        }
+      } else {
+        if (a.final_ml && quarter == 0) {
+          float* ml = a.final_ml + 2 * (static_cast<size_t>(b * a.kv.kv_heads + h) * a.rows + row);
+          ml[0] = m, ml[1] = l;
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+          *reinterpret_cast<u32x2_t*>(out + 16 * dt) = u32x2_t{
+              T::pack(o[dt][0] * inv, o[dt][1] * inv), T::pack(o[dt][2] * inv, o[dt][3] * inv)};
+      }
+    }
+    // Inf and NaN that were taken out, for the rows that see them: one wave after the
+    // other adds Inf or -Inf to the sums.
+    const uint32_t any_bad = SL > 1 ? badbuf[0] | badbuf[1] | badbuf[2] | badbuf[3] : __any(bad != 0);
+    if (any_bad) {
+#pragma unroll 1
+      for (int turn = 0; turn < SL; ++turn) {
+        if (SL > 1) __syncthreads();
+        if (turn != slice || !__any(bad != 0)) continue;
+#pragma unroll 1
+        for (int dt = 0; dt < DT; ++dt) {
+          // how many tokens that a row sees hold +Inf or NaN, -Inf or NaN
+          f32x4_t up = {0, 0, 0, 0}, down = {0, 0, 0, 0};
+#pragma unroll 1
+          for (int i = begin + slice; i < end; i += SL) {
+            const int t0 = (tiles.tile(i) << kTileShift) + 8 * quarter;
+            const int page = a.kv.page(b, t0 >> a.kv.page_shift);
+            uint32_t sees = 0;
+            u32x4_t v = {0, 0, 0, 0};
+            if (page >= 0) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                sees |= paged_sees(t0 + e, pos, a.window, a.sinks) ? 1u << e : 0u;
+              v = *reinterpret_cast<const u32x4_t*>(a.v + page * page_elems + head_elems +
+                                                    static_cast<size_t>(t0 & (P - 1)) * D + 8 * n +
+                                                    128 * dt);
+            }
+            const u32x4_t ones = seen_operand<T>(sees);
+            up = T::mfma(special_part<T>(v, ~0u), ones, up);
+            down = T::mfma(special_part<T>(v, 0), ones, down);
+          }
+          if (!real) continue;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float add = (up[e] > 0 ? __builtin_inff() : 0.0f) + (down[e] > 0 ? -__builtin_inff() : 0.0f);
+            if (whole)
+              out[16 * dt + e] = static_cast<uint16_t>(T::pack(T::value(out[16 * dt + e]) + add, 0.0f));
+            else
+              part_o[16 * dt + e] += add;
+          }
+        }
+      }
+      if (SL > 1) __syncthreads();
     }
   };
 
-  // Tiles that are seen whole: the next one's keys load while this one's
-  // weights are made, its values while the scores are.
-  int i = begin + slice;
-  while (i < end && !look_up(i)) i += SL;
-  if (i < end) load_k();
-  while (i < end) {
-    load_v();
-    const int tile0 = t0;
-    scores();
-    do i += SL;
-    while (i < end && !look_up(i));
-    if (i < end) load_k();
-    keep_scores(tile0);
-    softmax();
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[dt] = T::mfma(vf[dt], pf, o[dt]);
-  }
-  // The others: at the ends of the sequence, the window and the sinks, and
-  // where pages are absent.
+  const int per_seq = a.kv.kv_heads * a.zrows;
+  if constexpr (!RANGES) {
+    const int segment = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
+    const int b = segment / per_seq, all = uniform(a.count_of(b));
+    const int per = tiles_per_split(all, a.splits, a.least, 1);
+    const int begin = split * per, end = begin + per < all ? begin + per : all;
+    if (begin < end) part(b, segment % per_seq, begin, end, all, blockIdx.x);
+  } else {
+    const int total = Segments::total(a, a.kv.batch, lane), per = tiles_per_group(a, total);
+    if (blockIdx.x >= static_cast<unsigned>((total + per - 1) / per)) return;
+    int g = blockIdx.x * per;
+    const int stop = g + per < total ? g + per : total;
+    Segments segments = {};
+    segments.load(a, lane);
 #pragma unroll 1
-  for (i = begin + slice; i < end; i += SL) {
-    if (look_up(i)) continue;
-    load_k();
-    scores();
-    const bool has = (quarter < 2 ? pa : pb) >= 0;
-    uint32_t seen = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const bool sees = has && paged_sees(t0 + 8 * quarter + e, pos, a.window, a.sinks);
-      seen |= sees ? 1u << e : 0u;
-      t[e] = sees ? t[e] : -__builtin_inff();
+    while (g < stop) {
+      int all, start;
+      const int b = segments.find(a, lane, g, &all, &start);
+      const int hz = uniform((g - start) / all), begin = g - start - hz * all;
+      const int end = stop - g < all - begin ? begin + stop - g : all;
+      part(b, hz, begin, end, all, 2 * blockIdx.x + (begin == 0));
+      g += end - begin;
     }
-    keep_scores(t0);
-    softmax();
-    load_v();
-    // values of tokens that no row here sees may be anything: take them out
-    uint32_t some = seen, bad = 0;
-#pragma unroll
-    for (int x = 1; x < 16; x <<= 1) some |= __shfl_xor(static_cast<int>(some), x);
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-#pragma unroll
-      for (int w = 0; w < 4; ++w)
-        vf[dt][w] &= ((some >> (2 * w)) & 1 ? 0xFFFFu : 0u) |
-                     ((some >> (2 * w + 1)) & 1 ? 0xFFFF0000u : 0u);
-      bad |= special_bits<T>(vf[dt]);
-    }
-    if (__any(bad != 0)) {
-      const u32x4_t sees = seen_operand<T>(seen);
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        const f32x4_t up = T::mfma(special_part<T>(vf[dt], ~0u), sees, f32x4_t{0, 0, 0, 0});
-        const f32x4_t down = T::mfma(special_part<T>(vf[dt], 0), sees, f32x4_t{0, 0, 0, 0});
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          o[dt][e] += (up[e] > 0 ? __builtin_inff() : 0.0f) + (down[e] > 0 ? -__builtin_inff() : 0.0f);
-        vf[dt] = finite_part<T>(vf[dt]);
-        __builtin_amdgcn_sched_barrier(0);  // few registers over speed here
-      }
-    }
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[dt] = T::mfma(vf[dt], pf, o[dt]);
   }
-  l += __shfl_xor(l, 16);
-  l += __shfl_xor(l, 32);
-
-  // join the slices: the upper half of the waves hands its sums down
-  if (SL > 1) {
-    if (quarter == 0) mlbuf[wave][0][n] = m, mlbuf[wave][1][n] = l;
-    __syncthreads();
-    float all = m;
-#pragma unroll
-    for (int s = 0; s < SL; ++s) all = fmaxf(all, mlbuf[s * RT + rt][0][n]);
-    l = 0;
-#pragma unroll
-    for (int s = 0; s < SL; ++s)
-      l += mlbuf[s * RT + rt][1][n] * exp2_fast(mlbuf[s * RT + rt][0][n] - all);
-    const float r = exp2_fast(m - all);
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[dt] *= r;
-    m = all;
-#pragma unroll
-    for (int half = SL / 2; half > 0; half >>= 1) {
-      if (slice >= half && slice < 2 * half) {
-        float* p = obuf[(slice - half) * RT + rt] + n * kPitch + 4 * quarter;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4_t*>(p + 16 * dt) = o[dt];
-      }
-      __syncthreads();
-      if (slice < half) {
-        const float* p = obuf[slice * RT + rt] + n * kPitch + 4 * quarter;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[dt] += *reinterpret_cast<const f32x4_t*>(p + 16 * dt);
-      }
-      __syncthreads();
-    }
-    if (slice > 0) return;
-  }
-  if (!real) return;
-  if (a.part_o) {
-    const size_t at = (static_cast<size_t>(bh) * a.splits + split) * a.rows + row;
-    float* p = a.part_o + at * D + 4 * quarter;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4_t*>(p + 16 * dt) = o[dt];
-    if (quarter == 0) a.part_ml[2 * at] = m, a.part_ml[2 * at + 1] = l;
-    return;
-  }
-  if (a.final_ml && quarter == 0) {
-    const size_t at = static_cast<size_t>(bh) * a.rows + row;
-    a.final_ml[2 * at] = m;
-    a.final_ml[2 * at + 1] = l;
-  }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  const int heads = a.group * a.kv.kv_heads;
-  uint16_t* y = static_cast<uint16_t*>(a.out) +
-                ((static_cast<size_t>(b) * a.new_tokens + j) * heads + h * a.group + row - j * a.group) *
-                    D +
-                4 * quarter;
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
-    *reinterpret_cast<u32x2_t*>(y + 16 * dt) =
-        u32x2_t{T::pack(o[dt][0] * inv, o[dt][1] * inv), T::pack(o[dt][2] * inv, o[dt][3] * inv)};
 }
 
-// One workgroup per row: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s over
-// the splits of the row's sequence, a quarter of them per wave.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(const DecodeArgs a, int unit) {
-  constexpr int E = D / 64;
-  __shared__ float obuf[4][D];
-  __shared__ float lbuf[4];
+// CH x SW waves per row of a segment that has more than one part: out = sum_s
+// 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s. A wave takes 64 channels and every SW-th
+// part; D / 64 / CH workgroups make a row.
+template <typename T, int D, int CH, int SW>
+__global__ __launch_bounds__(64 * CH * SW) void paged_join_kernel(const DecodeArgs a) {
+  __shared__ float obuf[SW][64 * CH];
+  __shared__ float lbuf[SW];
   const int wave = wave_id(), lane = threadIdx.x & 63;
-  const int bh = blockIdx.x / a.rows, row = blockIdx.x % a.rows;
+  constexpr int kGroups = D / 64 / CH;
+  const int chunk = blockIdx.x % kGroups * CH + wave % CH, sw = wave / CH;
+  const int row = blockIdx.x / kGroups % a.rows, bh = blockIdx.x / kGroups / a.rows;
   const int b = bh / a.kv.kv_heads, h = bh % a.kv.kv_heads;
-  const int length = a.kv.uniform_length(b), first = length - a.new_tokens;
-  const PagedTiles tiles(length, first, length - 1, a.window, a.sinks, kTileShift);
-  const int per = tiles_per_split(tiles.count, a.splits, a.least, unit);
-  const int count = (tiles.count + per - 1) / per;
-  const size_t at = static_cast<size_t>(bh) * a.splits * a.rows + row;
-  const float* ml = a.part_ml + 2 * at;
+  const int all = a.count_of(b), zr = row / a.part_rows;
+  size_t slot0, slot1;  // of the first part and, less a step, of the others
+  int count, step;
+  if (a.splits) {
+    const int per = tiles_per_split(all, a.splits, a.least, 1);
+    count = (all + per - 1) / per;
+    slot0 = slot1 = (static_cast<size_t>(bh) * a.zrows + zr) * a.splits;
+    step = 1;
+  } else {
+    // workgroups w0 .. w1; their first parts, but for the first one's last
+    const int per = tiles_per_group(a, Segments::total(a, a.kv.batch, lane));
+    const int start = Segments::total(a, b, lane) + (h * a.zrows + zr) * all;
+    const int w0 = start / per, w1 = (start + all - 1) / per;
+    count = w1 - w0 + 1;
+    slot0 = 2 * static_cast<size_t>(w0) + 1;
+    slot1 = slot0 - 1;
+    step = 2;
+  }
+  if (count == 1) return;
+  auto at = [&](int s) {
+    return (s ? slot1 + static_cast<size_t>(s) * step : slot0) * a.part_rows + row - zr * a.part_rows;
+  };
   float M = kLowest;
-  for (int s = lane; s < count; s += 64) M = fmaxf(M, ml[2 * static_cast<size_t>(s) * a.rows]);
+  for (int s = lane; s < count; s += 64) M = fmaxf(M, a.part_ml[2 * at(s)]);
 #pragma unroll
   for (int x = 1; x < 64; x <<= 1) M = fmaxf(M, __shfl_xor(M, x));
-  float acc[E] = {}, l = 0;
-#pragma unroll 4
-  for (int s = wave; s < count; s += 4) {
-    const size_t r = static_cast<size_t>(s) * a.rows;
-    const float w = exp2_fast(ml[2 * r] - M);
-    l += w * ml[2 * r + 1];
-    const float* p = a.part_o + (at + r) * D + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] += w * p[e];
+  float acc = 0, l = 0;
+#pragma unroll 8
+  for (int s = sw; s < count; s += SW) {
+    const float w = exp2_fast(a.part_ml[2 * at(s)] - M);
+    l += w * a.part_ml[2 * at(s) + 1];
+    acc += w * a.part_o[at(s) * D + chunk * 64 + lane];
   }
+  if (SW > 1) {
+    obuf[sw][wave % CH * 64 + lane] = acc;
+    if (lane == 0 && wave % CH == 0) lbuf[sw] = l;
+    __syncthreads();
+    if (sw > 0) return;
+    acc = l = 0;
 #pragma unroll
-  for (int e = 0; e < E; ++e) obuf[wave][lane * E + e] = acc[e];
-  if (lane == 0) lbuf[wave] = l;
-  __syncthreads();
-  l = lbuf[0] + lbuf[1] + lbuf[2] + lbuf[3];
-  if (a.final_ml && threadIdx.x == 0) {
+    for (int w = 0; w < SW; ++w) acc += obuf[w][wave % CH * 64 + lane], l += lbuf[w];
+  }
+  if (a.final_ml && lane == 0 && chunk == 0) {
     const size_t f = static_cast<size_t>(bh) * a.rows + row;
     a.final_ml[2 * f] = M;
     a.final_ml[2 * f + 1] = l;
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const int j = row / a.group, heads = a.group * a.kv.kv_heads;
-  uint32_t* y = reinterpret_cast<uint32_t*>(a.out) +
-                ((static_cast<size_t>(b) * a.new_tokens + j) * heads + h * a.group + row - j * a.group) *
-                    (D / 2);
-  const int d = 2 * threadIdx.x;
-  if (d < D) {
-    float v[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-      v[e] = (obuf[0][d + e] + obuf[1][d + e] + (obuf[2][d + e] + obuf[3][d + e])) * inv;
-    y[threadIdx.x] = T::pack(v[0], v[1]);
-  }
+  uint16_t* y = static_cast<uint16_t*>(a.out) +
+                ((static_cast<size_t>(b) * a.new_tokens + j) * heads + h * a.group + row - j * a.group) * D;
+  y[chunk * 64 + lane] = static_cast<uint16_t>(T::pack(acc * inv, 0.0f));
 }
 
 // weights[t] (+)= sum over rows of 2^(score - M) / l.
 __global__ __launch_bounds__(256) void paged_weights_kernel(const DecodeArgs a, float* weights,
                                                             int add) {
   const int bh = blockIdx.y, b = bh / a.kv.kv_heads, h = bh % a.kv.kv_heads;
-  const int length = a.kv.uniform_length(b), first = length - a.new_tokens;
-  const PagedTiles tiles(length, first, length - 1, a.window, a.sinks, kTileShift);
+  const int length = a.kv.uniform_length(b);
+  const PagedTiles tiles = a.tiles_of(length);
   const int P = 1 << a.kv.page_shift;
   for (int t = blockIdx.x * 256 + threadIdx.x; t < length; t += gridDim.x * 256) {
     const int page = a.kv.page(b, t >> a.kv.page_shift);
@@ -376,10 +529,12 @@ __global__ __launch_bounds__(256) void paged_weights_kernel(const DecodeArgs a, 
   }
 }
 
-// How a call is cut: waves per row tile, splits, tiles a split takes at least.
+// How a call is cut.
 struct DecodePlan {
-  int rows, rt, zrows, splits, least, score_pitch;
+  int rows, rt, zrows, part_rows, groups, splits, least, score_pitch;
+  long long segments;
   size_t o_bytes, ml_bytes, final_bytes, score_bytes;
+  bool joins() const { return splits != 1; }
   size_t bytes() const { return o_bytes + ml_bytes + final_bytes + score_bytes; }
 };
 
@@ -389,6 +544,7 @@ DecodePlan plan_of(const cudalm_paged_kv* kv, const cudalm_paged_query* q, int n
   const int row_tiles = (p.rows + 15) / 16;
   p.rt = row_tiles > 2 ? 4 : row_tiles;
   p.zrows = (row_tiles + p.rt - 1) / p.rt;
+  p.part_rows = 16 * p.rt < p.rows ? 16 * p.rt : p.rows;
   const int len = expected_len(kv, q->max_len), window = window_of(q);
   long long tiles = (len + kTile - 1) / kTile;
   if (window > 0) {
@@ -396,39 +552,46 @@ DecodePlan plan_of(const cudalm_paged_kv* kv, const cudalm_paged_query* q, int n
                            (sinks_of(q) + kTile - 1) / kTile;
     tiles = near < tiles ? near : tiles;
   }
-  const int unit = 4 / p.rt;
-  const long long groups = static_cast<long long>(kv->batch) * kv->kv_heads * p.zrows;
-  const long long most = (tiles + unit - 1) / unit;
-  long long want = (8LL * cu_count() + groups - 1) / groups;
-  want = want < most ? want : most;
-  p.splits = static_cast<int>(want < 1 ? 1 : want);
-  p.least = static_cast<int>((tiles + p.splits - 1) / p.splits);
-  p.least = (p.least + unit - 1) / unit * unit;
-  p.splits = static_cast<int>((tiles + p.least - 1) / p.least);
-  if (p.splits < 1) p.splits = 1;
-  const size_t bh = static_cast<size_t>(kv->batch) * kv->kv_heads, parts = bh * p.splits * p.rows;
-  p.o_bytes = p.splits > 1 ? parts * kv->head_dim * 4 : 0;
-  p.ml_bytes = p.splits > 1 ? parts * 8 : 0;
+  const size_t bh = static_cast<size_t>(kv->batch) * kv->kv_heads;
+  p.segments = static_cast<long long>(bh) * p.zrows;
+  p.least = 4 / p.rt;  // a tile for each slice
+  const long long parts = (tiles + p.least - 1) / p.least;
+  const int at_once = (kv->head_dim == 64 ? 4 : 2) * cu_count();
+  size_t slots;
+  if (parts <= 1 || p.segments * parts <= at_once) {
+    p.splits = parts > 1 ? static_cast<int>(parts) : 1;
+    p.groups = 0;
+    slots = p.splits > 1 ? static_cast<size_t>(p.segments) * p.splits : 0;
+  } else {
+    p.splits = 0;
+    p.groups = at_once;
+    slots = 2 * static_cast<size_t>(at_once);
+  }
+  slots *= p.part_rows;
+  p.o_bytes = slots * kv->head_dim * 4;
+  p.ml_bytes = (slots * 8 + 15) / 16 * 16;
   p.score_pitch = mode ? (len + kTile - 1) / kTile * kTile : 0;
   p.final_bytes = mode ? (bh * p.rows * 8 + 15) / 16 * 16 : 0;
-  p.ml_bytes = (p.ml_bytes + 15) / 16 * 16;
   p.score_bytes = mode ? bh * p.rows * p.score_pitch * 4 : 0;
   return p;
 }
 
 template <typename T, int D>
 int launch(const DecodeArgs& a, const DecodePlan& p, hipStream_t stream) {
-  const unsigned grid = static_cast<unsigned>(static_cast<long long>(a.kv.batch) * a.kv.kv_heads *
-                                              p.zrows * p.splits);
-  if (p.rt == 1)
-    paged_decode_kernel<T, D, 1><<<grid, 256, 0, stream>>>(a);
-  else if (p.rt == 2)
-    paged_decode_kernel<T, D, 2><<<grid, 256, 0, stream>>>(a);
-  else
-    paged_decode_kernel<T, D, 4><<<grid, 256, 0, stream>>>(a);
-  if (p.splits > 1) {
+  const unsigned grid = p.groups ? p.groups : static_cast<unsigned>(p.segments * p.splits);
+  auto kernel = p.groups ? paged_decode_kernel<T, D, 1, true> : paged_decode_kernel<T, D, 1, false>;
+  if (p.rt == 2) kernel = p.groups ? paged_decode_kernel<T, D, 2, true> : paged_decode_kernel<T, D, 2, false>;
+  if (p.rt == 4) kernel = p.groups ? paged_decode_kernel<T, D, 4, true> : paged_decode_kernel<T, D, 4, false>;
+  kernel<<<grid, 256, 0, stream>>>(a);
+  if (p.joins()) {
     if (const int rc = launch_status()) return rc;
-    paged_join_kernel<T, D><<<a.kv.batch * a.kv.kv_heads * a.rows, 256, 0, stream>>>(a, 4 / p.rt);
+    const unsigned rows = static_cast<unsigned>(a.kv.batch * a.kv.kv_heads * a.rows);
+    // Few rows: all waves that help, a workgroup for 64 channels (one sequence of 32768
+    // tokens: 8 us, 16 with the other form); else one per row.
+    if (rows <= static_cast<unsigned>(cu_count()))
+      paged_join_kernel<T, D, 1, 16><<<rows * (D / 64), 1024, 0, stream>>>(a);
+    else
+      paged_join_kernel<T, D, D / 64, 1><<<rows, D, 0, stream>>>(a);
   }
   return launch_status();
 }
@@ -447,8 +610,11 @@ int check(const cudalm_paged_kv* kv, const cudalm_paged_query* q, int new_tokens
     return CUDALM_W4A16_EINVAL;
   const DecodePlan p = plan_of(kv, q, new_tokens, mode);
   const long long bh = static_cast<long long>(kv->batch) * kv->kv_heads;
-  if (bh * p.zrows * p.splits >= kMaxGemmTiles || bh * p.rows >= kMaxGemmTiles ||
-      (mode && bh > 65535))
+  // all tiles are numbered in 31 bits
+  const long long cap = (static_cast<long long>(kv->max_pages) * kv->page_size + kTile - 1) / kTile;
+  if (p.segments * (cap + 1) >= (1LL << 31)) return CUDALM_W4A16_ERANGE;
+  // the join's workgroups have up to 1024 threads
+  if (p.segments >= kMaxGemmTiles || bh * p.rows >= kMaxGemmTiles / 4 || (mode && bh > 65535))
     return CUDALM_W4A16_ERANGE;
   return CUDALM_W4A16_OK;
 }
@@ -457,13 +623,13 @@ int check(const cudalm_paged_kv* kv, const cudalm_paged_query* q, int new_tokens
 
 int paged_decode_regs(int type, int D) {
   if (type == CUDALM_PAGED_BF16)
-    return D == 64    ? regs_of(paged_decode_kernel<PagedBf16, 64, 1>)
-           : D == 128 ? regs_of(paged_decode_kernel<PagedBf16, 128, 1>)
-           : D == 256 ? regs_of(paged_decode_kernel<PagedBf16, 256, 1>)
+    return D == 64    ? regs_of(paged_decode_kernel<PagedBf16, 64, 1, true>)
+           : D == 128 ? regs_of(paged_decode_kernel<PagedBf16, 128, 1, true>)
+           : D == 256 ? regs_of(paged_decode_kernel<PagedBf16, 256, 1, true>)
                       : -1;
-  return D == 64    ? regs_of(paged_decode_kernel<PagedF16, 64, 1>)
-         : D == 128 ? regs_of(paged_decode_kernel<PagedF16, 128, 1>)
-         : D == 256 ? regs_of(paged_decode_kernel<PagedF16, 256, 1>)
+  return D == 64    ? regs_of(paged_decode_kernel<PagedF16, 64, 1, true>)
+         : D == 128 ? regs_of(paged_decode_kernel<PagedF16, 128, 1, true>)
+         : D == 256 ? regs_of(paged_decode_kernel<PagedF16, 256, 1, true>)
                     : -1;
 }
 
@@ -496,7 +662,7 @@ extern "C" int cudalm_paged_decode(const cudalm_paged_kv* kv, const cudalm_paged
   a.q = static_cast<const uint16_t*>(q->q);
   a.out = q->out;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  if (p.splits > 1) {
+  if (p.joins()) {
     a.part_o = reinterpret_cast<float*>(ws);
     a.part_ml = reinterpret_cast<float*>(ws + p.o_bytes);
   }
@@ -510,6 +676,9 @@ extern "C" int cudalm_paged_decode(const cudalm_paged_kv* kv, const cudalm_paged
   a.new_tokens = new_tokens;
   a.group = q->heads / kv->kv_heads;
   a.rows = p.rows;
+  a.zrows = p.zrows;
+  a.part_rows = p.part_rows;
+  a.groups = p.groups;
   a.splits = p.splits;
   a.least = p.least;
   a.window = window_of(q);

@@ -26,6 +26,7 @@ struct PagedBf16 {
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     return f32_to_bf16_rne2(lo, hi);
   }
+  static __device__ __forceinline__ float value(uint16_t x) { return bf16_lo(x); }
 };
 
 struct PagedF16 {
@@ -42,6 +43,9 @@ struct PagedF16 {
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(uint32_t, f16x2_t{static_cast<_Float16>(lo), static_cast<_Float16>(hi)});
+  }
+  static __device__ __forceinline__ float value(uint16_t x) {
+    return static_cast<float>(__builtin_bit_cast(_Float16, x));
   }
 };
 
