@@ -126,52 +126,81 @@ struct EvictArgs {
   int32_t* kept;      // [batch][kv_heads][keep]
   int32_t* new_lens;  // [batch]
   uint32_t* keys;     // [batch * kv_heads][pitch]
-  int dst_pages, keep, sinks, recent;
+  int dst_pages, keep, sinks, recent, lds_keys;
   long long pitch;
 };
 
-// A token's rank as a whole number: 0 absent, all ones the first and last
-// tokens that stay, else the order of the weights (NaN lowest, -0 as +0).
-__device__ __forceinline__ uint32_t evict_key(const EvictArgs& a, int b, int h, int t, int length) {
-  const int page = a.kv.page(b, t >> a.kv.page_shift);
-  if (page < 0) return 0;
-  const int s = a.sinks < a.keep ? a.sinks : a.keep;
-  const int r = a.recent < a.keep - s ? a.recent : a.keep - s;
-  if (t < s || t >= length - r) return 0xFFFFFFFFu;
-  const int P = 1 << a.kv.page_shift;
-  const float w =
-      a.weights[(static_cast<size_t>(page) * a.kv.kv_heads + h) * P + (t & (P - 1))] + 0.0f;
-  if (w != w) return 1;
-  const uint32_t u = __builtin_bit_cast(uint32_t, w);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+// A weight's rank as a whole number: NaN lowest (1), -0 as +0; 0 stands for absent
+// tokens, all ones for the first and last ones, which stay.
+__device__ __forceinline__ uint32_t weight_key(float w) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, w + 0.0f);
+  return w != w ? 1u : u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelect = 1024;  // threads of a selecting workgroup
+constexpr int kSelect = 1024;             // threads of a selecting workgroup
+constexpr int kSelectLdsKeys = 32 * 1024;  // keys that it holds in LDS at most
+constexpr int kSelectWords = 320;          // before the keys in LDS
 
-// One workgroup per (sequence, head): the key of the keep-th token in the order
-// of the keys, eight bits a pass over a histogram, then the kept positions in
-// order: each wave takes a sixteenth of the sequence, counts, and writes from
-// where the waves before it end. The keys are read (weights through the
-// tables) once and held in the workspace, which the passes find in the L2.
+// Adds 1 to hist[digit] for every lane with `in`: those that share the first one's
+// digit at once, since weights of one magnitude (or all zero) share their upper
+// digits, the others each.
+__device__ __forceinline__ void count_digit(uint32_t* hist, uint32_t digit, bool in) {
+  const uint64_t some = __ballot(in);
+  if (!some) return;
+  const int leader = __builtin_ctzll(some);
+  const bool same = in && digit == static_cast<uint32_t>(__builtin_amdgcn_readlane(digit, leader));
+  const uint64_t all = __ballot(same);
+  if (in && !same) atomicAdd(&hist[digit], 1u);
+  if ((threadIdx.x & 63) == static_cast<unsigned>(leader))
+    atomicAdd(&hist[digit], static_cast<uint32_t>(__popcll(all)));
+}
+
+// One workgroup per (sequence, head): the key of the keep-th token in the order of
+// the keys, eight bits a pass over a histogram, then the kept positions in order:
+// each wave takes a sixteenth of the sequence, counts, and writes from where the
+// waves before it end. The keys are made once (weights four at a time through the
+// tables) and held in LDS, those of longer sequences in the workspace.
 __global__ __launch_bounds__(kSelect) void paged_select_kernel(const EvictArgs a) {
-  __shared__ uint32_t hist[256];
-  __shared__ uint32_t found[2];  // digit, tokens with larger keys
-  __shared__ int above[kSelect / 64], equal[kSelect / 64];
+  extern __shared__ uint32_t select_lds[];
+  uint32_t* hist = select_lds;
+  uint32_t* found = hist + 256;  // digit, tokens with larger keys
+  uint32_t* above = found + 4;   // of each wave
+  uint32_t* equal = above + kSelect / 64;
+  static_assert(260 + 2 * (kSelect / 64) <= kSelectWords, "");
   const int bh = blockIdx.x, b = bh / a.kv.kv_heads, h = bh % a.kv.kv_heads;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int length = a.kv.length(b);
-  uint32_t* keys = a.keys + bh * a.pitch;
-  for (int t = tid; t < length; t += kSelect) keys[t] = evict_key(a, b, h, t, length);
+  uint32_t* keys = length <= a.lds_keys ? select_lds + kSelectWords : a.keys + bh * a.pitch;
+  const int s = a.sinks < a.keep ? a.sinks : a.keep;
+  const int r = a.recent < a.keep - s ? a.recent : a.keep - s;
+  const int P = 1 << a.kv.page_shift;
+#pragma unroll 4
+  for (int t = 4 * tid; t < length; t += 4 * kSelect) {
+    const int page = a.kv.page(b, t >> a.kv.page_shift);
+    typedef float f32x4_any_t __attribute__((ext_vector_type(4), aligned(4)));
+    const f32x4_any_t w = *reinterpret_cast<const f32x4_any_t*>(
+        a.weights + (static_cast<size_t>(page < 0 ? 0 : page) * a.kv.kv_heads + h) * P + (t & (P - 1)));
+    u32x4_t k = {weight_key(w[0]), weight_key(w[1]), weight_key(w[2]), weight_key(w[3])};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (t + i < s || t + i >= length - r) k[i] = 0xFFFFFFFFu;
+      if (page < 0) k[i] = 0;
+    }
+    *reinterpret_cast<u32x4_t*>(keys + t) = k;  // (both have room to a multiple of four)
+  }
   // Ranks from the largest: the keep-th, or the last where there are fewer.
   uint32_t prefix = 0, mask = 0;
   int left = a.keep;  // rank of the wanted key among those that match the prefix
-  __syncthreads();
   for (int shift = 24; shift >= 0; shift -= 8) {
     if (tid < 256) hist[tid] = 0;
     __syncthreads();
-    for (int t = tid; t < length; t += kSelect) {
-      const uint32_t k = keys[t];
-      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1u);
+    for (int t0 = 4 * (tid - lane); t0 < length; t0 += 4 * kSelect) {
+      const int t = t0 + 4 * lane;
+      u32x4_t k = {0, 0, 0, 0};
+      if (t < length) k = *reinterpret_cast<const u32x4_t*>(keys + t);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        count_digit(hist, (k[i] >> shift) & 255, t + i < length && (k[i] & mask) == prefix);
     }
     __syncthreads();
     if (tid < 64) {
@@ -203,7 +232,6 @@ __global__ __launch_bounds__(kSelect) void paged_select_kernel(const EvictArgs a
     prefix |= found[0] << shift;
     mask |= 255u << shift;
     left -= static_cast<int>(found[1]);
-    __syncthreads();
   }
   // tokens with larger keys stay, and the first `left` of those that have this
   // one (none with key 0: absent)
@@ -211,6 +239,7 @@ __global__ __launch_bounds__(kSelect) void paged_select_kernel(const EvictArgs a
   const int part = ((length + kSelect - 1) / kSelect) * 64;  // positions per wave
   const int t0 = wave * part, t1 = t0 + part < length ? t0 + part : length;
   int na = 0, ne = 0;
+#pragma unroll 4
   for (int t = t0; t < t1; t += 64) {
     const uint32_t k = t + lane < t1 ? keys[t + lane] : 0;
     na += __popcll(__ballot(k > key));
@@ -227,17 +256,18 @@ __global__ __launch_bounds__(kSelect) void paged_select_kernel(const EvictArgs a
   const int ties = left < alleq ? left : alleq;
   at += eq < ties ? eq : ties;
   int32_t* kept = a.kept + static_cast<size_t>(bh) * a.keep;
+#pragma unroll 4
   for (int t = t0; t < t1; t += 64) {
     const uint32_t k = t + lane < t1 ? keys[t + lane] : 0;
-    const unsigned long long e = __ballot(k == key && k != 0 && t + lane < t1);
-    const unsigned long long below = (1ull << lane) - 1;
+    const uint64_t e = __ballot(k == key && k != 0 && t + lane < t1);
+    const uint64_t below = (1ull << lane) - 1;
     const bool stays = k > key || (((e >> lane) & 1) && eq + __popcll(e & below) < ties);
-    const unsigned long long s = __ballot(stays);
+    const uint64_t st = __ballot(stays);
     if (stays) {
-      const int i = at + __popcll(s & below);
+      const int i = at + __popcll(st & below);
       if (i < a.keep) kept[i] = t + lane;
     }
-    at += __popcll(s);
+    at += __popcll(st);
     eq += __popcll(e);
   }
   const int count = all + ties < a.keep ? all + ties : a.keep;
@@ -245,57 +275,67 @@ __global__ __launch_bounds__(kSelect) void paged_select_kernel(const EvictArgs a
   if (h == 0 && tid == 0) a.new_lens[b] = count;
 }
 
-// One workgroup per eight kept tokens (one interleaved group of V in the fresh
-// page) of a (sequence, head).
+constexpr int kMove = 32;  // kept tokens of a copying workgroup
+
+// 32 kept tokens of a (sequence, head) per workgroup: their places first, a thread
+// each, so that the chain kept position, page, address is walked once for all; then
+// their key rows, and eight tokens' values of a channel per thread, one interleaved
+// unit of the fresh page. Bound by bytes: every line of the old values that holds a
+// kept token is read, which for a quarter kept is nine in ten.
 template <int D>
 __global__ __launch_bounds__(256) void paged_compact_kernel(const EvictArgs a) {
+  __shared__ long long src[kMove];  // place in the cache, in tokens; -1: none
+  __shared__ long long dst[kMove];
+  const int tid = threadIdx.x;
   const int bh = blockIdx.y, b = bh / a.kv.kv_heads, h = bh % a.kv.kv_heads;
-  const int i0 = blockIdx.x * 8;
+  const int i0 = blockIdx.x * kMove;
   const int P = 1 << a.kv.page_shift;
-  const int32_t* kept = a.kept + static_cast<size_t>(bh) * a.keep + i0;
-  const int most = a.keep - i0 < 8 ? a.keep - i0 : 8;
-  const int pi = i0 >> a.kv.page_shift;
-  if (pi >= a.dst_pages) return;
-  const int to = a.dst[static_cast<size_t>(b) * a.dst_pages + pi];
-  if (to < 0 || to >= a.kv.num_pages) return;
-  size_t src[8];  // token's place in the cache, in tokens
-  int n = 0;
-#pragma unroll
-  for (int t = 0; t < 8; ++t) {
-    const int pos = t < most ? kept[t] : -1;
-    if (pos < 0) continue;
-    const int page = a.kv.page(b, pos >> a.kv.page_shift);
-    src[t] = (static_cast<size_t>(page) * a.kv.kv_heads + h) * P + (pos & (P - 1));
-    n = t + 1;
-  }
-  if (n == 0) return;
-  const size_t dst = (static_cast<size_t>(to) * a.kv.kv_heads + h) * P + (i0 & (P - 1));
-#pragma unroll
-  for (int t = 0; t < 8; ++t) {
-    if (t >= n) break;
-    if (threadIdx.x == t) a.weights[dst + t] = a.weights[src[t]];
-    if (threadIdx.x / (D / 8) % 8 == t && threadIdx.x < D) {
-      const int c = threadIdx.x % (D / 8);
-      *reinterpret_cast<u32x4_t*>(a.ck + (dst + t) * D + 8 * c) =
-          *reinterpret_cast<const u32x4_t*>(a.ck + src[t] * D + 8 * c);
+  if (tid < kMove) {
+    const int i = i0 + tid, pos = i < a.keep ? a.kept[static_cast<size_t>(bh) * a.keep + i] : -1;
+    const int pi = i >> a.kv.page_shift;
+    const int to = pi < a.dst_pages ? a.dst[static_cast<size_t>(b) * a.dst_pages + pi] : -1;
+    const int from = pos >= 0 ? a.kv.page(b, pos >> a.kv.page_shift) : -1;
+    long long s = -1, d = -1;
+    if (from >= 0 && to >= 0 && to < a.kv.num_pages) {
+      s = (static_cast<long long>(from) * a.kv.kv_heads + h) * P + (pos & (P - 1));
+      d = (static_cast<long long>(to) * a.kv.kv_heads + h) * P + (i & (P - 1));
+      a.weights[d] = a.weights[s];
     }
+    src[tid] = s;
+    dst[tid] = d;
   }
-  const int d = threadIdx.x;
-  if (d >= D) return;
-  uint16_t x[8] = {};
+  __syncthreads();
+  constexpr int C = D / 8;
+#pragma unroll 4
+  for (int u = tid; u < kMove * C; u += 256) {
+    const int t = u / C, c = u % C;
+    const long long s = src[t];
+    if (s >= 0)
+      *reinterpret_cast<u32x4_t*>(a.ck + dst[t] * D + 8 * c) =
+          *reinterpret_cast<const u32x4_t*>(a.ck + s * D + 8 * c);
+  }
+#pragma unroll 4
+  for (int u = tid; u < kMove / 8 * D; u += 256) {
+    const int g = u / D * 8, d = u % D;
+    uint32_t x[8];
+    bool all = true;
 #pragma unroll
-  for (int t = 0; t < 8; ++t)
-    if (t < n) x[t] = a.cv[(src[t] & ~static_cast<size_t>(7)) * D + 8 * d + (src[t] & 7)];
-  uint16_t* cv = a.cv + dst * D + 8 * d;
-  if (n == 8) {
-    u32x4_t u;
+    for (int t = 0; t < 8; ++t) {
+      const long long s = src[g + t];
+      all = all && s >= 0;
+      x[t] = s >= 0 ? a.cv[(s & ~7LL) * D + 8 * d + (s & 7)] : 0;
+    }
+    if (all) {
+      u32x4_t w;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = x[2 * i] | (static_cast<uint32_t>(x[2 * i + 1]) << 16);
-    *reinterpret_cast<u32x4_t*>(cv) = u;
-  } else {
+      for (int i = 0; i < 4; ++i) w[i] = x[2 * i] | (x[2 * i + 1] << 16);
+      *reinterpret_cast<u32x4_t*>(a.cv + dst[g] * D + 8 * d) = w;
+    } else {
 #pragma unroll
-    for (int t = 0; t < 8; ++t)
-      if (t < n) cv[t] = x[t];
+      for (int t = 0; t < 8; ++t)
+        if (src[g + t] >= 0)
+          a.cv[(dst[g + t] & ~7LL) * D + 8 * d + t] = static_cast<uint16_t>(x[t]);
+    }
   }
 }
 
@@ -366,7 +406,7 @@ extern "C" int cudalm_paged_evict(const cudalm_paged_kv* kv, const int32_t* dst_
       !aligned(workspace, 16))
     return CUDALM_W4A16_EALIGN;
   const long long bh = static_cast<long long>(kv->batch) * kv->kv_heads;
-  const long long groups = (static_cast<long long>(keep) + 7) / 8;
+  const long long groups = (static_cast<long long>(keep) + kMove - 1) / kMove;
   if (workspace_bytes < cudalm_paged_evict_workspace_bytes(kv, max_len) || bh > 65535 ||
       groups * bh >= kMaxGemmTiles)
     return CUDALM_W4A16_ERANGE;
@@ -382,8 +422,13 @@ extern "C" int cudalm_paged_evict(const cudalm_paged_kv* kv, const int32_t* dst_
                  keep,
                  sinks,
                  recent,
+                 0,
                  static_cast<long long>(kv->max_pages) * kv->page_size};
-  paged_select_kernel<<<static_cast<unsigned>(bh), kSelect, 0, stream>>>(a);
+  const int expected = (expected_len(kv, max_len) + 3) / 4 * 4;
+  a.lds_keys = expected < kSelectLdsKeys ? expected : kSelectLdsKeys;
+  if (!allow_lds(paged_select_kernel, 4 * (kSelectWords + kSelectLdsKeys))) return CUDALM_W4A16_ELAUNCH;
+  paged_select_kernel<<<static_cast<unsigned>(bh), kSelect, 4 * (kSelectWords + a.lds_keys),
+                        stream>>>(a);
   if (const int rc = launch_status()) return rc;
   const dim3 grid(static_cast<unsigned>(groups), static_cast<unsigned>(bh));
   if (kv->head_dim == 64)
