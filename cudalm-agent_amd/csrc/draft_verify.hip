@@ -15,6 +15,7 @@ namespace {
 
 constexpr int kChunk = 4096;  // vocabulary entries per workgroup
 constexpr int kEach = kChunk / 256;
+constexpr int kSumGroups = 8;  // summing workgroups per CU that run at once
 constexpr int kMaxVocab = 1 << 22;  // 2^22 probabilities of at most 2^40 units: below 2^63
 
 struct VerifyArgs {
@@ -33,16 +34,26 @@ struct VerifyArgs {
 
 struct ProbF32 {
   typedef float type;
+  static __device__ __forceinline__ float of(u32x4_t v, int i) {
+    const uint32_t x = v[i];  // (a bit cast of the element itself takes element 0)
+    return __builtin_bit_cast(float, x);
+  }
   static __device__ __forceinline__ float value(float x) { return x; }
 };
 struct ProbBf16 {
   typedef uint16_t type;
+  static __device__ __forceinline__ float of(u32x4_t v, int i) {
+    return i & 1 ? bf16_hi(v[i / 2]) : bf16_lo(v[i / 2]);
+  }
   static __device__ __forceinline__ float value(uint16_t x) {
     return __builtin_bit_cast(float, static_cast<uint32_t>(x) << 16);
   }
 };
 struct ProbF16 {
   typedef uint16_t type;
+  static __device__ __forceinline__ float of(u32x4_t v, int i) {
+    return value(static_cast<uint16_t>(v[i / 2] >> (i & 1 ? 16 : 0)));
+  }
   static __device__ __forceinline__ float value(uint16_t x) {
     return static_cast<float>(__builtin_bit_cast(_Float16, x));
   }
@@ -101,8 +112,12 @@ struct Rows {
         one = a.tokens[static_cast<size_t>(b) * a.g + n];
     }
   }
+  // What the draft leaves of token v's probability pv.
+  __device__ __forceinline__ float left(int v, float pv, float qv) const {
+    return q ? pv - qv : v == one ? pv - 1.0f : pv;
+  }
   __device__ __forceinline__ float left(int v, float pv) const {
-    return q ? pv - P::value(q[v]) : v == one ? pv - 1.0f : pv;
+    return left(v, pv, q ? P::value(q[v]) : 0.0f);
   }
 };
 
@@ -129,37 +144,63 @@ __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* waves, uint
   return v;
 }
 
+// A sequence's chunks over gridDim.x workgroups, each of which finds the number of
+// accepted tokens for itself (a chain of three loads, so that no more workgroups are
+// launched than run at once).
 template <typename P>
 __global__ __launch_bounds__(256) void draft_sum_kernel(const VerifyArgs a) {
+  constexpr int V = 16 / sizeof(typename P::type);  // probabilities per load
   __shared__ int refused;
   __shared__ uint64_t waves[4];
-  const int b = blockIdx.y, v0 = blockIdx.x * kChunk + threadIdx.x;
+  const int b = blockIdx.y, tid = threadIdx.x;
   const int n = accepted_count<P>(a, b, &refused);
+  if (blockIdx.x == 0 && tid == 0) a.accepted[b] = n;
   const Rows<P> rows(a, b, n);
-  uint64_t rest = 0, whole = 0;
+  const bool wide = ((reinterpret_cast<uintptr_t>(rows.p) | reinterpret_cast<uintptr_t>(rows.q)) & 15) == 0;
+  for (int chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
+    uint64_t rest = 0, whole = 0;
+    if (wide && (chunk + 1) * kChunk <= a.vocab) {
+      const u32x4_t* pp = reinterpret_cast<const u32x4_t*>(rows.p) + chunk * (kChunk / V) + tid;
+      const u32x4_t* qp = reinterpret_cast<const u32x4_t*>(rows.q ? rows.q : rows.p) + chunk * (kChunk / V) + tid;
+      u32x4_t p[kEach / V], q[kEach / V];
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const int v = v0 + 256 * i;
-    if (v < a.vocab) {
-      const float p = P::value(rows.p[v]);
-      whole += units(p);
-      rest += units(rows.left(v, p));
+      for (int i = 0; i < kEach / V; ++i) {
+        p[i] = __builtin_nontemporal_load(pp + 256 * i);
+        q[i] = __builtin_nontemporal_load(qp + 256 * i);
+      }
+#pragma unroll
+      for (int i = 0; i < kEach / V; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float pv = P::of(p[i], e);
+          whole += units(pv);
+          rest += units(rows.left(chunk * kChunk + (256 * i + tid) * V + e, pv, P::of(q[i], e)));
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int v = chunk * kChunk + tid + 256 * i;
+        if (v < a.vocab) {
+          const float p = P::value(rows.p[v]);
+          whole += units(p);
+          rest += units(rows.left(v, p));
+        }
+      }
     }
+    uint64_t total;
+    block_scan(rest, waves, &total);
+    uint64_t* s = a.sums + 2 * (static_cast<size_t>(b) * a.chunks + chunk);
+    if (tid == 0) s[0] = total;
+    block_scan(whole, waves, &total);
+    if (tid == 0) s[1] = total;
   }
-  uint64_t total;
-  block_scan(rest, waves, &total);
-  uint64_t* s = a.sums + 2 * (static_cast<size_t>(b) * a.chunks + blockIdx.x);
-  if (threadIdx.x == 0) s[0] = total;
-  block_scan(whole, waves, &total);
-  if (threadIdx.x == 0) s[1] = total;
 }
 
 template <typename P>
 __global__ __launch_bounds__(256) void draft_pick_kernel(const VerifyArgs a) {
-  __shared__ int refused, chunk, token;
+  __shared__ int chunk, token;
   __shared__ uint64_t waves[4], before;
-  const int b = blockIdx.x, tid = threadIdx.x;
-  const int n = accepted_count<P>(a, b, &refused);
+  const int b = blockIdx.x, tid = threadIdx.x, n = a.accepted[b];
   const Rows<P> rows(a, b, n);
   const uint64_t* s = a.sums + 2 * static_cast<size_t>(b) * a.chunks;
   uint64_t c[2][4], sum[2] = {0, 0}, total[2];
@@ -205,12 +246,13 @@ __global__ __launch_bounds__(256) void draft_pick_kernel(const VerifyArgs a) {
   int32_t* out = a.out + static_cast<size_t>(b) * (a.g + 1);
   for (int i = tid; i <= a.g; i += 256)
     out[i] = i < n ? a.tokens[static_cast<size_t>(b) * a.g + i] : i == n ? token : -1;
-  if (tid == 0) a.accepted[b] = n;
 }
 
 template <typename P>
 int launch(const VerifyArgs& a, int batch, hipStream_t stream) {
-  draft_sum_kernel<P><<<dim3(a.chunks, batch), 256, 0, stream>>>(a);
+  const int at_once = kSumGroups * cu_count() / batch;
+  const int groups = at_once < 1 ? 1 : at_once < a.chunks ? at_once : a.chunks;
+  draft_sum_kernel<P><<<dim3(groups, batch), 256, 0, stream>>>(a);
   if (const int rc = launch_status()) return rc;
   draft_pick_kernel<P><<<batch, 256, 0, stream>>>(a);
   return launch_status();
