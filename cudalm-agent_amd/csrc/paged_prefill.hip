@@ -473,6 +473,7 @@ int check(const cudalm_paged_kv* kv, const cudalm_paged_query* q, int tokens) {
   if (tokens < 0) return CUDALM_W4A16_EINVAL;
   const long long rows = static_cast<long long>(tokens) * q->heads;
   if (rows >= (1LL << 26)) return CUDALM_W4A16_ERANGE;
+  if (tokens == 0) return CUDALM_W4A16_OK;
   const PrefillPlan p = plan_of(kv, q, tokens);
   if (p.units * kv->kv_heads * p.splits >= kMaxGemmTiles) return CUDALM_W4A16_ERANGE;
   return CUDALM_W4A16_OK;
@@ -497,7 +498,7 @@ using namespace cudalm_hip;
 
 extern "C" size_t cudalm_paged_prefill_workspace_bytes(const cudalm_paged_kv* kv,
                                                        const cudalm_paged_query* q, int tokens) {
-  if (check(kv, q, tokens) != CUDALM_W4A16_OK) return 0;
+  if (check(kv, q, tokens) != CUDALM_W4A16_OK || tokens == 0) return 0;
   return plan_of(kv, q, tokens).bytes();
 }
 

@@ -5,7 +5,7 @@ from __future__ import annotations
 import ctypes
 
 from . import _I, _P, _SZ, _check, _lib, _stream
-from .paged_kv import _workspace
+from .paged_kv import _devices, _workspace
 
 _L = ctypes.c_int64
 
@@ -28,14 +28,21 @@ def _need(ok, what):
         raise ValueError("draft: " + what)
 
 
-def _probs(p, B, rows, V, like, name):
+def _probs(p, B, rows, V, dtype, index, name):
     """Row stride of probabilities [B, rows, V]."""
     if rows == 0:
         return V
-    _need(tuple(p.shape) == (B, rows, V) and p.dtype == like.dtype and p.device == like.device and
-          p.stride(2) == 1 and (B == 1 or p.stride(0) == rows * p.stride(1)),
-          f"{name} is [{B}, {rows}, {V}] of the target's type, rows contiguous and equally spaced")
-    return p.stride(1) if rows > 1 or B == 1 else p.stride(0)
+    s = p.stride()
+    if (p.shape != (B, rows, V) or p.dtype != dtype or p.get_device() != index or s[2] != 1 or
+            (B != 1 and s[0] != rows * s[1])):
+        raise ValueError(f"draft: {name} is [{B}, {rows}, {V}] of the target's type and GPU, rows contiguous "
+                         "and equally spaced")
+    return s[1] if rows > 1 or B == 1 else s[0]
+
+
+def _plain(t, shape, dtype, index, name):
+    if t.shape != shape or t.dtype != dtype or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"draft: {name} is a contiguous {dtype} tensor {list(shape)} on the target's GPU")
 
 
 def verify(target, draft_probs, tokens, u_accept, u_next, counts=None, out=None, accepted=None,
@@ -51,38 +58,35 @@ def verify(target, draft_probs, tokens, u_accept, u_next, counts=None, out=None,
 
     if _types is None:
         _types = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-    _need(target.dim() == 3 and target.device.type == "cuda" and target.dtype in _types,
+    index, dtype = target.get_device(), target.dtype
+    _need(target.dim() == 3 and index >= 0 and dtype in _types,
           "target is [B, G + 1, V] in float32, bfloat16 or float16 on the GPU")
     B, G, V = target.shape
     G -= 1
-    device = target.device
     _need(B >= 1 and G >= 0 and V >= 1, "target has a row per drafted token and one more")
-    ts = _probs(target, B, G + 1, V, target, "target")
+    ts = _probs(target, B, G + 1, V, dtype, index, "target")
     ds, dp = 0, None
     if draft_probs is not None:
-        ds = _probs(draft_probs, B, G, V, target, "draft_probs")
+        ds = _probs(draft_probs, B, G, V, dtype, index, "draft_probs")
         dp = draft_probs.data_ptr()
-    for t, shape, dtype, name in ((tokens, (B, G), torch.int32, "tokens"),
-                                  (u_accept, (B, G), torch.float32, "u_accept"),
-                                  (u_next, (B,), torch.float32, "u_next")):
-        _need(tuple(t.shape) == shape and t.dtype == dtype and t.is_contiguous() and
-              t.device == device, f"{name} is a contiguous {dtype} tensor {list(shape)}")
+    _plain(tokens, (B, G), torch.int32, index, "tokens")
+    _plain(u_accept, (B, G), torch.float32, index, "u_accept")
+    _plain(u_next, (B,), torch.float32, index, "u_next")
     if counts is not None:
-        _need(tuple(counts.shape) == (B,) and counts.dtype == torch.int32 and
-              counts.is_contiguous() and counts.device == device,
-              "counts is a contiguous int32 tensor [B]")
+        _plain(counts, (B,), torch.int32, index, "counts")
     if out is None:
-        out = torch.empty(B, G + 1, dtype=torch.int32, device=device)
+        out = torch.empty(B, G + 1, dtype=torch.int32, device=_devices(index))
+    else:
+        _plain(out, (B, G + 1), torch.int32, index, "out")
     if accepted is None:
-        accepted = torch.empty(B, dtype=torch.int32, device=device)
-    for t, shape, name in ((out, (B, G + 1), "out"), (accepted, (B,), "accepted")):
-        _need(tuple(t.shape) == shape and t.dtype == torch.int32 and t.is_contiguous() and
-              t.device == device, f"{name} is a contiguous int32 tensor {list(shape)}")
+        accepted = torch.empty(B, dtype=torch.int32, device=_devices(index))
+    else:
+        _plain(accepted, (B,), torch.int32, index, "accepted")
     need = 0
     if workspace is None:
         need = _lib.cudalm_draft_verify_workspace_bytes(B, G, V)
-    at, size, held = _workspace(need, workspace, device, stream)
-    rc = _lib.cudalm_draft_verify(target.data_ptr(), ts, dp, ds, _types[target.dtype],
+    at, size, held = _workspace(need, workspace, index, stream)
+    rc = _lib.cudalm_draft_verify(target.data_ptr(), ts, dp, ds, _types[dtype],
                                   tokens.data_ptr(), None if counts is None else counts.data_ptr(),
                                   u_accept.data_ptr(), u_next.data_ptr(), out.data_ptr(),
                                   accepted.data_ptr(), B, G, V, at, size, _stream(stream))

@@ -22,6 +22,7 @@ counts): the work is split by it.
 from __future__ import annotations
 
 import ctypes
+import functools
 import struct
 
 from . import _I, _P, _SZ, _check, _lib, _stream
@@ -52,15 +53,20 @@ WEIGHTS_ADD = 2
 
 HEAD_DIMS = (64, 128, 256)
 
-_types = None
+_types = None  # torch's, once a call needs them
+
+
+def _load_types():
+    global _types, _int32_type, _float32_type
+    import torch
+
+    _types = {torch.bfloat16: BF16, torch.float16: F16}
+    _int32_type, _float32_type = torch.int32, torch.float32
 
 
 def _type_of(dtype) -> int:
-    global _types
     if _types is None:
-        import torch
-
-        _types = {torch.bfloat16: BF16, torch.float16: F16}
+        _load_types()
     try:
         return _types[dtype]
     except KeyError:
@@ -92,47 +98,58 @@ def _need(ok, what):
         raise ValueError("paged_kv: " + what)
 
 
-def _int32(t, shape, name, device):
-    import torch
+# The checks of a call are in its time (a decode step's small calls take about ten
+# microseconds): device indexes in place of device objects, sizes compared as
+# torch.Size, messages made where one is needed.
 
-    _need(t.dtype == torch.int32 and tuple(t.shape) == shape and t.is_contiguous() and
-          t.device == device, f"{name} is a contiguous int32 tensor {list(shape)} on {device}")
+def _bad_int32(name, shape):
+    raise ValueError(f"paged_kv: {name} is a contiguous int32 tensor {list(shape)} on the cache's GPU")
+
+
+def _int32(t, shape, name, index):
+    if t.shape != shape or t.dtype != _int32_type or t.get_device() != index or not t.is_contiguous():
+        _bad_int32(name, shape)
 
 
 def _cache(k, v, tables, lens, weights):
-    """struct cudalm_paged_kv of the tensors, as bytes."""
-    import torch
-
-    _need(k.dim() == 4 and v.dim() == 5 and tables.dim() == 2,
-          "k is [pages, kv_heads, page_size, D], v [pages, kv_heads, page_size / 8, D, 8], "
-          "tables [B, W]")
+    """(struct cudalm_paged_kv of the tensors as bytes, GPU index)."""
+    if _types is None:
+        _load_types()
+    if k.dim() != 4 or tables.dim() != 2:
+        raise ValueError("paged_kv: k is [pages, kv_heads, page_size, D], tables [B, W]")
     pages, heads, size, D = k.shape
-    _need(tuple(v.shape) == (pages, heads, size // 8, D, 8) and size % 8 == 0 and
-          v.dtype == k.dtype, "v does not match k")
-    _need(k.is_contiguous() and v.is_contiguous(), "k and v are contiguous")
-    device = k.device
-    _need(device.type == "cuda" and v.device == device, "k and v are on one GPU")
+    index = k.get_device()
+    dtype = k.dtype
+    kind = _types.get(dtype)
+    if kind is None:
+        _type_of(dtype)
+    if (v.shape != (pages, heads, size // 8, D, 8) or v.dtype != dtype or v.get_device() != index or
+            size % 8 or index < 0 or not k.is_contiguous() or not v.is_contiguous()):
+        raise ValueError("paged_kv: k and v are contiguous, of one type and on one GPU, v is [pages, "
+                         "kv_heads, page_size / 8, D, 8]")
     B, W = tables.shape
-    _int32(tables, (B, W), "tables", device)
-    _int32(lens, (B,), "lens", device)
+    if (tables.dtype != _int32_type or tables.get_device() != index or not tables.is_contiguous()):
+        _bad_int32("tables", (B, W))
+    _int32(lens, (B,), "lens", index)
     w = 0
     if weights is not None:
-        _need(weights.dtype == torch.float32 and tuple(weights.shape) == (pages, heads, size) and
-              weights.is_contiguous() and weights.device == device,
-              "weights is a contiguous float32 tensor [pages, kv_heads, page_size]")
+        if (weights.shape != (pages, heads, size) or weights.dtype != _float32_type or
+                weights.get_device() != index or not weights.is_contiguous()):
+            raise ValueError("paged_kv: weights is a contiguous float32 tensor [pages, kv_heads, "
+                             "page_size] on the cache's GPU")
         w = weights.data_ptr()
     return _pack_kv(k.data_ptr(), v.data_ptr(), w, tables.data_ptr(), lens.data_ptr(), pages, size,
-                    heads, D, _type_of(k.dtype), B, W)
+                    heads, D, kind, B, W), index
 
 
-def _rows(x, cols, heads, D, like, name):
-    """(token stride, head stride) of x, rows of [heads, D] over its leading dimensions."""
-    _need(x.dim() == cols + 2 and x.shape[-1] == D and x.dtype == like.dtype and
-          x.device == like.device and (heads is None or x.shape[-2] == heads),
-          f"{name} is {x.dtype} {list(x.shape)}, which does not match the cache")
-    s = x.stride()
-    _need(s[-1] == 1 and (cols == 1 or x.shape[0] == 1 or s[0] == x.shape[1] * s[1]),
-          f"{name}: heads are contiguous and tokens equally spaced")
+def _rows(x, cols, heads, like, index, name):
+    """(token stride, head stride) of x: rows of [heads, D] over its leading dimensions."""
+    shape, s = x.shape, x.stride()
+    if (len(shape) != cols + 2 or shape[-1] != like.shape[3] or x.dtype != like.dtype or
+            x.get_device() != index or (heads and shape[-2] != heads)):
+        raise ValueError(f"paged_kv: {name} ({x.dtype} {list(shape)} on {x.device}) does not match the cache")
+    if s[-1] != 1 or (cols == 2 and shape[0] != 1 and s[0] != shape[1] * s[1]):
+        raise ValueError(f"paged_kv: {name}: heads are contiguous and tokens equally spaced")
     return s[-3], s[-2]
 
 
@@ -142,32 +159,39 @@ def _query(q, out, token_stride, head_stride, scale, window, sinks, max_len):
                        D ** -0.5 if scale is None else scale, window, sinks, max_len or 0)
 
 
-def _workspace(nbytes, workspace, device, stream):
+def _workspace(nbytes, workspace, index, stream):
     """(address, bytes) of the caller's workspace or of a new one, with what holds it."""
-    import torch
-
     if workspace is not None:
-        _need(workspace.is_contiguous() and workspace.device == device,
-              "workspace is a contiguous tensor on the cache's GPU")
+        _need(workspace.is_contiguous() and workspace.get_device() == index,
+              "workspace is a contiguous tensor on the GPU of the call")
         return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
     if nbytes == 0:
         return None, 0, None
+    import torch
+
     if stream is None:
-        w = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        w = torch.empty(nbytes, dtype=torch.uint8, device=_devices(index))
     else:  # memory that is not handed out again before this stream has passed
         s = torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream
         with torch.cuda.stream(s):
-            w = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            w = torch.empty(nbytes, dtype=torch.uint8, device=_devices(index))
     return w.data_ptr(), nbytes, w
 
 
-def _out_like(q, out):
+@functools.lru_cache(maxsize=None)
+def _devices(index):
     import torch
 
+    return torch.device("cuda", index)
+
+
+def _out_like(q, out, index):
     if out is None:
+        import torch
+
         return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _need(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous() and
-          out.device == q.device, "out is contiguous and like q")
+    if out.shape != q.shape or out.dtype != q.dtype or out.get_device() != index or not out.is_contiguous():
+        raise ValueError("paged_kv: out is contiguous and like q")
     return out
 
 
@@ -192,15 +216,16 @@ def append(k_new, v_new, k, v, tables, lens, cu_new=None, weights=None, stream=N
     strides that are multiples of 8) into their pages, and zeros into their
     weights. Rows cu_new[b] .. cu_new[b + 1] - 1 are the last tokens of
     sequence b; without cu_new every sequence has T / B of them."""
-    kv = _cache(k, v, tables, lens, weights)
-    heads, D = k.shape[1], k.shape[3]
-    kt, kh = _rows(k_new, 1, heads, D, k, "k_new")
-    vt, vh = _rows(v_new, 1, heads, D, k, "v_new")
+    kv, index = _cache(k, v, tables, lens, weights)
+    heads = k.shape[1]
+    kt, kh = _rows(k_new, 1, heads, k, index, "k_new")
+    vt, vh = _rows(v_new, 1, heads, k, index, "v_new")
     T = k_new.shape[0]
-    _need(v_new.shape[0] == T, "k_new and v_new have one row per token")
+    if v_new.shape[0] != T:
+        raise ValueError("paged_kv: k_new and v_new have one row per token")
     cu = None
     if cu_new is not None:
-        _int32(cu_new, (tables.shape[0] + 1,), "cu_new", k.device)
+        _int32(cu_new, (tables.shape[0] + 1,), "cu_new", index)
         cu = cu_new.data_ptr()
     rc = _lib.cudalm_paged_append(kv, k_new.data_ptr(), v_new.data_ptr(), kt, kh, vt, vh, cu, T,
                                   _stream(stream))
@@ -216,19 +241,19 @@ def decode(q, k, v, tables, lens, scale=None, window: int = 0, sinks: int = 0, w
     first `sinks`. With weights, what every cached token received (summed over
     the new tokens and a group's query heads) is added to them, or, with
     accumulate=False, replaces them; max_len then has to hold."""
-    kv = _cache(k, v, tables, lens, weights)
-    D = k.shape[3]
+    kv, index = _cache(k, v, tables, lens, weights)
     one = q.dim() == 3
-    ts, hs = _rows(q, 1 if one else 2, None, D, k, "q")
-    _need(q.shape[0] == tables.shape[0], "q has one entry per sequence")
+    ts, hs = _rows(q, 1 if one else 2, None, k, index, "q")
+    if q.shape[0] != tables.shape[0]:
+        raise ValueError("paged_kv: q has one entry per sequence")
     Q = 1 if one else q.shape[1]
     mode = 0 if weights is None else WEIGHTS_ADD if accumulate else WEIGHTS_SET
-    out = _out_like(q, out)
+    out = _out_like(q, out, index)
     query = _query(q, out, ts, hs, scale, window, sinks, max_len)
     need = 0
     if workspace is None:
         need = _lib.cudalm_paged_decode_workspace_bytes(kv, query, Q, mode)
-    at, size, held = _workspace(need, workspace, k.device, stream)
+    at, size, held = _workspace(need, workspace, index, stream)
     rc = _lib.cudalm_paged_decode(kv, query, Q, mode, at, size, _stream(stream))
     _check(rc, "cudalm_paged_decode")
     return out
@@ -238,16 +263,16 @@ def prefill(q, cu_new, k, v, tables, lens, scale=None, window: int = 0, sinks: i
             out=None, workspace=None, stream=None):
     """Attention of a chunk: rows cu_new[b] .. cu_new[b + 1] - 1 of q [T, heads,
     D] are the last tokens of sequence b. Arguments as in decode()."""
-    kv = _cache(k, v, tables, lens, None)
-    ts, hs = _rows(q, 1, None, k.shape[3], k, "q")
-    _int32(cu_new, (tables.shape[0] + 1,), "cu_new", k.device)
+    kv, index = _cache(k, v, tables, lens, None)
+    ts, hs = _rows(q, 1, None, k, index, "q")
+    _int32(cu_new, (tables.shape[0] + 1,), "cu_new", index)
     T = q.shape[0]
-    out = _out_like(q, out)
+    out = _out_like(q, out, index)
     query = _query(q, out, ts, hs, scale, window, sinks, max_len)
     need = 0
     if workspace is None:
         need = _lib.cudalm_paged_prefill_workspace_bytes(kv, query, T)
-    at, size, held = _workspace(need, workspace, k.device, stream)
+    at, size, held = _workspace(need, workspace, index, stream)
     rc = _lib.cudalm_paged_prefill(kv, query, cu_new.data_ptr(), T, at, size, _stream(stream))
     _check(rc, "cudalm_paged_prefill")
     return out
@@ -263,21 +288,23 @@ def evict(k, v, tables, lens, weights, dst_tables, keep: int, sinks: int = 4, re
     import torch
 
     _need(weights is not None, "eviction goes by the weights")
-    kv = _cache(k, v, tables, lens, weights)
+    kv, index = _cache(k, v, tables, lens, weights)
     B, heads = tables.shape[0], k.shape[1]
     _need(dst_tables.dim() == 2, "dst_tables is [B, W']")
-    _int32(dst_tables, (B, dst_tables.shape[1]), "dst_tables", k.device)
+    _int32(dst_tables, (B, dst_tables.shape[1]), "dst_tables", index)
     _need(keep >= 1, "keep is at least 1")
     if kept is None:
-        kept = torch.empty(B, heads, keep, dtype=torch.int32, device=k.device)
-    _int32(kept, (B, heads, keep), "kept", k.device)
+        kept = torch.empty(B, heads, keep, dtype=torch.int32, device=_devices(index))
+    else:
+        _int32(kept, (B, heads, keep), "kept", index)
     if new_lens is None:
-        new_lens = torch.empty(B, dtype=torch.int32, device=k.device)
-    _int32(new_lens, (B,), "new_lens", k.device)
+        new_lens = torch.empty(B, dtype=torch.int32, device=_devices(index))
+    else:
+        _int32(new_lens, (B,), "new_lens", index)
     need = 0
     if workspace is None:
         need = _lib.cudalm_paged_evict_workspace_bytes(kv, max_len or 0)
-    at, size, held = _workspace(need, workspace, k.device, stream)
+    at, size, held = _workspace(need, workspace, index, stream)
     rc = _lib.cudalm_paged_evict(kv, dst_tables.data_ptr(), dst_tables.shape[1], keep, sinks, recent,
                                  kept.data_ptr(), new_lens.data_ptr(), max_len or 0, at, size,
                                  _stream(stream))
