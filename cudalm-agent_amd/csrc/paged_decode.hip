@@ -228,8 +228,7 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(const DecodeArgs a
       float top = t[0];
 #pragma unroll
       for (int e = 1; e < 8; ++e) top = fmaxf(top, t[e]);
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
+      top = max_across_32(max_across_16(top));
       // The maximum may lag by up to 2^8: weights stay below 256, which neither
       // fp32 sums nor 16-bit weights mind, and most tiles rescale nothing.
       if (__any(top > m + 8.0f)) {

@@ -99,6 +99,22 @@ __device__ __forceinline__ u32x4_t seen_operand(uint32_t seen) {
   return r;
 }
 
+// The larger of a lane's x and that of the lane 32 (16) away: one exchange of half
+// waves (of odd rows of 16 lanes with even ones) in the vector unit, where a
+// shuffle goes through the LDS.
+__device__ __forceinline__ float max_across_32(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const uint32_t a = r[0], b = r[1];
+  return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+__device__ __forceinline__ float max_across_16(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t a = r[0], b = r[1];
+  return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // A load that no store of the kernel changes, from a wave-uniform address.

@@ -249,7 +249,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : D == 128 ? 3 : 4) void 
     float top = s[0];
 #pragma unroll
     for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
-    top = fmaxf(top, __shfl_xor(top, 32)) * a.scale_log2;
+    top = max_across_32(top) * a.scale_log2;
     // The maximum may lag by up to 2^8 (as in the decode kernel).
     if (__any(top > m + 8.0f)) {
       const float next = fmaxf(m, top), r = exp2_fast(m - next);
