@@ -33,6 +33,7 @@ namespace {
 
 constexpr int kTile = 32;      // tokens per step of a wave
 constexpr int kTileShift = 5;
+constexpr int kMaxRows = 1024;  // new tokens x query heads of a key-value head
 
 // (sequence, head, 64 rows) in this order are the segments of a call.
 struct DecodeArgs {
@@ -82,10 +83,16 @@ struct Segments {
   int block, base;  // first sequence of the 64, tiles before it
   int count, end;   // this lane's sequence: tiles of a segment, end of its last one
 
-  // Tiles of sequences 0 .. batch - 1.
-  static __device__ __forceinline__ int total(const DecodeArgs& a, int batch, int lane) {
-    int all = 0;
-    for (int b = lane; b < batch; b += 64) all += a.count_of(b);
+  // Tiles of all sequences, and of those before sequence `to`.
+  static __device__ __forceinline__ int total(const DecodeArgs& a, int lane, int to = 0,
+                                              int* before = nullptr) {
+    int all = 0, some = 0;
+    for (int b = lane; b < a.kv.batch; b += 64) {
+      const int n = a.count_of(b);
+      all += n;
+      some += b < to ? n : 0;
+    }
+    if (before) *before = wave_sum(some) * a.kv.kv_heads * a.zrows;
     return wave_sum(all) * a.kv.kv_heads * a.zrows;
   }
   __device__ __forceinline__ void load(const DecodeArgs& a, int lane) {
@@ -416,7 +423,7 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(const DecodeArgs a
     const int begin = split * per, end = begin + per < all ? begin + per : all;
     if (begin < end) part(b, segment % per_seq, begin, end, all, blockIdx.x);
   } else {
-    const int total = Segments::total(a, a.kv.batch, lane), per = tiles_per_group(a, total);
+    const int total = Segments::total(a, lane), per = tiles_per_group(a, total);
     if (blockIdx.x >= static_cast<unsigned>((total + per - 1) / per)) return;
     int g = blockIdx.x * per;
     const int stop = g + per < total ? g + per : total;
@@ -434,97 +441,143 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(const DecodeArgs a
   }
 }
 
-// CH x SW waves per row of a segment that has more than one part: out = sum_s
-// 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s. A wave takes 64 channels and every SW-th
-// part; D / 64 / CH workgroups make a row.
-template <typename T, int D, int CH, int SW>
-__global__ __launch_bounds__(64 * CH * SW) void paged_join_kernel(const DecodeArgs a) {
-  __shared__ float obuf[SW][64 * CH];
-  __shared__ float lbuf[SW];
-  const int wave = wave_id(), lane = threadIdx.x & 63;
-  constexpr int kGroups = D / 64 / CH;
-  const int chunk = blockIdx.x % kGroups * CH + wave % CH, sw = wave / CH;
-  const int row = blockIdx.x / kGroups % a.rows, bh = blockIdx.x / kGroups / a.rows;
-  const int b = bh / a.kv.kv_heads, h = bh % a.kv.kv_heads;
-  const int all = a.count_of(b), zr = row / a.part_rows;
-  size_t slot0, slot1;  // of the first part and, less a step, of the others
+// Where the parts of a segment are in the workspace: part 0 at slot0, part s > 0 at
+// slot1 + s * step. One part: the output holds the result.
+struct Parts {
+  size_t slot0, slot1;
   int count, step;
-  if (a.splits) {
-    const int per = tiles_per_split(all, a.splits, a.least, 1);
-    count = (all + per - 1) / per;
-    slot0 = slot1 = (static_cast<size_t>(bh) * a.zrows + zr) * a.splits;
-    step = 1;
-  } else {
-    // workgroups w0 .. w1; their first parts, but for the first one's last
-    const int per = tiles_per_group(a, Segments::total(a, a.kv.batch, lane));
-    const int start = Segments::total(a, b, lane) + (h * a.zrows + zr) * all;
-    const int w0 = start / per, w1 = (start + all - 1) / per;
-    count = w1 - w0 + 1;
-    slot0 = 2 * static_cast<size_t>(w0) + 1;
-    slot1 = slot0 - 1;
-    step = 2;
-  }
-  if (count == 1) return;
-  auto at = [&](int s) {
-    return (s ? slot1 + static_cast<size_t>(s) * step : slot0) * a.part_rows + row - zr * a.part_rows;
-  };
-  float M = kLowest;
-  for (int s = lane; s < count; s += 64) M = fmaxf(M, a.part_ml[2 * at(s)]);
-#pragma unroll
-  for (int x = 1; x < 64; x <<= 1) M = fmaxf(M, __shfl_xor(M, x));
-  float acc = 0, l = 0;
-#pragma unroll 8
-  for (int s = sw; s < count; s += SW) {
-    const float w = exp2_fast(a.part_ml[2 * at(s)] - M);
-    l += w * a.part_ml[2 * at(s) + 1];
-    acc += w * a.part_o[at(s) * D + chunk * 64 + lane];
-  }
-  if (SW > 1) {
-    obuf[sw][wave % CH * 64 + lane] = acc;
-    if (lane == 0 && wave % CH == 0) lbuf[sw] = l;
-    __syncthreads();
-    if (sw > 0) return;
-    acc = l = 0;
-#pragma unroll
-    for (int w = 0; w < SW; ++w) acc += obuf[w][wave % CH * 64 + lane], l += lbuf[w];
-  }
-  if (a.final_ml && lane == 0 && chunk == 0) {
-    const size_t f = static_cast<size_t>(bh) * a.rows + row;
-    a.final_ml[2 * f] = M;
-    a.final_ml[2 * f + 1] = l;
-  }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  const int j = row / a.group, heads = a.group * a.kv.kv_heads;
-  uint16_t* y = static_cast<uint16_t*>(a.out) +
-                ((static_cast<size_t>(b) * a.new_tokens + j) * heads + h * a.group + row - j * a.group) * D;
-  y[chunk * 64 + lane] = static_cast<uint16_t>(T::pack(acc * inv, 0.0f));
-}
 
-// weights[t] (+)= sum over rows of 2^(score - M) / l.
-__global__ __launch_bounds__(256) void paged_weights_kernel(const DecodeArgs a, float* weights,
-                                                            int add) {
-  const int bh = blockIdx.y, b = bh / a.kv.kv_heads, h = bh % a.kv.kv_heads;
+  __device__ __forceinline__ Parts(const DecodeArgs& a, int b, int h, int zr, int lane) {
+    const int all = uniform(a.count_of(b));
+    if (a.splits) {
+      const int per = tiles_per_split(all, a.splits, a.least, 1);
+      count = (all + per - 1) / per;
+      slot0 = slot1 = (static_cast<size_t>(b * a.kv.kv_heads + h) * a.zrows + zr) * a.splits;
+      step = 1;
+    } else {
+      // workgroups w0 .. w1; their first parts, but for the first one's last
+      int before;
+      const int per = tiles_per_group(a, Segments::total(a, lane, b, &before));
+      const int start = before + (h * a.zrows + zr) * all;
+      const int w0 = start / per, w1 = (start + all - 1) / per;
+      count = w1 - w0 + 1;
+      slot0 = 2 * static_cast<size_t>(w0) + 1;
+      slot1 = slot0 - 1;
+      step = 2;
+    }
+  }
+  __device__ __forceinline__ size_t at(int s) const {
+    return s ? slot1 + static_cast<size_t>(s) * step : slot0;
+  }
+};
+
+// The first `join_groups` workgroups: CH x SW waves per row of a segment that has more
+// than one part, out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s. A wave takes 64
+// channels and every SW-th part; D / 64 / CH workgroups make a row.
+// The others: weights[t] (+)= sum over rows of 2^(score - M) / l, for four tokens of a
+// (sequence, head) per thread, with the rows' M and l joined from the parts.
+template <typename T, int D, int CH, int SW>
+__global__ __launch_bounds__(64 * CH * SW) void paged_finish_kernel(const DecodeArgs a,
+                                                                    unsigned join_groups,
+                                                                    float* weights, int add,
+                                                                    int token_groups) {
+  union Shared {
+    struct {
+      float o[SW][64 * CH], l[SW];
+    } join;
+    float ml[2][kMaxRows];
+  };
+  __shared__ Shared shared;
+  const int wave = wave_id(), lane = threadIdx.x & 63;
+  if (blockIdx.x < join_groups) {
+    constexpr int kGroups = D / 64 / CH;
+    const int chunk = blockIdx.x % kGroups * CH + wave % CH, sw = wave / CH;
+    const int row = blockIdx.x / kGroups % a.rows, bh = blockIdx.x / kGroups / a.rows;
+    const int b = bh / a.kv.kv_heads, h = bh % a.kv.kv_heads, zr = row / a.part_rows;
+    const Parts parts(a, b, h, zr, lane);
+    if (parts.count == 1) return;
+    auto at = [&](int s) { return parts.at(s) * a.part_rows + row - zr * a.part_rows; };
+    float M = kLowest;
+    for (int s = lane; s < parts.count; s += 64) M = fmaxf(M, a.part_ml[2 * at(s)]);
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) M = fmaxf(M, __shfl_xor(M, x));
+    float acc = 0, l = 0;
+#pragma unroll 8
+    for (int s = sw; s < parts.count; s += SW) {
+      const float w = exp2_fast(a.part_ml[2 * at(s)] - M);
+      l += w * a.part_ml[2 * at(s) + 1];
+      acc += w * a.part_o[at(s) * D + chunk * 64 + lane];
+    }
+    if (SW > 1) {
+      shared.join.o[sw][wave % CH * 64 + lane] = acc;
+      if (lane == 0 && wave % CH == 0) shared.join.l[sw] = l;
+      __syncthreads();
+      if (sw > 0) return;
+      acc = l = 0;
+#pragma unroll
+      for (int w = 0; w < SW; ++w)
+        acc += shared.join.o[w][wave % CH * 64 + lane], l += shared.join.l[w];
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int j = row / a.group, heads = a.group * a.kv.kv_heads;
+    uint16_t* y = static_cast<uint16_t*>(a.out) +
+                  ((static_cast<size_t>(b) * a.new_tokens + j) * heads + h * a.group + row - j * a.group) * D;
+    y[chunk * 64 + lane] = static_cast<uint16_t>(T::pack(acc * inv, 0.0f));
+    return;
+  }
+  const int id = blockIdx.x - join_groups, bh = id / token_groups;
+  const int b = bh / a.kv.kv_heads, h = bh % a.kv.kv_heads;
   const int length = a.kv.uniform_length(b);
+  const int t0 = 4 * (id % token_groups * blockDim.x + threadIdx.x);  // four tokens each
+  if (t0 - 4 * static_cast<int>(threadIdx.x) >= length) return;
+  for (int zr = wave; zr < a.zrows; zr += CH * SW) {
+    const Parts parts(a, b, h, zr, lane);
+    const int row = zr * a.part_rows + lane;
+    if (lane < a.part_rows && row < a.rows) {
+      float M = kLowest, l = 0;
+      if (parts.count == 1) {
+        const float* ml = a.final_ml + 2 * (static_cast<size_t>(bh) * a.rows + row);
+        M = ml[0], l = ml[1];
+      } else {
+        for (int s = 0; s < parts.count; ++s) M = fmaxf(M, a.part_ml[2 * (parts.at(s) * a.part_rows + lane)]);
+        for (int s = 0; s < parts.count; ++s) {
+          const float* ml = a.part_ml + 2 * (parts.at(s) * a.part_rows + lane);
+          l += exp2_fast(ml[0] - M) * ml[1];
+        }
+      }
+      shared.ml[0][row] = M;
+      shared.ml[1][row] = l == 0.0f ? 0.0f : 1.0f / l;
+    }
+  }
+  __syncthreads();
   const PagedTiles tiles = a.tiles_of(length);
   const int P = 1 << a.kv.page_shift;
-  for (int t = blockIdx.x * 256 + threadIdx.x; t < length; t += gridDim.x * 256) {
+  typedef float f32x4_any_t __attribute__((ext_vector_type(4), aligned(4)));
+  for (int t = t0; t < length; t += 4 * token_groups * blockDim.x) {
     const int page = a.kv.page(b, t >> a.kv.page_shift);
     if (page < 0) continue;
     const int tile = t >> kTileShift;
-    float w = 0;
+    f32x4_t w = {0, 0, 0, 0};
     if ((tile < tiles.sink_tiles || tile >= tiles.sink_tiles + tiles.from) &&
         ((tile + 1) << kTileShift) <= a.score_pitch) {
       const float* sp = a.scores + static_cast<size_t>(bh) * a.rows * a.score_pitch + t;
-      const float* ml = a.final_ml + 2 * static_cast<size_t>(bh) * a.rows;
-#pragma unroll 4
+#pragma unroll 8
       for (int r = 0; r < a.rows; ++r) {
-        const float l = ml[2 * r + 1];
-        w += exp2_fast(sp[static_cast<size_t>(r) * a.score_pitch] - ml[2 * r]) *
-             (l == 0.0f ? 0.0f : 1.0f / l);
+        const f32x4_t s = *reinterpret_cast<const f32x4_t*>(sp + static_cast<size_t>(r) * a.score_pitch);
+        const float M = shared.ml[0][r], inv = shared.ml[1][r];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] += exp2_fast(s[e] - M) * inv;
       }
     }
     float* dst = weights + (static_cast<size_t>(page) * a.kv.kv_heads + h) * P + (t & (P - 1));
-    *dst = add ? *dst + w : w;
+    if (t + 4 <= length) {
+      f32x4_any_t* d = reinterpret_cast<f32x4_any_t*>(dst);
+      *d = add ? *d + w : w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (t + e < length) dst[e] = add ? dst[e] + w[e] : w[e];
+    }
   }
 }
 
@@ -576,45 +629,51 @@ DecodePlan plan_of(const cudalm_paged_kv* kv, const cudalm_paged_query* q, int n
 }
 
 template <typename T, int D>
-int launch(const DecodeArgs& a, const DecodePlan& p, hipStream_t stream) {
+int launch(const DecodeArgs& a, const DecodePlan& p, float* weights, int mode, hipStream_t stream) {
   const unsigned grid = p.groups ? p.groups : static_cast<unsigned>(p.segments * p.splits);
   auto kernel = p.groups ? paged_decode_kernel<T, D, 1, true> : paged_decode_kernel<T, D, 1, false>;
   if (p.rt == 2) kernel = p.groups ? paged_decode_kernel<T, D, 2, true> : paged_decode_kernel<T, D, 2, false>;
   if (p.rt == 4) kernel = p.groups ? paged_decode_kernel<T, D, 4, true> : paged_decode_kernel<T, D, 4, false>;
   kernel<<<grid, 256, 0, stream>>>(a);
-  if (p.joins()) {
-    if (const int rc = launch_status()) return rc;
-    const unsigned rows = static_cast<unsigned>(a.kv.batch * a.kv.kv_heads * a.rows);
-    // Few rows: all waves that help, a workgroup for 64 channels (one sequence of 32768
-    // tokens: 8 us, 16 with the other form); else one per row.
-    if (rows <= static_cast<unsigned>(cu_count()))
-      paged_join_kernel<T, D, 1, 16><<<rows * (D / 64), 1024, 0, stream>>>(a);
-    else
-      paged_join_kernel<T, D, D / 64, 1><<<rows, D, 0, stream>>>(a);
-  }
+  if (!p.joins() && !mode) return launch_status();
+  if (const int rc = launch_status()) return rc;
+  // Few rows: all waves that help, a workgroup for 64 channels (one sequence of 32768
+  // tokens: 8 us, 16 with the other form); else one per row.
+  const unsigned rows = static_cast<unsigned>(a.kv.batch * a.kv.kv_heads * a.rows);
+  const bool few = rows <= static_cast<unsigned>(cu_count());
+  const unsigned join = !p.joins() ? 0 : few ? rows * (D / 64) : rows;
+  const int threads = few ? 1024 : D;
+  const int token_groups = (p.score_pitch + 4 * threads - 1) / (4 * threads);
+  const unsigned all = join + (mode ? a.kv.batch * a.kv.kv_heads * token_groups : 0);
+  const int add = mode == CUDALM_PAGED_WEIGHTS_ADD;
+  if (few)
+    paged_finish_kernel<T, D, 1, 16><<<all, 1024, 0, stream>>>(a, join, weights, add, token_groups);
+  else
+    paged_finish_kernel<T, D, D / 64, 1><<<all, D, 0, stream>>>(a, join, weights, add, token_groups);
   return launch_status();
 }
 
 template <typename T>
-int launch_d(int D, const DecodeArgs& a, const DecodePlan& p, hipStream_t stream) {
-  return D == 64    ? launch<T, 64>(a, p, stream)
-         : D == 128 ? launch<T, 128>(a, p, stream)
-                    : launch<T, 256>(a, p, stream);
+int launch_d(int D, const DecodeArgs& a, const DecodePlan& p, float* weights, int mode,
+             hipStream_t stream) {
+  return D == 64    ? launch<T, 64>(a, p, weights, mode, stream)
+         : D == 128 ? launch<T, 128>(a, p, weights, mode, stream)
+                    : launch<T, 256>(a, p, weights, mode, stream);
 }
 
 int check(const cudalm_paged_kv* kv, const cudalm_paged_query* q, int new_tokens, int mode) {
   if (const int rc = paged_check_query(kv, q)) return rc;
   if (new_tokens < 1 || mode < 0 || mode > CUDALM_PAGED_WEIGHTS_ADD) return CUDALM_W4A16_EINVAL;
-  if (static_cast<long long>(new_tokens) * (q->heads / kv->kv_heads) > 1024)
+  if (static_cast<long long>(new_tokens) * (q->heads / kv->kv_heads) > kMaxRows)
     return CUDALM_W4A16_EINVAL;
   const DecodePlan p = plan_of(kv, q, new_tokens, mode);
   const long long bh = static_cast<long long>(kv->batch) * kv->kv_heads;
   // all tiles are numbered in 31 bits
   const long long cap = (static_cast<long long>(kv->max_pages) * kv->page_size + kTile - 1) / kTile;
   if (p.segments * (cap + 1) >= (1LL << 31)) return CUDALM_W4A16_ERANGE;
-  // the join's workgroups have up to 1024 threads
-  if (p.segments >= kMaxGemmTiles || bh * p.rows >= kMaxGemmTiles / 4 || (mode && bh > 65535))
-    return CUDALM_W4A16_ERANGE;
+  // workgroups of up to 1024 threads; with weights, one per 256 or more tokens
+  const long long work = bh * p.rows + (mode ? bh * (p.score_pitch / 256 + 1) : 0);
+  if (p.segments >= kMaxGemmTiles || work >= kMaxGemmTiles / 4) return CUDALM_W4A16_ERANGE;
   return CUDALM_W4A16_OK;
 }
 
@@ -683,11 +742,7 @@ extern "C" int cudalm_paged_decode(const cudalm_paged_kv* kv, const cudalm_paged
   a.window = window_of(q);
   a.sinks = sinks_of(q);
   a.score_pitch = p.score_pitch;
-  const int rc = kv->type == CUDALM_PAGED_BF16 ? launch_d<PagedBf16>(kv->head_dim, a, p, stream)
-                                               : launch_d<PagedF16>(kv->head_dim, a, p, stream);
-  if (rc || !weights_mode) return rc;
-  const dim3 grid((p.score_pitch + 255) / 256, kv->batch * kv->kv_heads);
-  paged_weights_kernel<<<grid, 256, 0, stream>>>(a, kv->weights,
-                                                 weights_mode == CUDALM_PAGED_WEIGHTS_ADD);
-  return launch_status();
+  return kv->type == CUDALM_PAGED_BF16
+             ? launch_d<PagedBf16>(kv->head_dim, a, p, kv->weights, weights_mode, stream)
+             : launch_d<PagedF16>(kv->head_dim, a, p, kv->weights, weights_mode, stream);
 }
