@@ -15,8 +15,8 @@
 // is the lane whose operand of the second product wants just those. Nothing
 // goes through LDS before the end.
 //
-// A workgroup of four waves takes RT tiles of 16 rows and 4 / RT slices of the
-// tokens, which it joins in LDS. A call's tiles of 32 tokens, those of all
+// A workgroup of WV waves takes RT tiles of 16 rows and WV / RT slices of the tokens,
+// which it joins in LDS. A call's tiles of 32 tokens, those of all
 // sequences and heads in a row, are cut into as many equal ranges as workgroups
 // run at once: sequences of any mix of lengths keep all of them busy to the end.
 // A range may end inside a sequence; such parts go to the workspace and a second
@@ -128,20 +128,21 @@ __device__ __forceinline__ int tiles_per_group(const DecodeArgs& a, int total) {
   return r > a.least ? r : a.least;
 }
 
-// RANGES: equal ranges of all tiles, else fixed splits.
-template <typename T, int D, int RT, bool RANGES>
-__global__ __launch_bounds__(256, 2) void paged_decode_kernel(const DecodeArgs a) {
-  constexpr int KK = D / 32, DT = D / 16, SL = 4 / RT;
+// WV waves: RT tiles of rows, WV / RT slices. RANGES: equal ranges of all tiles, else
+// fixed splits.
+template <typename T, int D, int RT, int WV, bool RANGES>
+__global__ __launch_bounds__(64 * WV, 2) void paged_decode_kernel(const DecodeArgs a) {
+  constexpr int KK = D / 32, DT = D / 16, SL = WV / RT;
   constexpr int kPitch = D + 4;
-  // Each wave's queries in the order of its operands (registers are for what is on
-  // its way from memory), later the sums of two waves.
+  // The queries of a tile of rows in the order of the operands (registers are for what
+  // is on its way from memory), later the sums of two waves.
   union Shared {
-    u32x4_t q[4][KK][64];
+    u32x4_t q[RT][KK][64];
     float o[2][16 * kPitch];
   };
   __shared__ Shared shared;
-  __shared__ float mlbuf[4][2][16];
-  __shared__ uint32_t badbuf[4];
+  __shared__ float mlbuf[WV][2][16];
+  __shared__ uint32_t badbuf[WV];
   const int wave = wave_id(), lane = threadIdx.x & 63;
   const int n = lane & 15, quarter = lane >> 4;
   const int rt = wave % RT, slice = wave / RT;
@@ -160,7 +161,7 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(const DecodeArgs a
     const bool real = row < a.rows;
     const int j = row / a.group;
     const int pos = real ? first + j : -1;
-    {
+    if (slice == 0) {
       const uint16_t* qp =
           a.q +
           (static_cast<long long>(b) * a.new_tokens + (real ? j : 0)) * a.token_stride +
@@ -170,10 +171,11 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(const DecodeArgs a
       for (int kk = 0; kk < KK; ++kk) {
         u32x4_t v = *reinterpret_cast<const u32x4_t*>(qp + 32 * kk);
         if (!real) v = u32x4_t{0, 0, 0, 0};
-        shared.q[wave][kk][lane] = v;
+        shared.q[rt][kk][lane] = v;
       }
-      wave_lds_sync();
+      if (SL == 1) wave_lds_sync();
     }
+    if (SL > 1) __syncthreads();
     const size_t head_elems = static_cast<size_t>(P) * D * h;
     f32x4_t o[DT];
 #pragma unroll
@@ -212,7 +214,7 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(const DecodeArgs a
       asm volatile("" ::: "memory");  // the queries stay in LDS between tiles
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
-        const u32x4_t qf = shared.q[wave][kk][lane];
+        const u32x4_t qf = shared.q[rt][kk][lane];
         s0 = T::mfma(kf[0][kk], qf, s0);
         s1 = T::mfma(kf[1][kk], qf, s1);
       }
@@ -323,20 +325,24 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(const DecodeArgs a
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) o[dt] *= r;
       m = top;
+      // the last one or two slices that still have sums add them to those before
+      constexpr int kHands = 2 / RT > 0 ? 2 / RT : 1;
 #pragma unroll
-      for (int half = SL / 2; half > 0; half >>= 1) {
-        if (slice >= half && slice < 2 * half) {
-          float* p = shared.o[(slice - half) * RT + rt] + n * kPitch + 4 * quarter;
+      for (int left = SL; left > 1;) {
+        const int hands = kHands < left / 2 ? kHands : left / 2;
+        if (slice >= left - hands && slice < left) {
+          float* p = shared.o[(slice - left + hands) * RT + rt] + n * kPitch + 4 * quarter;
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4_t*>(p + 16 * dt) = o[dt];
         }
         __syncthreads();
-        if (slice < half) {
-          const float* p = shared.o[slice * RT + rt] + n * kPitch + 4 * quarter;
+        if (slice >= left - 2 * hands && slice < left - hands) {
+          const float* p = shared.o[(slice - left + 2 * hands) * RT + rt] + n * kPitch + 4 * quarter;
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) o[dt] += *reinterpret_cast<const f32x4_t*>(p + 16 * dt);
         }
         __syncthreads();
+        left -= hands;
       }
     }
     // to the workspace, or the output if the segment is all here
@@ -372,7 +378,9 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(const DecodeArgs a
     }
     // Inf and NaN that were taken out, for the rows that see them: one wave after the
     // other adds Inf or -Inf to the sums.
-    const uint32_t any_bad = SL > 1 ? badbuf[0] | badbuf[1] | badbuf[2] | badbuf[3] : __any(bad != 0);
+    uint32_t any_bad = __any(bad != 0);
+    if (SL > 1)
+      for (int w = 0; w < WV; ++w) any_bad |= badbuf[w];
     if (any_bad) {
 #pragma unroll 1
       for (int turn = 0; turn < SL; ++turn) {
@@ -584,6 +592,7 @@ __global__ __launch_bounds__(64 * CH * SW) void paged_finish_kernel(const Decode
 // How a call is cut.
 struct DecodePlan {
   int rows, rt, zrows, part_rows, groups, splits, least, score_pitch;
+  bool single;  // eight waves for a segment, and no join
   long long segments;
   size_t o_bytes, ml_bytes, final_bytes, score_bytes;
   bool joins() const { return splits != 1; }
@@ -610,7 +619,15 @@ DecodePlan plan_of(const cudalm_paged_kv* kv, const cudalm_paged_query* q, int n
   const long long parts = (tiles + p.least - 1) / p.least;
   const int at_once = (kv->head_dim == 64 ? 4 : 2) * cu_count();
   size_t slots;
-  if (parts <= 1 || p.segments * parts <= at_once) {
+  // One CU reads some 40 GB/s; up to 330 KB that takes less than a second launch (8
+  // sequences of 500 tokens, 32 query heads on 8 of 128: 12.6 us against 18.3; one of
+  // 777 on 2 of 256, past it: 24.5 against 15).
+  p.single = p.rt < 4 && tiles * p.rt * kv->head_dim <= 2560 && p.segments * parts <= at_once;
+  if (p.single) {
+    p.splits = 1;
+    p.groups = 0;
+    slots = 0;
+  } else if (parts <= 1 || p.segments * parts <= at_once) {
     p.splits = parts > 1 ? static_cast<int>(parts) : 1;
     p.groups = 0;
     slots = p.splits > 1 ? static_cast<size_t>(p.segments) * p.splits : 0;
@@ -631,10 +648,15 @@ DecodePlan plan_of(const cudalm_paged_kv* kv, const cudalm_paged_query* q, int n
 template <typename T, int D>
 int launch(const DecodeArgs& a, const DecodePlan& p, float* weights, int mode, hipStream_t stream) {
   const unsigned grid = p.groups ? p.groups : static_cast<unsigned>(p.segments * p.splits);
-  auto kernel = p.groups ? paged_decode_kernel<T, D, 1, true> : paged_decode_kernel<T, D, 1, false>;
-  if (p.rt == 2) kernel = p.groups ? paged_decode_kernel<T, D, 2, true> : paged_decode_kernel<T, D, 2, false>;
-  if (p.rt == 4) kernel = p.groups ? paged_decode_kernel<T, D, 4, true> : paged_decode_kernel<T, D, 4, false>;
-  kernel<<<grid, 256, 0, stream>>>(a);
+  auto kernel = p.groups ? paged_decode_kernel<T, D, 1, 4, true> : paged_decode_kernel<T, D, 1, 4, false>;
+  if (p.rt == 2) kernel = p.groups ? paged_decode_kernel<T, D, 2, 4, true> : paged_decode_kernel<T, D, 2, 4, false>;
+  if (p.rt == 4) kernel = p.groups ? paged_decode_kernel<T, D, 4, 4, true> : paged_decode_kernel<T, D, 4, 4, false>;
+  int threads = 256;
+  if (p.single && p.rt < 4) {
+    kernel = p.rt == 1 ? paged_decode_kernel<T, D, 1, 8, false> : paged_decode_kernel<T, D, 2, 8, false>;
+    threads = 512;
+  }
+  kernel<<<grid, threads, 0, stream>>>(a);
   if (!p.joins() && !mode) return launch_status();
   if (const int rc = launch_status()) return rc;
   // Few rows: all waves that help, a workgroup for 64 channels (one sequence of 32768
@@ -642,7 +664,7 @@ int launch(const DecodeArgs& a, const DecodePlan& p, float* weights, int mode, h
   const unsigned rows = static_cast<unsigned>(a.kv.batch * a.kv.kv_heads * a.rows);
   const bool few = rows <= static_cast<unsigned>(cu_count());
   const unsigned join = !p.joins() ? 0 : few ? rows * (D / 64) : rows;
-  const int threads = few ? 1024 : D;
+  threads = few ? 1024 : D;
   const int token_groups = (p.score_pitch + 4 * threads - 1) / (4 * threads);
   const unsigned all = join + (mode ? a.kv.batch * a.kv.kv_heads * token_groups : 0);
   const int add = mode == CUDALM_PAGED_WEIGHTS_ADD;
@@ -681,13 +703,13 @@ int check(const cudalm_paged_kv* kv, const cudalm_paged_query* q, int new_tokens
 
 int paged_decode_regs(int type, int D) {
   if (type == CUDALM_PAGED_BF16)
-    return D == 64    ? regs_of(paged_decode_kernel<PagedBf16, 64, 1, true>)
-           : D == 128 ? regs_of(paged_decode_kernel<PagedBf16, 128, 1, true>)
-           : D == 256 ? regs_of(paged_decode_kernel<PagedBf16, 256, 1, true>)
+    return D == 64    ? regs_of(paged_decode_kernel<PagedBf16, 64, 1, 4, true>)
+           : D == 128 ? regs_of(paged_decode_kernel<PagedBf16, 128, 1, 4, true>)
+           : D == 256 ? regs_of(paged_decode_kernel<PagedBf16, 256, 1, 4, true>)
                       : -1;
-  return D == 64    ? regs_of(paged_decode_kernel<PagedF16, 64, 1, true>)
-         : D == 128 ? regs_of(paged_decode_kernel<PagedF16, 128, 1, true>)
-         : D == 256 ? regs_of(paged_decode_kernel<PagedF16, 256, 1, true>)
+  return D == 64    ? regs_of(paged_decode_kernel<PagedF16, 64, 1, 4, true>)
+         : D == 128 ? regs_of(paged_decode_kernel<PagedF16, 128, 1, 4, true>)
+         : D == 256 ? regs_of(paged_decode_kernel<PagedF16, 256, 1, 4, true>)
                     : -1;
 }
 
