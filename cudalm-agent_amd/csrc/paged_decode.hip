@@ -187,12 +187,7 @@ __global__ __launch_bounds__(64 * WV, 2) void paged_decode_kernel(const DecodeAr
     // The next 32 tiles of this wave: lanes 2 i and 2 i + 1 hold the halves of tile i.
     int tile = 0;            // first token
     uint64_t half_at = 0;    // of the half's first key, and value, in its cache
-    auto place = [&](int x) {
-      return static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(half_at), x)) |
-             static_cast<uint64_t>(static_cast<uint32_t>(
-                 __builtin_amdgcn_readlane(static_cast<uint32_t>(half_at >> 32), x)))
-                 << 32;
-    };
+    auto place = [&](int x) { return readlane64(half_at, x); };
     auto load_k = [&](int x) {
       const uint64_t at0 = place(x), at1 = place(x + 1), at = n < 8 ? at0 : at1;
       const uint16_t* kp = a.k + at + static_cast<uint32_t>((ktok & 15) * D + 8 * quarter);

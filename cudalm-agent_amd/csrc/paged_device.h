@@ -123,6 +123,14 @@ __device__ __forceinline__ int load_uniform(const int32_t* p) {
       reinterpret_cast<uintptr_t>(p));
 }
 
+// Lane x's 64-bit value. (The builtin's result is signed: without the casts a low word
+// from 2^31 on would fill the high one.)
+__device__ __forceinline__ uint64_t readlane64(uint64_t v, int x) {
+  const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(v), x));
+  const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(v >> 32), x));
+  return static_cast<uint64_t>(hi) << 32 | lo;
+}
+
 // The cache as the kernels take it.
 struct PagedView {
   const int32_t* tables;

@@ -161,12 +161,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : D == 128 ? 3 : 4) void 
     whole_bits = __ballot(wave_full && seen_whole(first_token, wave_first, wave_last));
     wg_whole_bits = __ballot(wg_full && seen_whole(first_token, wg_first, wg_last));
   };
-  auto half_place = [&](int x) {
-    return static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(half_at), x)) |
-           static_cast<uint64_t>(
-               static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(half_at >> 32), x)))
-               << 32;
-  };
+  auto half_place = [&](int x) { return readlane64(half_at, x); };
   uint32_t absent = 0;  // of the tile fetched last: a bit for each half
   bool whole = false, wg_whole = false;
   auto fetch = [&](int i, int buf) {
@@ -529,7 +524,8 @@ extern "C" int cudalm_paged_prefill(const cudalm_paged_kv* kv, const cudalm_page
   a.token_stride = q->token_stride;
   a.head_stride = q->head_stride;
   a.negate = q->scale < 0;
-  a.scale_log2 = (a.negate ? -q->scale : q->scale) * kLog2e;
+  // Not zero: hidden scores of -inf are multiplied by it.
+  a.scale_log2 = fmaxf((a.negate ? -q->scale : q->scale) * kLog2e, 1e-38f);
   a.tokens = tokens;
   a.heads = q->heads;
   a.group = q->heads / kv->kv_heads;

@@ -117,6 +117,12 @@ def test_decode_weights(pk, dev, mode, D, P, Q, window, sinks):
                   weights=mode)
 
 
+def test_decode_weights_of_many_rows(pk, dev):
+    # 68 and 128 rows: two groups of 64, of which each may have its own parts
+    _check_decode(pk, dev, [17, 300, 900], 17, 8, 2, 64, 16, "bf16", weights="set")
+    _check_decode(pk, dev, [40, 2000], 2, 64, 1, 64, 32, "f16", 500, 4, weights="add")
+
+
 def test_decode_strided_and_scale(pk, dev):
     _check_decode(pk, dev, [9, 50], 2, 8, 2, 256, 16, "bf16", fused=True, scale=0.11)
     _check_decode(pk, dev, [9, 50], 1, 8, 2, 128, 16, "f16", fused=True, scale=-0.2)
@@ -169,7 +175,7 @@ def test_decode_shared_pages(pk, dev):
 
 
 def _check_prefill(pk, dev, lens, new, H, kv, D, P, dtype, window=0, sinks=0, absent=(), max_len=None,
-                   fused=False, extra=0, size=1.0, change=None, seed=0):
+                   fused=False, extra=0, size=1.0, change=None, seed=0, scale=None):
     c = ref.Cache(seed + 29 * D + P, lens, kv, D, P, dtype, dev, absent)
     if change:
         change(c)
@@ -178,11 +184,12 @@ def _check_prefill(pk, dev, lens, new, H, kv, D, P, dtype, window=0, sinks=0, ab
     q, qd = _queries(seed + 7, T + extra, H, D, dtype, dev, fused, size)
     cu = [sum(new[:i]) for i in range(len(new) + 1)]
     out = torch.full((T + extra, H, D), 7.0, dtype=q.dtype, device=dev)
-    pk.prefill(qd, torch.tensor(cu, dtype=torch.int32, device=dev), k, v, tables, tl, window=window,
-               sinks=sinks, max_len=max_len, out=out)
+    pk.prefill(qd, torch.tensor(cu, dtype=torch.int32, device=dev), k, v, tables, tl, scale=scale,
+               window=window, sinks=sinks, max_len=max_len, out=out)
+    s = D ** -0.5 if scale is None else scale
     torch.cuda.synchronize()
     for b, n in enumerate(new):
-        o, _, mag, big = _expect(c, b, q[cu[b]:cu[b + 1]], n, D ** -0.5, window, sinks)
+        o, _, mag, big = _expect(c, b, q[cu[b]:cu[b + 1]], n, s, window, sinks)
         vmax = float(c.v[b].double().nan_to_num(0, 0, 0).abs().max()) if lens[b] else 0.0
         ref.check_out(out[cu[b]:cu[b + 1]], o, mag, big, lens[b], vmax, dtype, D, ("prefill", b, n))
     assert bool((out[T:] == 7.0).all()), "rows of no sequence"
@@ -228,6 +235,12 @@ def test_prefill_splits(pk, dev, max_len, D):
 def test_prefill_strided_and_extra_rows(pk, dev):
     _check_prefill(pk, dev, [50, 60], [50, 20], 8, 2, 256, 16, "bf16", fused=True, extra=5)
     _check_prefill(pk, dev, [2000], [4], 8, 2, 128, 16, "f16", fused=True, extra=3)
+
+
+@pytest.mark.parametrize("scale", [0.3, -0.2, 0.0])
+def test_prefill_scale(pk, dev, scale):
+    _check_prefill(pk, dev, [70, 33], [70, 5], 4, 2, 128, 16, "bf16", window=20, sinks=3, scale=scale)
+    _check_prefill(pk, dev, [70, 33], [70, 5], 4, 2, 256, 16, "f16", scale=scale)
 
 
 def test_prefill_large_scores(pk, dev):
@@ -372,6 +385,42 @@ def test_evict_long(pk, dev, max_len):
     _check_evict(pk, dev, [41000, 300], 1, 64, 128, "bf16", 5000, 4, 100, _heavy, max_len=max_len)
 
 
+# --- a pool past 32-bit offsets ------------------------------------------------------
+
+
+def test_offsets_past_32_bits(pk, dev):
+    """Pages beyond 2^32 bytes and 2^31 elements of the pool, for every operator."""
+    pages, kv, P, D, L = 5200, 2, 1024, 256, 1500
+    k = torch.empty(pages, kv, P, D, dtype=torch.bfloat16, device=dev)
+    v = torch.empty(pages, kv, P // 8, D, 8, dtype=torch.bfloat16, device=dev)
+    w = torch.zeros(pages, kv, P, device=dev)
+    assert (pages - 10) * kv * P * D > 2 ** 31
+    c = ref.Cache(11, [L, 70], kv, D, P, "bf16", dev, width=2)
+    tables = torch.tensor([[pages - 1, pages - 3], [pages - 2, -1]], dtype=torch.int32, device=dev)
+    tl = torch.tensor([L, 70], dtype=torch.int32, device=dev)
+    cu = torch.tensor([0, L, L + 70], dtype=torch.int32, device=dev)
+    pk.append(torch.cat(c.k).to(dev), torch.cat(c.v).to(dev), k, v, tables, tl, cu_new=cu, weights=w)
+    q, qd = _queries(12, 2, 8, D, "bf16", dev)
+    out = pk.decode(qd, k, v, tables, tl, weights=w)
+    for b in range(2):
+        o, ww, mag, big = _expect(c, b, q[b:b + 1], 1, D ** -0.5, 0, 0)
+        ref.check_out(out[b:b + 1], o, mag, big, L, 6.0, "bf16", D, ("decode", b))
+    q, qd = _queries(13, 40, 8, D, "bf16", dev)
+    out = pk.prefill(qd, torch.tensor([0, 33, 40], dtype=torch.int32, device=dev), k, v, tables, tl)
+    for b, (a, e) in enumerate(((0, 33), (33, 40))):
+        o, _, mag, big = _expect(c, b, q[a:e], e - a, D ** -0.5, 0, 0)
+        ref.check_out(out[a:e], o, mag, big, L, 6.0, "bf16", D, ("prefill", b))
+    dst = torch.tensor([[pages - 5], [pages - 6]], dtype=torch.int32, device=dev)
+    kept, lens = pk.evict(k, v, tables, tl, w, dst, 500, 4, 16)
+    assert lens.tolist() == [500, 70]
+    for b, n in enumerate((500, 70)):
+        for h in range(kv):
+            src = kept[b, h, :n].cpu().long()
+            i, to = torch.arange(n, device=dev), int(dst[b, 0])
+            assert torch.equal(k[to, h, :n].cpu(), c.k[b][src, h])
+            assert torch.equal(v[to, h, i // 8, :, i % 8].cpu(), c.v[b][src, h])
+
+
 # --- streams and graphs ---------------------------------------------------------------
 
 
@@ -423,6 +472,43 @@ def test_side_stream_and_graph(pk, dev):
     got = pk.prefill(qp, cu, k, v, tables, tl, stream=side)
     side.synchronize()
     assert torch.equal(got, expect)
+
+
+def test_prefill_and_eviction_in_a_graph(pk, dev):
+    lens, kv, D = [700, 90], 2, 128
+    c = ref.Cache(21, lens, kv, D, 16, "f16", dev, spare=40)
+    k, v, tables, tl = c.upload()
+    used = set(c.tables[c.tables >= 0].tolist())
+    free = [p for p in range(c.num_pages) if p not in used]
+    dst = torch.tensor(free[:32], dtype=torch.int32, device=dev).view(2, 16)
+    w = torch.zeros(c.num_pages, kv, 16, device=dev)
+    cu = torch.tensor([0, 60, 100], dtype=torch.int32, device=dev)
+    _, qp = _queries(22, 100, 8, D, "f16", dev)
+    graph = torch.cuda.CUDAGraph()
+
+    def both():
+        return (pk.prefill(qp, cu, k, v, tables, tl), *pk.evict(k, v, tables, tl, w, dst, 250, 4, 32))
+
+    both()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        got = both()
+    for i in range(3):
+        w.uniform_()
+        qp.mul_(-1.1)
+        eager = both()
+        first = [t.clone() for t in (k, v, w)]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, eager)), i
+        assert torch.equal(w, first[2]) and torch.equal(k.view(torch.int16), first[0].view(torch.int16))
+
+
+def test_kernel_registers(pk, dev):
+    for dtype in (torch.bfloat16, torch.float16):
+        for D in pk.HEAD_DIMS:
+            assert 0 < pk.kernel_regs(dtype, D) <= 256 and 0 < pk.kernel_regs(dtype, D, prefill=True) <= 256
 
 
 def test_repeated_calls_give_the_same_bits(pk, dev):
