@@ -4,8 +4,9 @@
 // exact, have no order and the drawn token is the same however the vocabulary
 // is split. What is read is one row of the target and one of the draft per
 // sequence (where the first token is refused, or after the last), next to the
-// drafted tokens' own probabilities: bytes bound a batch, two launches'
-// latency a single sequence.
+// drafted tokens' own probabilities: bytes bound a batch (64 sequences with seven
+// drafted tokens of 248320, fp32, 127 MB: 22 us, 5.8 TB/s with what stays cached, and
+// 9 for the draw), two launches' latency a single sequence (6 + 7 us).
 
 #include "cudalm_draft.h"
 #include "hip_common.h"
@@ -196,6 +197,9 @@ __global__ __launch_bounds__(256) void draft_sum_kernel(const VerifyArgs a) {
   }
 }
 
+// One workgroup per sequence: the chunk that holds the mark, then the token in it, by
+// prefix sums of whole units. Latency bounds it, 7 to 9 us: the chunks' sums, two scans,
+// one chunk, a scan.
 template <typename P>
 __global__ __launch_bounds__(256) void draft_pick_kernel(const VerifyArgs a) {
   __shared__ int chunk, token;

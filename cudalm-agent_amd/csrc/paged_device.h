@@ -1,5 +1,5 @@
-// What the paged key-value kernels share (gfx950): element types, the pages of
-// a tile, which tokens a query sees, the join of partial softmax sums.
+// What the paged key-value kernels share (gfx950): element types, values that are
+// not finite, the pages of a tile, which tokens a query sees.
 #ifndef CUDALM_PAGED_DEVICE_H
 #define CUDALM_PAGED_DEVICE_H
 
@@ -59,7 +59,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // finite, the product takes them without those (finite_part), and the rows that
 // do see them get theirs from two more products of whole numbers: how many
 // tokens that a row sees (ones in `seen_operand`) hold +Inf or NaN, and how
-// many -Inf or NaN (positive_part, negative_part); Inf is added for the one,
+// many -Inf or NaN (special_part); Inf is added for the one,
 // -Inf for the other.
 // Both halves of a word at once: an all-ones exponent plus its lowest bit carries
 // into bit 15, a mantissa that is not zero plus its mask into the exponent.
@@ -141,15 +141,10 @@ struct PagedView {
     const int n = lens[b], cap = max_pages << page_shift;
     return n < 0 ? 0 : n < cap ? n : cap;
   }
-  // length() and page() for wave-uniform arguments: scalar loads.
+  // length() for a wave-uniform argument: a scalar load.
   __device__ __forceinline__ int uniform_length(int b) const {
     const int n = load_uniform(lens + b), cap = max_pages << page_shift;
     return n < 0 ? 0 : n < cap ? n : cap;
-  }
-  __device__ __forceinline__ int uniform_page(int b, int i) const {
-    if (i >= max_pages) return -1;
-    const int p = load_uniform(tables + static_cast<size_t>(b) * max_pages + i);
-    return p >= 0 && p < num_pages ? p : -1;
   }
   // The page of table entry i of sequence b; -1 where these tokens are absent.
   __device__ __forceinline__ int page(int b, int i) const {
@@ -159,9 +154,9 @@ struct PagedView {
   }
 };
 
-// Tiles of `tile` tokens (a power of two) that some query of positions
-// first .. length - 1 sees: the tiles of the sinks, then those from the
-// earliest window's first token on.
+// Tiles of 2^tile_shift tokens that some query of positions first .. last
+// sees: the tiles of the sinks, then those from the earliest window's first
+// token on.
 struct PagedTiles {
   int sink_tiles, from, count;
 
@@ -186,11 +181,10 @@ __device__ __forceinline__ bool paged_sees(int t, int p, int window, int sinks) 
 }
 
 // How many of `tiles` tiles each of at most `splits` parts takes: the least the
-// host asks for, more where that would leave tiles over; a multiple of `unit`.
-__device__ __forceinline__ int tiles_per_split(int tiles, int splits, int least, int unit) {
-  int c = (tiles + splits - 1) / splits;
-  c = c > least ? c : least;
-  return (c + unit - 1) / unit * unit;
+// host asks for, more where that would leave tiles over.
+__device__ __forceinline__ int tiles_per_split(int tiles, int splits, int least) {
+  const int c = (tiles + splits - 1) / splits;
+  return c > least ? c : least;
 }
 
 // The sequence whose units contain unit u, where sequence b's begin at

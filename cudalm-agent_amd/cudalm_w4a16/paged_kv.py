@@ -17,7 +17,7 @@ RuntimeError. What tables and lens hold is on the GPU and not checked by the
 host: the kernels skip pages that are out of range.
 
 max_len is what the caller knows of the longest sequence (else the tables' width
-counts): the work is split by it.
+counts): the work is split by it, and decode's weights are zero past it.
 """
 from __future__ import annotations
 

@@ -80,8 +80,9 @@ typedef struct cudalm_paged_query {
   float scale; /* of the scores, normally D^-1/2 */
   int window;  /* <= 0: none */
   int sinks;   /* first tokens that stay visible behind the window */
-  int max_len; /* no sequence is expected to be longer: only the split of the
-                  work goes by it (<= 0: max_pages * page_size) */
+  int max_len; /* no sequence is expected to be longer (<= 0: max_pages *
+                  page_size): the split of the work goes by it, and decode's
+                  room for weights, which are zero past it */
 } cudalm_paged_query;
 
 /* Writes the keys and values of the new tokens of every sequence into its
@@ -130,8 +131,8 @@ int cudalm_paged_prefill(const cudalm_paged_kv* kv, const cudalm_paged_query* q,
  * the last); new_lens[b] is their number. Other places of the pages stay as
  * they are. No page of dst_tables may be read through kv->tables by the same
  * call; dst_pages * P >= keep. Entries of dst_tables outside [0, num_pages)
- * drop the tokens that belong there from the copy. max_len: as in
- * cudalm_paged_query. */
+ * drop the tokens that belong there from the copy. max_len: no sequence is
+ * expected to be longer (<= 0: max_pages * page_size); only speed goes by it. */
 size_t cudalm_paged_evict_workspace_bytes(const cudalm_paged_kv* kv, int max_len);
 int cudalm_paged_evict(const cudalm_paged_kv* kv, const int32_t* dst_tables, int dst_pages,
                        int keep, int sinks, int recent, int32_t* kept, int32_t* new_lens,
