@@ -5,7 +5,7 @@ from __future__ import annotations
 import ctypes
 
 from . import _I, _P, _SZ, _check, _lib, _stream
-from .paged_kv import _devices, _workspace
+from .paged_kv import _empty, _workspace
 
 _L = ctypes.c_int64
 
@@ -75,11 +75,11 @@ def verify(target, draft_probs, tokens, u_accept, u_next, counts=None, out=None,
     if counts is not None:
         _plain(counts, (B,), torch.int32, index, "counts")
     if out is None:
-        out = torch.empty(B, G + 1, dtype=torch.int32, device=_devices(index))
+        out = _empty((B, G + 1), torch.int32, index, stream)
     else:
         _plain(out, (B, G + 1), torch.int32, index, "out")
     if accepted is None:
-        accepted = torch.empty(B, dtype=torch.int32, device=_devices(index))
+        accepted = _empty((B,), torch.int32, index, stream)
     else:
         _plain(accepted, (B,), torch.int32, index, "accepted")
     need = 0

@@ -159,6 +159,18 @@ def _query(q, out, token_stride, head_stride, scale, window, sinks, max_len):
                        D ** -0.5 if scale is None else scale, window, sinks, max_len or 0)
 
 
+def _empty(shape, dtype, index, stream):
+    """Memory of the stream that the call runs on: what another stream's work may still
+    use is not in it, and it is not handed out again before this one has passed."""
+    import torch
+
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=_devices(index))
+    s = torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream
+    with torch.cuda.stream(s):
+        return torch.empty(shape, dtype=dtype, device=_devices(index))
+
+
 def _workspace(nbytes, workspace, index, stream):
     """(address, bytes) of the caller's workspace or of a new one, with what holds it."""
     if workspace is not None:
@@ -169,12 +181,7 @@ def _workspace(nbytes, workspace, index, stream):
         return None, 0, None
     import torch
 
-    if stream is None:
-        w = torch.empty(nbytes, dtype=torch.uint8, device=_devices(index))
-    else:  # memory that is not handed out again before this stream has passed
-        s = torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream
-        with torch.cuda.stream(s):
-            w = torch.empty(nbytes, dtype=torch.uint8, device=_devices(index))
+    w = _empty((nbytes,), torch.uint8, index, stream)
     return w.data_ptr(), nbytes, w
 
 
@@ -185,11 +192,9 @@ def _devices(index):
     return torch.device("cuda", index)
 
 
-def _out_like(q, out, index):
+def _out_like(q, out, index, stream):
     if out is None:
-        import torch
-
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        return _empty(q.shape, q.dtype, index, stream)
     if out.shape != q.shape or out.dtype != q.dtype or out.get_device() != index or not out.is_contiguous():
         raise ValueError("paged_kv: out is contiguous and like q")
     return out
@@ -248,7 +253,7 @@ def decode(q, k, v, tables, lens, scale=None, window: int = 0, sinks: int = 0, w
         raise ValueError("paged_kv: q has one entry per sequence")
     Q = 1 if one else q.shape[1]
     mode = 0 if weights is None else WEIGHTS_ADD if accumulate else WEIGHTS_SET
-    out = _out_like(q, out, index)
+    out = _out_like(q, out, index, stream)
     query = _query(q, out, ts, hs, scale, window, sinks, max_len)
     need = 0
     if workspace is None:
@@ -267,7 +272,7 @@ def prefill(q, cu_new, k, v, tables, lens, scale=None, window: int = 0, sinks: i
     ts, hs = _rows(q, 1, None, k, index, "q")
     _int32(cu_new, (tables.shape[0] + 1,), "cu_new", index)
     T = q.shape[0]
-    out = _out_like(q, out, index)
+    out = _out_like(q, out, index, stream)
     query = _query(q, out, ts, hs, scale, window, sinks, max_len)
     need = 0
     if workspace is None:
@@ -294,11 +299,11 @@ def evict(k, v, tables, lens, weights, dst_tables, keep: int, sinks: int = 4, re
     _int32(dst_tables, (B, dst_tables.shape[1]), "dst_tables", index)
     _need(keep >= 1, "keep is at least 1")
     if kept is None:
-        kept = torch.empty(B, heads, keep, dtype=torch.int32, device=_devices(index))
+        kept = _empty((B, heads, keep), torch.int32, index, stream)
     else:
         _int32(kept, (B, heads, keep), "kept", index)
     if new_lens is None:
-        new_lens = torch.empty(B, dtype=torch.int32, device=_devices(index))
+        new_lens = _empty((B,), torch.int32, index, stream)
     else:
         _int32(new_lens, (B,), "new_lens", index)
     need = 0

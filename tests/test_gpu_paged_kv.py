@@ -474,6 +474,35 @@ def test_side_stream_and_graph(pk, dev):
     assert torch.equal(got, expect)
 
 
+def test_outputs_are_memory_of_their_stream(pk, dev):
+    """A call on another stream does not write memory that was freed on the current one,
+    whose work may still use it."""
+    c = ref.Cache(18, [700, 90], 2, 64, 16, "f16", dev)
+    k, v, tables, tl = c.upload()
+    _, q = _queries(3, 2, 8, 64, "f16", dev)
+    _, qp = _queries(4, 100, 8, 64, "f16", dev)
+    cu = torch.tensor([0, 60, 100], dtype=torch.int32, device=dev)
+    w = torch.rand(c.num_pages, 2, 16, device=dev)
+    dst = torch.full((2, 2), -1, dtype=torch.int32, device=dev)  # (nothing is copied)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def fresh(like, call):
+        t = torch.empty_like(like)
+        at = t.data_ptr()
+        del t
+        got = call()
+        side.synchronize()
+        assert got.shape == like.shape and got.data_ptr() != at
+
+    fresh(q, lambda: pk.decode(q, k, v, tables, tl, stream=side))
+    fresh(qp, lambda: pk.prefill(qp, cu, k, v, tables, tl, stream=side))
+    kept = torch.empty(2, 2, 20, dtype=torch.int32, device=dev)
+    lens = torch.empty(2, dtype=torch.int32, device=dev)
+    fresh(kept, lambda: pk.evict(k, v, tables, tl, w, dst, 20, new_lens=lens, stream=side)[0])
+    fresh(lens, lambda: pk.evict(k, v, tables, tl, w, dst, 20, kept=kept, stream=side)[1])
+
+
 def test_prefill_and_eviction_in_a_graph(pk, dev):
     lens, kv, D = [700, 90], 2, 128
     c = ref.Cache(21, lens, kv, D, 16, "f16", dev, spare=40)
