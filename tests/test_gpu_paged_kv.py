@@ -385,6 +385,38 @@ def test_evict_long(pk, dev, max_len):
     _check_evict(pk, dev, [41000, 300], 1, 64, 128, "bf16", 5000, 4, 100, _heavy, max_len=max_len)
 
 
+# --- more sequences than a wave has lanes ----------------------------------------------
+
+MANY = [(37 * i * i + 11 * i) % 501 for i in range(150)]  # 0 .. 500 tokens
+
+
+@pytest.mark.parametrize("Q,weights", [(1, None), (5, "add")])
+def test_decode_many_sequences(pk, dev, Q, weights):
+    _check_decode(pk, dev, MANY, Q, 8, 2, 64, 16, "bf16", weights=weights)
+    _check_decode(pk, dev, MANY[:65], Q, 8, 2, 128, 32, "f16", window=100, sinks=4, weights=weights)
+
+
+def test_prefill_append_and_evict_many_sequences(pk, dev):
+    new = [min(n, 1 + (7 * i) % 40) for i, n in enumerate(MANY)]
+    _check_prefill(pk, dev, MANY, new, 8, 2, 64, 16, "f16")
+    _check_prefill(pk, dev, MANY[:129], new[:129], 4, 4, 128, 32, "bf16", window=50, sinks=4)
+    _check_evict(pk, dev, MANY, 2, 64, 16, "bf16", 40, 4, 8, _heavy)
+    kv, D, P = 2, 64, 16
+    c = ref.Cache(7, MANY, kv, D, P, "bf16", dev)
+    k, v, tables, tl = c.upload()
+    want_k, want_v = k.clone(), v.clone()
+    for b, (n, m) in enumerate(zip(MANY, new)):
+        t = torch.arange(n - m, n)
+        at = c.tables[b, t // P].long()
+        k[at, :, t % P] = 0
+        v[at, :, t % P // 8, :, t % 8] = 0
+    nk, nv = (torch.cat([x[b][n - m:] for b, (n, m) in enumerate(zip(MANY, new))]).to(dev) for x in (c.k, c.v))
+    cu = torch.tensor([sum(new[:i]) for i in range(151)], dtype=torch.int32, device=dev)
+    pk.append(nk, nv, k, v, tables, tl, cu_new=cu)
+    assert torch.equal(k.view(torch.int16), want_k.view(torch.int16))
+    assert torch.equal(v.view(torch.int16), want_v.view(torch.int16))
+
+
 # --- a pool past 32-bit offsets ------------------------------------------------------
 
 
