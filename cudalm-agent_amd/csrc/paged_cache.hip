@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const AppendArgs a) {
     n = a.each;
     g = blockIdx.x % units;
   }
-  if (n < 1 || n > a.tokens - begin) return;
+  if (n < 1 || n > a.tokens - begin || g < 0) return;  // (g < 0 where cu does not ascend)
   const int length = a.kv.length(b), first = length - n;  // position of row `begin`
   const int p0 = (((first > 0 ? first : 0) >> 3) + g) * 8;
   if (p0 >= length) return;

@@ -105,7 +105,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : D == 128 ? 3 : 4) void 
   const int new_tokens = end_row - begin_row;
   const int row0 = (unit - (begin_row * a.group / kRows + b)) * kRows;
   const int rows = new_tokens * a.group;
-  if (row0 >= rows) return;
+  if (row0 < 0 || row0 >= rows) return;  // (below 0 where cu does not ascend)
   const int length = a.kv.uniform_length(b), first = length - new_tokens;
 
   // this lane's row, and the positions of the wave's and the workgroup's first and last

@@ -112,9 +112,10 @@ int cudalm_paged_decode(const cudalm_paged_kv* kv, const cudalm_paged_query* q, 
                         hipStream_t stream);
 
 /* Attention of a chunk: rows cu_new[b] .. cu_new[b + 1] - 1 (device,
- * [batch + 1], from 0 to `tokens`) of q and out are the last tokens of
- * sequence b; their keys and values are in the cache. Rows that belong to no
- * sequence are not written. */
+ * [batch + 1], ascending from 0 to `tokens`) of q and out are the last tokens
+ * of sequence b; their keys and values are in the cache. Rows that belong to no
+ * sequence are not written. (Ranges that do not ascend or leave 0 .. tokens make
+ * their rows' results unspecified; nothing outside of the tensors is touched.) */
 size_t cudalm_paged_prefill_workspace_bytes(const cudalm_paged_kv* kv, const cudalm_paged_query* q,
                                             int tokens);
 int cudalm_paged_prefill(const cudalm_paged_kv* kv, const cudalm_paged_query* q,

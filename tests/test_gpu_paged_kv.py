@@ -417,6 +417,28 @@ def test_prefill_append_and_evict_many_sequences(pk, dev):
     assert torch.equal(v.view(torch.int16), want_v.view(torch.int16))
 
 
+def test_row_ranges_that_do_not_ascend(pk, dev):
+    """Sequences 1 and 2 have ranges that end before they begin and after the last row: sequence 0 gets
+    its results, and the others' pages stay as they are."""
+    c = ref.Cache(9, [70, 50, 600], 2, 64, 16, "bf16", dev)
+    k, v, tables, tl = c.upload()
+    cu = torch.tensor([0, 60, 30, 500], dtype=torch.int32, device=dev)
+    q, qd = _queries(11, 100, 8, 64, "bf16", dev)
+    out = pk.prefill(qd, cu, k, v, tables, tl, max_len=100)
+    o, _, mag, big = _expect(c, 0, q[:60], 60, 0.125, 0, 0)
+    ref.check_out(out[:60], o, mag, big, 70, float(c.v[0].abs().max()), "bf16", 64, 0)
+    before_k, before_v = k.clone(), v.clone()
+    nk, nv = (torch.randn(100, 2, 64, device=dev).to(k.dtype) for _ in range(2))
+    nk[:60], nv[:60] = c.k[0][10:].to(dev), c.v[0][10:].to(dev)
+    pk.append(nk, nv, k, v, tables, tl, cu_new=cu)
+    assert torch.equal(k.view(torch.int16), before_k.view(torch.int16))
+    assert torch.equal(v.view(torch.int16), before_v.view(torch.int16))
+    cu = torch.tensor([50, 0, -7, 100], dtype=torch.int32, device=dev)
+    pk.prefill(qd, cu, k, v, tables, tl)
+    pk.append(nk, nv, k, v, torch.full_like(tables, -1), tl, cu_new=cu)
+    torch.cuda.synchronize()
+
+
 # --- a pool past 32-bit offsets ------------------------------------------------------
 
 
