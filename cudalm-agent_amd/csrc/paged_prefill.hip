@@ -24,7 +24,7 @@
 // of 256: 233-257 us (box to box) and 15 for the join, 1.08 PFLOP/s at best, where an
 // 8192-wide product of the library reaches 1.37. Two tiles of rows per wave halve the LDS
 // reads but need more registers than two waves per SIMD leave (a 2048-token chunk at 6144,
-// 32 heads on 8 of 128: 408 us, 276 with one). 8 prompts of up to 1000 tokens with a window
+// 32 heads on 8 of 128: 408 us, 261-288 with one). 8 prompts of up to 1000 tokens with a window
 // of 512, same heads: 83-88 us, 19 tiles per workgroup of which 16 are the window's; 4% go
 // into cleaning tiles that are seen in part.
 
@@ -269,7 +269,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : D == 128 ? 3 : 4) void 
     u32x4_t pf[2];
     float sum = 0;
     const u32x4_t* vp = reinterpret_cast<const u32x4_t*>(vt) + half * D + n;
-    constexpr int kFirst = D == 256 ? 3 : 1;  // value operands that load during the exponentials
+    constexpr int kFirst = 1 + D / 128;  // value operands that load during the exponentials
     u32x4_t vf[kFirst];
 #pragma unroll
     for (int x = 0; x < kFirst; ++x) vf[x] = vp[(x / DT) * 2 * D + 32 * (x % DT)];
@@ -289,7 +289,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : D == 128 ? 3 : 4) void 
       if (x + kFirst < 2 * DT) vf[x % kFirst] = vp[((x + kFirst) / DT) * 2 * D + 32 * ((x + kFirst) % DT)];
       o[x % DT] = T::mfma32(w, pf[x / DT], o[x % DT]);
     }
-    if (D == 256) {
+    if (D >= 128) {
       __builtin_amdgcn_sched_group_barrier(0x100, kFirst, 0);
 #pragma unroll
       for (int x = 0; x < 2 * DT - kFirst; ++x) {
