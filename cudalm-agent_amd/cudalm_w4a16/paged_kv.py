@@ -166,8 +166,12 @@ def _empty(shape, dtype, index, stream):
 
     if stream is None:
         return torch.empty(shape, dtype=dtype, device=_devices(index))
-    s = torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream
-    with torch.cuda.stream(s):
+    if isinstance(stream, int):
+        # (handle 0 is the default stream; ExternalStream takes 0 for none given and would
+        # give a stream of torch's pool)
+        stream = (torch.cuda.ExternalStream(stream, device=_devices(index)) if stream
+                  else torch.cuda.default_stream(_devices(index)))
+    with torch.cuda.stream(stream):
         return torch.empty(shape, dtype=dtype, device=_devices(index))
 
 

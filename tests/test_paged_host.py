@@ -1,0 +1,36 @@
+"""The host side of the paged cache's and draft verification's Python layer, on
+the CPU: where memory comes from, first calls of several threads, arguments that
+do not fit the C types."""
+import contextlib
+import sys
+
+import pytest
+
+
+@pytest.fixture
+def pk():
+    from cudalm_w4a16 import paged_kv
+
+    return paged_kv
+
+
+@pytest.mark.parametrize("stream,want", [(0, ("default", 0)), (0x5500, ("external", 0x5500)), (None, None),
+                                         ("a stream object", "a stream object")])
+def test_memory_is_of_the_stream_that_the_call_runs_on(pk, monkeypatch, stream, want):
+    """Handle 0 is the default stream, which torch gives by another name than streams of a handle
+    (0 there means no handle, and a stream of torch's pool)."""
+    import torch
+
+    current = [None]
+
+    @contextlib.contextmanager
+    def run_on(s):
+        current[0] = s
+        yield
+        current[0] = None
+
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda handle, device=None: ("external", handle))
+    monkeypatch.setattr(torch.cuda, "default_stream", lambda device=None: ("default", getattr(device, "index", device)))
+    monkeypatch.setattr(torch.cuda, "stream", run_on)
+    monkeypatch.setattr(torch, "empty", lambda *a, **k: current[0])
+    assert pk._empty((3,), torch.uint8, 0, stream) == want
