@@ -275,7 +275,6 @@ __global__ __launch_bounds__(kSelect) void paged_select_kernel(const EvictArgs a
   }
   const int count = all + ties < a.keep ? all + ties : a.keep;
   for (int i = count + tid; i < a.keep; i += kSelect) kept[i] = -1;
-  if (h == 0 && tid == 0) a.new_lens[b] = count;
 }
 
 constexpr int kMove = 32;  // kept tokens of a copying workgroup
@@ -296,7 +295,14 @@ __global__ __launch_bounds__(256) void paged_compact_kernel(const EvictArgs a) {
   const int i0 = blockIdx.x * kMove;
   const int P = 1 << a.kv.page_shift;
   if (tid < kMove) {
-    const int i = i0 + tid, pos = i < a.keep ? a.kept[static_cast<size_t>(bh) * a.keep + i] : -1;
+    const int32_t* kept = a.kept + static_cast<size_t>(bh) * a.keep;
+    const int i = i0 + tid, pos = i < a.keep ? kept[i] : -1;
+    // The new length here and not in the selection: there, new_lens may be the lengths
+    // that other heads' workgroups have still to read. It is where kept ends.
+    if (h == 0) {
+      if (pos >= 0 && (i + 1 == a.keep || kept[i + 1] < 0)) a.new_lens[b] = i + 1;
+      if (i == 0 && pos < 0) a.new_lens[b] = 0;
+    }
     const int pi = i >> a.kv.page_shift;
     const int to = pi < a.dst_pages ? a.dst[static_cast<size_t>(b) * a.dst_pages + pi] : -1;
     const int from = pos >= 0 ? a.kv.page(b, pos >> a.kv.page_shift) : -1;

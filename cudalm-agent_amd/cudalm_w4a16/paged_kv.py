@@ -293,7 +293,7 @@ def evict(k, v, tables, lens, weights, dst_tables, keep: int, sinks: int = 4, re
     `sinks`, the last `recent`, and those with the largest weights) and copies
     them, in order, into the pages of dst_tables [B, W'], which no sequence of
     the call reads. Returns (kept [B, kv_heads, keep] int32 old positions, -1
-    past the last; new_lens [B] int32)."""
+    past the last; new_lens [B] int32, which may be given as `lens` itself)."""
     import torch
 
     _need(weights is not None, "eviction goes by the weights")

@@ -129,8 +129,8 @@ int cudalm_paged_prefill(const cudalm_paged_kv* kv, const cudalm_paged_query* q,
  * weights: the earlier token). The kept tokens' keys, values and weights are
  * copied, in their order, into the pages of dst_tables [batch][dst_pages],
  * and their old positions written to kept [batch][kv_heads][keep] (-1 past
- * the last); new_lens[b] is their number. Other places of the pages stay as
- * they are. No page of dst_tables may be read through kv->tables by the same
+ * the last); new_lens[b] is their number, and may be kv->lens itself. Other
+ * places of the pages stay as they are. No page of dst_tables may be read through kv->tables by the same
  * call; dst_pages * P >= keep. Entries of dst_tables outside [0, num_pages)
  * drop the tokens that belong there from the copy. max_len: no sequence is
  * expected to be longer (<= 0: max_pages * page_size); only speed goes by it. */
