@@ -155,7 +155,9 @@ __global__ __launch_bounds__(256) void draft_sum_kernel(const VerifyArgs a) {
   __shared__ uint64_t waves[4];
   const int b = blockIdx.y, tid = threadIdx.x;
   const int n = accepted_count<P>(a, b, &refused);
-  if (blockIdx.x == 0 && tid == 0) a.accepted[b] = n;
+  // through out, and not to `accepted`, which may be the counts that other workgroups and
+  // the next kernel have still to read
+  if (blockIdx.x == 0 && tid == 0) a.out[static_cast<size_t>(b) * (a.g + 1)] = n;
   const Rows<P> rows(a, b, n);
   const bool wide = ((reinterpret_cast<uintptr_t>(rows.p) | reinterpret_cast<uintptr_t>(rows.q)) & 15) == 0;
   for (int chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
@@ -204,7 +206,9 @@ template <typename P>
 __global__ __launch_bounds__(256) void draft_pick_kernel(const VerifyArgs a) {
   __shared__ int chunk, token;
   __shared__ uint64_t waves[4], before;
-  const int b = blockIdx.x, tid = threadIdx.x, n = a.accepted[b];
+  const int b = blockIdx.x, tid = threadIdx.x;
+  int32_t* out = a.out + static_cast<size_t>(b) * (a.g + 1);
+  const int n = out[0];
   const Rows<P> rows(a, b, n);
   const uint64_t* s = a.sums + 2 * static_cast<size_t>(b) * a.chunks;
   uint64_t c[2][4], sum[2] = {0, 0}, total[2];
@@ -247,7 +251,7 @@ __global__ __launch_bounds__(256) void draft_pick_kernel(const VerifyArgs a) {
     }
   }
   __syncthreads();
-  int32_t* out = a.out + static_cast<size_t>(b) * (a.g + 1);
+  if (tid == 0) a.accepted[b] = n;
   for (int i = tid; i <= a.g; i += 256)
     out[i] = i < n ? a.tokens[static_cast<size_t>(b) * a.g + i] : i == n ? token : -1;
 }

@@ -52,7 +52,7 @@ def verify(target, draft_probs, tokens, u_accept, u_next, counts=None, out=None,
     int32 are the drafted ones, counts [B] int32 how many are valid (None: G),
     u_accept [B, G] and u_next [B] float32 random numbers of [0, 1). Returns
     (out [B, G + 1] int32: the accepted tokens, the next one, -1 after it;
-    accepted [B] int32)."""
+    accepted [B] int32, which may be given as `counts` itself)."""
     global _types
     import torch
 

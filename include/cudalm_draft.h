@@ -26,8 +26,8 @@
  *   sum_{w <= v} r_w > floor(sum_w r_w * U / 2^24),   U = floor(u_next * 2^24)
  *
  * out [batch][draft + 1] gets the accepted tokens, the next one, and -1 in the
- * remaining places; accepted [batch] gets n. Where p_n is zero everywhere the
- * next token is -1.
+ * remaining places; accepted [batch] gets n, and may be counts itself. Where
+ * p_n is zero everywhere the next token is -1.
  */
 #ifndef CUDALM_DRAFT_H
 #define CUDALM_DRAFT_H
