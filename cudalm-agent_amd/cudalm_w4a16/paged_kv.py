@@ -143,14 +143,21 @@ def _cache(k, v, tables, lens, weights):
 
 
 def _rows(x, cols, heads, like, index, name):
-    """(token stride, head stride) of x: rows of [heads, D] over its leading dimensions."""
+    """(token stride, head stride) of x: rows of [heads, D] over its leading dimensions.
+    Strides of dimensions of one entry have no meaning; 0 where that is all there is."""
     shape, s = x.shape, x.stride()
     if (len(shape) != cols + 2 or shape[-1] != like.shape[3] or x.dtype != like.dtype or
             x.get_device() != index or (heads and shape[-2] != heads)):
         raise ValueError(f"paged_kv: {name} ({x.dtype} {list(shape)} on {x.device}) does not match the cache")
-    if s[-1] != 1 or (cols == 2 and shape[0] != 1 and s[0] != shape[1] * s[1]):
-        raise ValueError(f"paged_kv: {name}: heads are contiguous and tokens equally spaced")
-    return s[-3], s[-2]
+    between = s[-3] if shape[-3] != 1 else 0
+    if cols == 2 and shape[0] != 1:
+        if shape[1] == 1:
+            between = s[0]
+        elif s[0] != shape[1] * s[1]:
+            raise ValueError(f"paged_kv: {name}: tokens are equally spaced")
+    if s[-1] != 1:
+        raise ValueError(f"paged_kv: {name}: a head's elements are contiguous")
+    return between, s[-2] if shape[-2] != 1 else 0
 
 
 def _query(q, out, token_stride, head_stride, scale, window, sinks, max_len):

@@ -34,3 +34,25 @@ def test_memory_is_of_the_stream_that_the_call_runs_on(pk, monkeypatch, stream, 
     monkeypatch.setattr(torch.cuda, "stream", run_on)
     monkeypatch.setattr(torch, "empty", lambda *a, **k: current[0])
     assert pk._empty((3,), torch.uint8, 0, stream) == want
+
+
+def test_rows_of_one_token_are_equally_spaced(pk):
+    """The strides of dimensions of one entry say nothing: one token per sequence out of a longer tensor
+    has the batch's stride, a single one any."""
+    import torch
+
+    like = torch.empty(1, 2, 16, 128, dtype=torch.bfloat16)
+    x = torch.empty(3, 5, 8, 128, dtype=torch.bfloat16)
+    rows = lambda t, cols: pk._rows(t, cols, None, like, -1, "q")  # noqa: E731
+    assert rows(x[:, -1:], 2) == (5 * 8 * 128, 128)
+    assert rows(x[:, -1], 1) == (5 * 8 * 128, 128)
+    assert rows(x, 2) == (8 * 128, 128)
+    assert rows(x[:1, 1:3], 2) == (8 * 128, 128)
+    assert rows(x[:, :, :1], 2) == (8 * 128, 0)
+    odd = torch.empty(9, 8, 132, dtype=torch.bfloat16)[:, :, :128]
+    assert rows(odd.as_strided((1, 8, 128), (3, 128, 1)), 1) == (0, 128)
+    assert rows(odd.as_strided((1, 1, 1, 128), (3, 5, 7, 1)), 2) == (0, 0)
+    with pytest.raises(ValueError):
+        rows(x[:, 1:3], 2)  # two tokens of each of five
+    with pytest.raises(ValueError):
+        rows(x[:, -1:].transpose(2, 3).reshape(3, 1, 128, 8).transpose(2, 3), 2)  # a head's elements apart
