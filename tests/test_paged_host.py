@@ -55,4 +55,4 @@ def test_rows_of_one_token_are_equally_spaced(pk):
     with pytest.raises(ValueError):
         rows(x[:, 1:3], 2)  # two tokens of each of five
     with pytest.raises(ValueError):
-        rows(x[:, -1:].transpose(2, 3).reshape(3, 1, 128, 8).transpose(2, 3), 2)  # a head's elements apart
+        rows(x[:, -1:].transpose(2, 3).contiguous().transpose(2, 3), 2)  # a head's elements apart
