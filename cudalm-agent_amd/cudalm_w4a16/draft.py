@@ -33,11 +33,12 @@ def _probs(p, B, rows, V, dtype, index, name):
     if rows == 0:
         return V
     s = p.stride()
-    if (p.shape != (B, rows, V) or p.dtype != dtype or p.get_device() != index or s[2] != 1 or
-            (B != 1 and s[0] != rows * s[1])):
+    if (p.shape != (B, rows, V) or p.dtype != dtype or p.get_device() != index or (s[2] != 1 and V != 1) or
+            (B != 1 and rows != 1 and s[0] != rows * s[1])):
         raise ValueError(f"draft: {name} is [{B}, {rows}, {V}] of the target's type and GPU, rows contiguous "
                          "and equally spaced")
-    return s[1] if rows > 1 or B == 1 else s[0]
+    # one row per sequence is always equally spaced; the stride of a single row has no meaning
+    return s[1] if rows != 1 else s[0] if B != 1 else V
 
 
 def _plain(t, shape, dtype, index, name):

@@ -56,3 +56,23 @@ def test_rows_of_one_token_are_equally_spaced(pk):
         rows(x[:, 1:3], 2)  # two tokens of each of five
     with pytest.raises(ValueError):
         rows(x[:, -1:].transpose(2, 3).contiguous().transpose(2, 3), 2)  # a head's elements apart
+
+
+def test_one_row_of_probabilities_per_sequence():
+    import torch
+
+    from cudalm_w4a16 import draft
+
+    probs = lambda t, rows, V: draft._probs(t, t.shape[0], rows, V, torch.float32, -1, "target")  # noqa: E731
+    x = torch.empty(3, 5, 100)
+    assert probs(x[:, :1], 1, 100) == 500
+    assert probs(x[:, :1, :90], 1, 90) == 500
+    assert probs(x, 5, 100) == 100
+    assert probs(x[:1, 1:3], 2, 100) == 100
+    assert probs(x[:1, 1:2], 1, 100) >= 100
+    assert probs(x.as_strided((1, 1, 100), (1, 3, 1)), 1, 100) >= 100
+    assert probs(x.as_strided((3, 5, 1), (500, 100, 2)), 5, 1) == 100  # a vocabulary of one
+    with pytest.raises(ValueError):
+        probs(x[:, 1:3], 2, 100)
+    with pytest.raises(ValueError):
+        probs(x[:, :1, ::2], 1, 50)
