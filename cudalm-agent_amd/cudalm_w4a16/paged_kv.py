@@ -160,10 +160,21 @@ def _rows(x, cols, heads, like, index, name):
     return between, s[-2] if shape[-2] != 1 else 0
 
 
+def _need_ints(**values):
+    """Whole numbers that the C types hold: ctypes would pass the lower 32 bits of others."""
+    for name, x in values.items():
+        if not -2 ** 31 <= x < 2 ** 31:
+            raise ValueError(f"paged_kv: {name} {x} is past 32 bits")
+
+
 def _query(q, out, token_stride, head_stride, scale, window, sinks, max_len):
     D = q.shape[-1]
-    return _pack_query(q.data_ptr(), out.data_ptr(), token_stride, head_stride, q.shape[-2],
-                       D ** -0.5 if scale is None else scale, window, sinks, max_len or 0)
+    try:
+        return _pack_query(q.data_ptr(), out.data_ptr(), token_stride, head_stride, q.shape[-2],
+                           D ** -0.5 if scale is None else scale, window, sinks, max_len or 0)
+    except struct.error:
+        _need_ints(window=window, sinks=sinks, max_len=max_len or 0)
+        raise
 
 
 def _empty(shape, dtype, index, stream):
@@ -304,6 +315,7 @@ def evict(k, v, tables, lens, weights, dst_tables, keep: int, sinks: int = 4, re
     import torch
 
     _need(weights is not None, "eviction goes by the weights")
+    _need_ints(keep=keep, sinks=sinks, recent=recent, max_len=max_len or 0)
     kv, index = _cache(k, v, tables, lens, weights)
     B, heads = tables.shape[0], k.shape[1]
     _need(dst_tables.dim() == 2, "dst_tables is [B, W']")

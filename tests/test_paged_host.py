@@ -76,3 +76,28 @@ def test_one_row_of_probabilities_per_sequence():
         probs(x[:, 1:3], 2, 100)
     with pytest.raises(ValueError):
         probs(x[:, :1, ::2], 1, 50)
+
+
+BIG = [2 ** 31, 2 ** 32 + 5, -2 ** 31 - 1, 10 ** 30]
+
+
+@pytest.mark.parametrize("value", BIG)
+@pytest.mark.parametrize("name", ["window", "sinks", "max_len"])
+def test_options_past_32_bits_of_a_query_are_refused(pk, name, value):
+    import torch
+
+    q = torch.empty(3, 8, 128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match=name):
+        pk._query(q, q, 1024, 128, None, **{**dict(window=0, sinks=0, max_len=None), name: value})
+
+
+@pytest.mark.parametrize("value", BIG)
+@pytest.mark.parametrize("name", ["keep", "sinks", "recent", "max_len"])
+def test_options_past_32_bits_of_an_eviction_are_refused(pk, name, value):
+    """ctypes would pass their lower 32 bits."""
+    import torch
+
+    k, v, w = pk.empty_cache(4, 16, 2, 128, torch.bfloat16, device="cpu", weights=True)
+    tables, lens = torch.zeros(3, 2, dtype=torch.int32), torch.ones(3, dtype=torch.int32)
+    with pytest.raises(ValueError, match=name):
+        pk.evict(k, v, tables, lens, w, tables, **{"keep": 3, name: value})
