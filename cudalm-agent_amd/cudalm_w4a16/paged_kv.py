@@ -60,8 +60,8 @@ def _load_types():
     global _types, _int32_type, _float32_type
     import torch
 
-    _types = {torch.bfloat16: BF16, torch.float16: F16}
     _int32_type, _float32_type = torch.int32, torch.float32
+    _types = {torch.bfloat16: BF16, torch.float16: F16}  # last: other threads go by it
 
 
 def _type_of(dtype) -> int:

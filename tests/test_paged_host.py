@@ -101,3 +101,22 @@ def test_options_past_32_bits_of_an_eviction_are_refused(pk, name, value):
     tables, lens = torch.zeros(3, 2, dtype=torch.int32), torch.ones(3, dtype=torch.int32)
     with pytest.raises(ValueError, match=name):
         pk.evict(k, v, tables, lens, w, tables, **{"keep": 3, name: value})
+
+
+def test_types_are_all_there_once_the_first_is_seen(pk, monkeypatch):
+    """A second thread's first call goes on as soon as _types is set."""
+    import torch
+
+    seen = []
+
+    class Torch:
+        def __getattr__(self, name):
+            seen.append((name, pk._types))
+            return getattr(torch, name)
+
+    monkeypatch.setitem(sys.modules, "torch", Torch())
+    monkeypatch.setattr(pk, "_types", None)
+    pk._load_types()
+    assert {"bfloat16", "float16", "int32", "float32"} <= {n for n, _ in seen}
+    assert all(types is None for _, types in seen)
+    assert pk._types == {torch.bfloat16: pk.BF16, torch.float16: pk.F16} and pk._int32_type is torch.int32
