@@ -695,9 +695,10 @@ int check(const cudalm_paged_kv* kv, const cudalm_paged_query* q, int new_tokens
     return CUDALM_W4A16_EINVAL;
   const DecodePlan p = plan_of(kv, q, new_tokens, mode);
   const long long bh = static_cast<long long>(kv->batch) * kv->kv_heads;
-  // all tiles are numbered in 31 bits
+  // all tiles are numbered in 31 bits, and where the last workgroup's range would end
   const long long cap = (static_cast<long long>(kv->max_pages) * kv->page_size + kTile - 1) / kTile;
-  if (p.segments * (cap + 1) >= (1LL << 31)) return CUDALM_W4A16_ERANGE;
+  const long long tiles = p.segments * (cap + 1);
+  if (tiles + (p.groups ? tiles / p.groups + p.groups : 0) >= (1LL << 31)) return CUDALM_W4A16_ERANGE;
   // workgroups of up to 1024 threads; with weights, one per 256 or more tokens
   const long long work = bh * p.rows + (mode ? bh * (p.score_pitch / 256 + 1) : 0);
   if (p.segments >= kMaxGemmTiles || work >= kMaxGemmTiles / 4) return CUDALM_W4A16_ERANGE;

@@ -120,3 +120,24 @@ def test_types_are_all_there_once_the_first_is_seen(pk, monkeypatch):
     assert {"bfloat16", "float16", "int32", "float32"} <= {n for n, _ in seen}
     assert all(types is None for _, types in seen)
     assert pk._types == {torch.bfloat16: pk.BF16, torch.float16: pk.F16} and pk._int32_type is torch.int32
+
+
+def test_decode_of_tiles_that_31_bits_do_not_number_is_refused(pk, w4):
+    """The last workgroup's range of tiles ends past the last tile: there has to be room for it."""
+    import ctypes
+
+    lib, fake = w4.lib(), 0x100000
+    q = pk.Query(q=fake, out=fake, token_stride=1024, head_stride=128, heads=8, scale=0.1)
+
+    def served(batch, max_pages):
+        kv = pk.KV(k=fake, v=fake, tables=fake, lens=fake, num_pages=10, page_size=16, kv_heads=2, head_dim=128,
+                   batch=batch, max_pages=max_pages)
+        args = (ctypes.byref(kv), ctypes.byref(q), 1, 0)
+        if lib.cudalm_paged_decode_workspace_bytes(*args):
+            return True
+        assert lib.cudalm_paged_decode(*args, fake, 1 << 40, None) == w4.ERANGE
+        return False
+
+    assert not served(33, 2 ** 26) and not served(32, 2 ** 26)
+    assert not served(32, 2 ** 26 - 4)  # 64 x (2^25 - 2) tiles of 32 tokens
+    assert served(31, 2 ** 26) and served(62, 2 ** 25)
