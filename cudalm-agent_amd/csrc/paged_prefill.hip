@@ -324,8 +324,9 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : D == 128 ? 3 : 4) void 
     }
     if (here <= wave_last) step(seen, here, gone, kt, vt);  // not above the wave's rows
   }
-  // Inf or NaN for the sums of channels 32 dt .. whose rows see such a value (in
-  // tiles that were not cleaned of it they have it already): how many tokens hold +Inf or NaN, -Inf or NaN.
+  // Inf or NaN for the sums of channels 32 dt .. whose rows see such a value: how many
+  // tokens hold +Inf or NaN, -Inf or NaN. In tiles that were not cleaned a weight that
+  // underflows has made NaN of Inf, so what the sums hold there does not count.
   auto add_special = [&](f32x16_t& r, int dt) {
     f32x16_t up, down;
 #pragma unroll
@@ -354,9 +355,15 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : D == 128 ? 3 : 4) void 
     }
 #pragma unroll
     for (int e = 0; e < 16; ++e)
-      r[e] += (up[e] > 0 ? __builtin_inff() : 0.0f) + (down[e] > 0 ? -__builtin_inff() : 0.0f);
+      if (up[e] > 0 || down[e] > 0)
+        r[e] = (up[e] > 0 ? __builtin_inff() : 0.0f) + (down[e] > 0 ? -__builtin_inff() : 0.0f);
   };
-  votes[wave] = __any(special != 0);
+  float all = 0;  // NaN if one of the sums is not finite
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) all = __builtin_fmaf(o[dt][e], 0.0f, all);
+  votes[wave] = __any(special != 0 || all != all);
   __syncthreads();
   special = 0;
 #pragma unroll

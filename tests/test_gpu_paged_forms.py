@@ -1,8 +1,8 @@
 """Attention over the paged cache in every form that the calls are cut into: one launch
 of eight waves, fixed splits and equal ranges of all tiles, one, two and four tiles of
 rows, whole and split chunks, each by the name of the kernel that runs. With windows,
-sinks, absent pages and weights; with Inf and NaN in values that rows see. Expected
-results are float64, by the definition in the header; tolerances follow from the
+sinks, absent pages and weights; with Inf and NaN in values that rows see, whatever
+their weights. Expected results are float64, by the definition in the header; tolerances follow from the
 roundings (paged_reference.py)."""
 import pytest
 import torch
@@ -83,6 +83,28 @@ def specials(c):
         c.v[b][n - 3, :, 9] = float("-inf")
         if c.kv > 1:
             c.k[b][n // 3, c.kv - 1, 1] = float("nan")
+
+
+def faint(c):
+    """Inf and NaN in tokens whose scores are 400 below the others, so that their weights underflow."""
+    for b, n in enumerate(c.lens):
+        if n < 60:
+            continue
+        for t, channel, x in ((3, 1, float("inf")), (n // 2, 2, float("-inf")), (n // 2 + 9, 3, float("nan")),
+                              (n - 9, 4, float("inf"))):
+            c.k[b][t, :, 0] = -200
+            c.v[b][t, :, channel] = x
+
+
+def rise(c):
+    """One token takes all the weight; Inf and NaN in ordinary ones before and after it."""
+    for b, n in enumerate(c.lens):
+        if n < 60:
+            continue
+        c.k[b][n // 2 + 7, :, 0] = 200
+        for t, channel, x in ((1, 1, float("inf")), (n // 2 - 30, 2, float("-inf")), (n // 2 + 12, 3, float("nan")),
+                              (n - 7, 4, float("inf"))):
+            c.v[b][t, :, channel] = x
 
 
 # every query's first channel is 16: with scale 1/8, a key's first channel of -200 gives -400
@@ -228,3 +250,9 @@ def test_prefill(pk, dev, name, absent):
 @pytest.mark.parametrize("name", PREFILL)
 def test_prefill_specials(pk, dev, name):
     _prefill(pk, dev, name, specials)
+
+
+@pytest.mark.parametrize("change", [faint, rise])
+@pytest.mark.parametrize("name", [n for n in PREFILL if n.startswith("whole")])
+def test_prefill_specials_of_tiny_weight(pk, dev, name, change):
+    _prefill(pk, dev, name, change)
