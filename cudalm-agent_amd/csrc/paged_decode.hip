@@ -519,7 +519,7 @@ __global__ __launch_bounds__(64 * CH * SW) void paged_finish_kernel(const Decode
     for (int s = sw; s < parts.count; s += SW) {
       const float w = exp2_fast(a.part_ml[2 * at(s)] - M);
       l += w * a.part_ml[2 * at(s) + 1];
-      acc += w * a.part_o[at(s) * D + chunk * 64 + lane];
+      acc += joined(w, a.part_o[at(s) * D + chunk * 64 + lane]);
     }
     if (SW > 1) {
       shared.join.o[sw][wave % CH * 64 + lane] = acc;

@@ -180,6 +180,12 @@ __device__ __forceinline__ bool paged_sees(int t, int p, int window, int sinks) 
   return t <= p && (window <= 0 || t > p - window || t < sinks);
 }
 
+// A part's sum under the weight that the join gives it: Inf and NaN of values that a
+// row sees stay, also under a weight that has underflowed.
+__device__ __forceinline__ float joined(float w, float sum) {
+  return w == 0.0f && !(fabsf(sum) < __builtin_inff()) ? sum : w * sum;
+}
+
 // How many of `tiles` tiles each of at most `splits` parts takes: the least the
 // host asks for, more where that would leave tiles over.
 __device__ __forceinline__ int tiles_per_split(int tiles, int splits, int least) {

@@ -371,14 +371,18 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : D == 128 ? 3 : 4) void 
   l += __shfl_xor(l, 32);
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const size_t at = static_cast<size_t>(split) * a.tokens * a.heads + out_row;
-  if (a.part_o && real && half == 0) a.part_ml[2 * at] = m, a.part_ml[2 * at + 1] = l;
+  // -inf tells the join that there is nothing to read: no weight here, nor Inf or NaN
+  if (a.part_o && real && half == 0) {
+    a.part_ml[2 * at] = l == 0.0f && !special ? -__builtin_inff() : m;
+    a.part_ml[2 * at + 1] = l;
+  }
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) {
     f32x16_t r = o[dt];
     if (special) add_special(r, dt);
     if (!real) continue;
     if (a.part_o) {
-      if (begin >= end) continue;  // the join goes by l
+      if (begin >= end) continue;  // (l is zero)
       float* p = a.part_o + at * D + 32 * dt + 4 * half;
 #pragma unroll
       for (int y = 0; y < 4; ++y)
@@ -410,13 +414,13 @@ __global__ __launch_bounds__(256) void paged_prefill_join_kernel(const PrefillAr
   for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.part_ml[2 * (s * rows + row)]);
   float acc[E] = {}, l = 0;
   for (int s = 0; s < a.splits; ++s) {
-    const float ls = a.part_ml[2 * (s * rows + row) + 1];
-    if (ls == 0.0f) continue;  // no tokens: nothing was written
-    const float w = exp2_fast(a.part_ml[2 * (s * rows + row)] - M);
-    l += w * ls;
+    const float ms = a.part_ml[2 * (s * rows + row)];
+    if (ms == -__builtin_inff()) continue;
+    const float w = exp2_fast(ms - M);
+    l += w * a.part_ml[2 * (s * rows + row) + 1];
     const float* p = a.part_o + (s * rows + row) * D + lane * E;
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] += w * p[e];
+    for (int e = 0; e < E; ++e) acc[e] += joined(w, p[e]);
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   uint16_t* y = a.out + row * D + lane * E;

@@ -209,6 +209,12 @@ def test_decode_specials(pk, dev, name):
     _decode(pk, dev, name, specials)
 
 
+@pytest.mark.parametrize("change", [faint, rise])
+@pytest.mark.parametrize("name", DECODE)
+def test_decode_specials_of_tiny_weight(pk, dev, name, change):
+    _decode(pk, dev, name, change)
+
+
 # --- prefill ----------------------------------------------------------------------------
 
 # (D, P, dtype, new tokens, heads, kv heads, lengths, window, sinks): split over the length or not
@@ -253,6 +259,6 @@ def test_prefill_specials(pk, dev, name):
 
 
 @pytest.mark.parametrize("change", [faint, rise])
-@pytest.mark.parametrize("name", [n for n in PREFILL if n.startswith("whole")])
+@pytest.mark.parametrize("name", PREFILL)
 def test_prefill_specials_of_tiny_weight(pk, dev, name, change):
     _prefill(pk, dev, name, change)
