@@ -411,7 +411,7 @@ __global__ __launch_bounds__(64 * WV, 2) void paged_decode_kernel(const DecodeAr
             up = T::mfma(special_part<T>(v, ~0u), ones, up);
             down = T::mfma(special_part<T>(v, 0), ones, down);
           }
-          if (!real) continue;
+          if (!real || (whole && l == 0.0f)) continue;  // (no weight at all: zeros)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float add = (up[e] > 0 ? __builtin_inff() : 0.0f) + (down[e] > 0 ? -__builtin_inff() : 0.0f);
@@ -531,11 +531,11 @@ __global__ __launch_bounds__(64 * CH * SW) void paged_finish_kernel(const Decode
       for (int w = 0; w < SW; ++w)
         acc += shared.join.o[w][wave % CH * 64 + lane], l += shared.join.l[w];
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = 1.0f / l;
     const int j = row / a.group, heads = a.group * a.kv.kv_heads;
     uint16_t* y = static_cast<uint16_t*>(a.out) +
                   ((static_cast<size_t>(b) * a.new_tokens + j) * heads + h * a.group + row - j * a.group) * D;
-    y[chunk * 64 + lane] = static_cast<uint16_t>(T::pack(acc * inv, 0.0f));
+    y[chunk * 64 + lane] = static_cast<uint16_t>(T::pack(l == 0.0f ? 0.0f : acc * inv, 0.0f));
     return;
   }
   const int id = blockIdx.x - join_groups, bh = id / token_groups;

@@ -380,6 +380,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : D == 128 ? 3 : 4) void 
   for (int dt = 0; dt < DT; ++dt) {
     f32x16_t r = o[dt];
     if (special) add_special(r, dt);
+    // (no weight at all: zeros, whatever the values; parts keep theirs for the join)
+    if (special && l == 0.0f && !a.part_o) r = 0.0f;
     if (!real) continue;
     if (a.part_o) {
       if (begin >= end) continue;  // (l is zero)
@@ -422,7 +424,12 @@ __global__ __launch_bounds__(256) void paged_prefill_join_kernel(const PrefillAr
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] += joined(w, p[e]);
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  float inv = 1.0f / l;
+  if (l == 0.0f) {  // no weight at all: zeros, whatever the values
+    inv = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0;
+  }
   uint16_t* y = a.out + row * D + lane * E;
   if constexpr (E == 1) {
     y[0] = static_cast<uint16_t>(T::pack(acc[0] * inv, 0.0f));

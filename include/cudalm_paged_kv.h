@@ -29,8 +29,9 @@
  *
  * out = sum_t softmax_t(scale * q . k_t) v_t over the tokens it sees, and
  * zeros where it sees none (p < 0, absent pages) or where every score is
- * -inf. Whatever stands in places that no query sees (NaN included) has no
- * effect. Query head h reads key-value head h / (heads / kv_heads). Scores,
+ * -inf. Inf and NaN in the values that it sees count whatever their weights,
+ * also ones that underflow or are zero next to others. Whatever stands in places
+ * that no query sees (NaN included) has no effect. Query head h reads key-value head h / (heads / kv_heads). Scores,
  * statistics, sums and weights are fp32; outputs are rounded once.
  *
  * Ownership, threading and errors are those of cudalm_w4a16.h: the caller

@@ -2,7 +2,8 @@
 of eight waves, fixed splits and equal ranges of all tiles, one, two and four tiles of
 rows, whole and split chunks, each by the name of the kernel that runs. With windows,
 sinks, absent pages and weights; with Inf and NaN in values that rows see, whatever
-their weights. Expected results are float64, by the definition in the header; tolerances follow from the
+their weights (one that underflows, one of zero); with rows whose scores are all -inf.
+Expected results are float64, by the definition in the header; tolerances follow from the
 roundings (paged_reference.py)."""
 import pytest
 import torch
@@ -104,6 +105,18 @@ def rise(c):
         c.k[b][n // 2 + 7, :, 0] = 200
         for t, channel, x in ((1, 1, float("inf")), (n // 2 - 30, 2, float("-inf")), (n // 2 + 12, 3, float("nan")),
                               (n - 7, 4, float("inf"))):
+            c.v[b][t, :, channel] = x
+
+
+def lowest(c):
+    """Every score of the first key-value head is -inf; in the last one those of the first half are."""
+    for b, n in enumerate(c.lens):
+        if n < 60:
+            continue
+        c.k[b][:, 0, 0] = float("-inf")
+        if c.kv > 1:
+            c.k[b][:n // 2, c.kv - 1, 0] = float("-inf")
+        for t, channel, x in ((5, 1, float("inf")), (n // 2, 2, float("-inf")), (n - 4, 3, float("nan"))):
             c.v[b][t, :, channel] = x
 
 
@@ -215,6 +228,11 @@ def test_decode_specials_of_tiny_weight(pk, dev, name, change):
     _decode(pk, dev, name, change)
 
 
+@pytest.mark.parametrize("name", DECODE)
+def test_decode_of_scores_that_are_all_lowest(pk, dev, name):
+    _decode(pk, dev, name, lowest, weights=True)
+
+
 # --- prefill ----------------------------------------------------------------------------
 
 # (D, P, dtype, new tokens, heads, kv heads, lengths, window, sinks): split over the length or not
@@ -262,3 +280,8 @@ def test_prefill_specials(pk, dev, name):
 @pytest.mark.parametrize("name", PREFILL)
 def test_prefill_specials_of_tiny_weight(pk, dev, name, change):
     _prefill(pk, dev, name, change)
+
+
+@pytest.mark.parametrize("name", PREFILL)
+def test_prefill_of_scores_that_are_all_lowest(pk, dev, name):
+    _prefill(pk, dev, name, lowest)
