@@ -267,7 +267,8 @@ def decode(q, k, v, tables, lens, scale=None, window: int = 0, sinks: int = 0, w
     window > 0: a token sees the last `window` tokens (itself included) and the
     first `sinks`. With weights, what every cached token received (summed over
     the new tokens and a group's query heads) is added to them, or, with
-    accumulate=False, replaces them; max_len then has to hold."""
+    accumulate=False, replaces them; max_len then has to hold. (Drafted tokens that are
+    refused later count as well.)"""
     kv, index = _cache(k, v, tables, lens, weights)
     one = q.dim() == 3
     ts, hs = _rows(q, 1 if one else 2, None, k, index, "q")

@@ -110,7 +110,8 @@ class Chat:
         return self.model(torch.tensor(tokens, device="cuda"), self.caches, attend)
 
     def forget(self, count):
-        """Takes back the last tokens, whose drafts were refused."""
+        """Takes back the last tokens, whose drafts were refused (what their queries added to the
+        weights of others stays)."""
         self.length -= count
 
     def evict(self):
@@ -138,9 +139,11 @@ def _guess(history, count):
 
 
 def generate(model, prompt, count, drafts=4, temperature=0.0, seed=0, **chat):
-    """(`count` tokens after `prompt`, model steps taken, the chat). Drafted tokens
-    change neither the most likely continuation (temperature 0) nor, otherwise, the
-    distribution of the text, only the number of steps."""
+    """(`count` tokens after `prompt`, model steps taken, the chat). Without a budget, drafted
+    tokens change neither the most likely continuation (temperature 0) nor, otherwise, the
+    distribution of the text, only the number of steps. With one they do: the weights that
+    eviction goes by are summed before verification, over the queries of refused tokens too,
+    and evictions come after steps of another length."""
     g = torch.Generator(device="cuda").manual_seed(seed)
     chat = Chat(model, **chat)
     history, steps = list(prompt), 0

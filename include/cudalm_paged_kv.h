@@ -102,7 +102,9 @@ int cudalm_paged_append(const cudalm_paged_kv* kv, const void* k, const void* v,
  * weights_mode: 0 none; CUDALM_PAGED_WEIGHTS_SET / _ADD: the weight of every
  * token t < lens[b], summed over the new tokens and the query heads of its
  * key-value head, replaces / is added to kv->weights (zero for tokens that no
- * query sees). A page that two sequences of the call share gets the weights
+ * query sees). That counts every new token of the call: with drafted tokens, also those
+ * that are refused afterwards (to leave them out, decode the accepted ones alone with
+ * weights, after verification). A page that two sequences of the call share gets the weights
  * of one of them, unspecified which. */
 #define CUDALM_PAGED_WEIGHTS_SET 1
 #define CUDALM_PAGED_WEIGHTS_ADD 2
