@@ -358,16 +358,21 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : D == 128 ? 3 : 4) void 
       if (up[e] > 0 || down[e] > 0)
         r[e] = (up[e] > 0 ? __builtin_inff() : 0.0f) + (down[e] > 0 ? -__builtin_inff() : 0.0f);
   };
-  float all = 0;  // NaN if one of the sums is not finite
+  f32x16_t most = o[0];  // of the sums' sizes, NaN if one of them is
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) all = __builtin_fmaf(o[dt][e], 0.0f, all);
-  votes[wave] = __any(special != 0 || all != all);
+    for (int e = 0; e < 16; ++e) most[e] = __builtin_elementwise_maximum(fabsf(most[e]), fabsf(o[dt][e]));
+#pragma unroll
+  for (int x = 8; x > 0; x >>= 1)
+#pragma unroll
+    for (int e = 0; e < x; ++e) most[e] = __builtin_elementwise_maximum(most[e], most[e + x]);
+  votes[wave] = __any(special != 0 || !(most[0] < __builtin_inff()));
   __syncthreads();
   special = 0;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) special |= votes[w];
+  special = __builtin_amdgcn_readfirstlane(special);
   l += __shfl_xor(l, 32);
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const size_t at = static_cast<size_t>(split) * a.tokens * a.heads + out_row;
@@ -379,9 +384,11 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : D == 128 ? 3 : 4) void 
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) {
     f32x16_t r = o[dt];
-    if (special) add_special(r, dt);
-    // (no weight at all: zeros, whatever the values; parts keep theirs for the join)
-    if (special && l == 0.0f && !a.part_o) r = 0.0f;
+    if (special) {
+      add_special(r, dt);
+      // (no weight at all: zeros, whatever the values; parts keep theirs for the join)
+      if (l == 0.0f && !a.part_o) r = 0.0f;
+    }
     if (!real) continue;
     if (a.part_o) {
       if (begin >= end) continue;  // (l is zero)
