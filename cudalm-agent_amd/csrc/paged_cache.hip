@@ -284,7 +284,7 @@ constexpr int kMove = 32;  // kept tokens of a copying workgroup
 // their key rows, and eight tokens' values of a channel per thread, one interleaved
 // unit of the fresh page. Bound by bytes: every line of the old values that holds a
 // kept token is read, which for a quarter kept is nine in ten. 12 x 8 heads cut from
-// up to 30000 to 8000 tokens: 195-214 us (box to box); counters show 711 MB fetched and
+// up to 30000 to 8000 tokens: 195-214 us (card to card); counters show 711 MB fetched and
 // 396 written, 5.2 TB/s, a copy's rate. (A thread per place took 413.)
 template <int D>
 __global__ __launch_bounds__(256) void paged_compact_kernel(const EvictArgs a) {

@@ -28,7 +28,7 @@
 // tokens and multiply 0.3 MFLOP with them. 64 sequences of up to 8192 tokens (678 MB):
 // 127-133 us and 6 for the join, 5.1 TB/s together, what a 1 GiB copy reaches; counters
 // show 708 MB fetched. Five new tokens of 16 sequences of up to 5001, 32 heads on 8 of
-// 128, with weights (215 MB): 52-65 us (box to box) and 16 for join and weights. One
+// 128, with weights (215 MB): 52-65 us (card to card) and 16 for join and weights. One
 // sequence of 777 tokens: 9 us and 4, chains of loads (table, keys, products, join).
 
 #include <cstdint>
@@ -488,7 +488,9 @@ struct Parts {
 // The others: weights[t] (+)= sum over rows of 2^(score - M) / l, for four tokens of a
 // (sequence, head) per thread, with the rows' M and l joined from the parts. Five new
 // tokens of 16 sequences of up to 5001, 32 heads on 8 of 128: 16 us, where a kernel
-// for each of the two took 10 + 10.
+// for each of the two took 10 + 10. A row's parts are walked by one lane, which many
+// parts of few rows wait for: one sequence of 32768 tokens, 8 heads on 2 of 256, takes 61
+// us with weights, 29 without.
 template <typename T, int D, int CH, int SW>
 __global__ __launch_bounds__(64 * CH * SW) void paged_finish_kernel(const DecodeArgs a,
                                                                     unsigned join_groups,

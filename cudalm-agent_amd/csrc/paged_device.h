@@ -59,8 +59,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 // finite, the product takes them without those (finite_part), and the rows that
 // do see them get theirs from two more products of whole numbers: how many
 // tokens that a row sees (ones in `seen_operand`) hold +Inf or NaN, and how
-// many -Inf or NaN (special_part); Inf is added for the one,
-// -Inf for the other.
+// many -Inf or NaN (special_part). The one gives Inf, the other -Inf, whatever the
+// tokens' weights: also where they underflow, in a part or in the join of parts, so
+// that results do not depend on how a call is cut.
 // Both halves of a word at once: an all-ones exponent plus its lowest bit carries
 // into bit 15, a mantissa that is not zero plus its mask into the exponent.
 template <typename T>

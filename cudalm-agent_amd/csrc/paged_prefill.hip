@@ -21,7 +21,7 @@
 // The matrix and the vector unit bound it together: 32 tokens of 128 channels are 512
 // cycles of products per wave, some 600 of exponentials, maxima and rounding, and the
 // LDS reads of four waves fill 512 more. A chunk of 2048 tokens at 14336, 8 query heads on 2
-// of 256: 233-257 us (box to box) and 15 for the join, 1.08 PFLOP/s at best, where an
+// of 256: 233-257 us (card to card) and 15 for the join, 1.08 PFLOP/s at best, where an
 // 8192-wide product of the library reaches 1.37. Two tiles of rows per wave halve the LDS
 // reads but need more registers than two waves per SIMD leave (a 2048-token chunk at 6144,
 // 32 heads on 8 of 128: 408 us, 261-288 with one). 8 prompts of up to 1000 tokens with a window

@@ -102,10 +102,10 @@ int cudalm_paged_append(const cudalm_paged_kv* kv, const void* k, const void* v,
  * weights_mode: 0 none; CUDALM_PAGED_WEIGHTS_SET / _ADD: the weight of every
  * token t < lens[b], summed over the new tokens and the query heads of its
  * key-value head, replaces / is added to kv->weights (zero for tokens that no
- * query sees). That counts every new token of the call: with drafted tokens, also those
- * that are refused afterwards (to leave them out, decode the accepted ones alone with
- * weights, after verification). A page that two sequences of the call share gets the weights
- * of one of them, unspecified which. */
+ * query sees). That counts every new token of the call: with drafted tokens,
+ * also those that are refused afterwards (to leave them out, decode the accepted
+ * ones alone with weights, after verification). A page that two sequences of the
+ * call share gets the weights of one of them, unspecified which. */
 #define CUDALM_PAGED_WEIGHTS_SET 1
 #define CUDALM_PAGED_WEIGHTS_ADD 2
 size_t cudalm_paged_decode_workspace_bytes(const cudalm_paged_kv* kv, const cudalm_paged_query* q,
@@ -133,10 +133,13 @@ int cudalm_paged_prefill(const cudalm_paged_kv* kv, const cudalm_paged_query* q,
  * copied, in their order, into the pages of dst_tables [batch][dst_pages],
  * and their old positions written to kept [batch][kv_heads][keep] (-1 past
  * the last); new_lens[b] is their number, and may be kv->lens itself. Other
- * places of the pages stay as they are. No page of dst_tables may be read through kv->tables by the same
- * call; dst_pages * P >= keep. Entries of dst_tables outside [0, num_pages)
- * drop the tokens that belong there from the copy. max_len: no sequence is
- * expected to be longer (<= 0: max_pages * page_size); only speed goes by it. */
+ * places of the pages stay as they are. No page of dst_tables may be read
+ * through kv->tables by the same call; dst_pages * P >= keep. Entries of
+ * dst_tables outside [0, num_pages) drop the tokens that belong there from the
+ * copy. max_len: no sequence is expected to be longer (<= 0: max_pages *
+ * page_size); only speed goes by it. Every head keeps tokens of its own, so a
+ * place of the new cache stands for another old position in each; positions,
+ * windows and sinks of later calls count places. */
 size_t cudalm_paged_evict_workspace_bytes(const cudalm_paged_kv* kv, int max_len);
 int cudalm_paged_evict(const cudalm_paged_kv* kv, const int32_t* dst_tables, int dst_pages,
                        int keep, int sinks, int recent, int32_t* kept, int32_t* new_lens,
