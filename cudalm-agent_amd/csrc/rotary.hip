@@ -1,0 +1,431 @@
+// Rotary positions: rows of heads rotated by their positions, and new tokens' keys
+// rotated on their way into the pages of the paged cache.
+//
+// The cosines and sines of a token's pairs are those of all its heads: a workgroup takes
+// up to eight tokens, makes theirs once in LDS, and every thread keeps those of eight
+// pairs of one token in registers while it walks over heads. p f / pi is made in 64 bits
+// (31 bits of position times 24 of frequency), reduced there to [-1, 1], and only then
+// rounded to fp32 for the sine: positions of 10^6 are as exact as small ones.
+
+#include "cudalm_rotary.h"
+
+#include "paged_device.h"
+
+namespace cudalm_hip {
+namespace {
+
+constexpr int kTokens = 8;   // of a workgroup at most; a group of eight values in the cache
+constexpr int kThreads = 256;
+
+// How rows are turned. Axis of pair i: bits 2 i of `axis`.
+struct Turn {
+  const float* freqs;
+  const int32_t* positions;  // [axes][tokens], or NULL: consecutive from the first token's
+  long long tokens;
+  int pairs, adjacent;
+  float scale;
+  uint32_t axis[CUDALM_ROTARY_MAX_PAIRS / 16];
+};
+
+// cosine and sine of `count` tokens' pairs: row `row0` on, places p0 on.
+__device__ __forceinline__ void make_angles(float2* cs, const Turn& a, long long row0, int p0,
+                                            int count) {
+  for (int i = threadIdx.x; i < count * a.pairs; i += kThreads) {
+    const int t = i / a.pairs, pair = i - t * a.pairs;
+    int p = p0 + t;
+    if (a.positions) {
+      const int axis = (a.axis[pair >> 4] >> (2 * (pair & 15))) & 3;
+      p = a.positions[axis * a.tokens + row0 + t];
+    }
+    const double half_turns = static_cast<double>(p) * static_cast<double>(a.freqs[pair]) *
+                              0.318309886183790671537767526745;
+    const float r = static_cast<float>(half_turns - 2.0 * rint(0.5 * half_turns));
+    float s, c;
+    sincospif(r, &s, &c);
+    cs[i] = float2{c * a.scale, s * a.scale};
+  }
+}
+
+// Eight pairs, or 16 channels that are copied, of one token: where they are in a head.
+struct Chunk {
+  int at0, at1;  // channels; at1 < 0: none (eight channels are left to copy)
+  bool turned;
+};
+__device__ __forceinline__ Chunk chunk_of(const Turn& a, int c, int D) {
+  const int turned = a.pairs / 8;
+  Chunk r;
+  r.turned = c < turned;
+  if (r.turned) {
+    r.at0 = a.adjacent ? 16 * c : 8 * c;
+    r.at1 = a.adjacent ? 16 * c + 8 : a.pairs + 8 * c;
+  } else {
+    r.at0 = 16 * c;
+    r.at1 = r.at0 + 8 < D ? r.at0 + 8 : -1;
+  }
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void turn_pair(const float2 cs, float& x0, float& x1) {
+  const float y0 = __builtin_fmaf(x0, cs.x, -(x1 * cs.y));
+  x1 = __builtin_fmaf(x1, cs.x, x0 * cs.y);
+  x0 = y0;
+}
+
+template <typename T>
+__device__ __forceinline__ float upper(uint32_t w) {
+  return T::value(static_cast<uint16_t>(w >> 16));
+}
+template <typename T>
+__device__ __forceinline__ float lower(uint32_t w) {
+  return T::value(static_cast<uint16_t>(w));
+}
+
+// Turns the pairs that u and v hold: of channels at0 .. and at1 .. (element e of both
+// is a pair), or pairs side by side.
+template <typename T>
+__device__ __forceinline__ void turn_chunk(bool adjacent, const float2* cs, u32x4_t& u, u32x4_t& v) {
+  if (adjacent) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float x0 = lower<T>(u[e]), x1 = upper<T>(u[e]);
+      turn_pair<T>(cs[e], x0, x1);
+      u[e] = T::pack(x0, x1);
+      x0 = lower<T>(v[e]), x1 = upper<T>(v[e]);
+      turn_pair<T>(cs[4 + e], x0, x1);
+      v[e] = T::pack(x0, x1);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float x0 = lower<T>(u[e]), x1 = lower<T>(v[e]), z0 = upper<T>(u[e]), z1 = upper<T>(v[e]);
+      turn_pair<T>(cs[2 * e], x0, x1);
+      turn_pair<T>(cs[2 * e + 1], z0, z1);
+      u[e] = T::pack(x0, z0);
+      v[e] = T::pack(x1, z1);
+    }
+  }
+}
+
+__device__ __forceinline__ u32x4_t load16(const uint16_t* p) {
+  return *reinterpret_cast<const u32x4_t*>(p);
+}
+__device__ __forceinline__ void store16(uint16_t* p, u32x4_t v) { *reinterpret_cast<u32x4_t*>(p) = v; }
+
+struct RotateArgs {
+  Turn turn;
+  const uint16_t* x;
+  uint16_t* out;
+  long long x_token, x_head, out_token, out_head;
+  int heads, D, each;  // each: tokens of a workgroup
+};
+
+// 16 bytes at a time.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void rotate_kernel(const RotateArgs a) {
+  extern __shared__ float2 angles[];
+  const long long row0 = static_cast<long long>(blockIdx.x) * a.each;
+  const long long left = a.turn.tokens - row0;
+  const int count = left < a.each ? static_cast<int>(left) : a.each;
+  make_angles(angles, a.turn, row0, 0, count);
+  __syncthreads();
+  const int chunks = (a.D + 15) / 16, items = count * chunks, together = kThreads / items;
+  const int first = threadIdx.x / items, item = threadIdx.x - first * items;
+  if (first >= together) return;
+  const int t = item / chunks;
+  const Chunk c = chunk_of(a.turn, item - t * chunks, a.D);
+  float2 cs[8];
+  if (c.turned)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) cs[e] = angles[t * a.turn.pairs + 8 * (item - t * chunks) + e];
+  const uint16_t* x = a.x + (row0 + t) * a.x_token;
+  uint16_t* out = a.out + (row0 + t) * a.out_token;
+  for (int h = first; h < a.heads; h += together) {
+    u32x4_t u = load16(x + h * a.x_head + c.at0), v = {0, 0, 0, 0};
+    if (c.at1 >= 0) v = load16(x + h * a.x_head + c.at1);
+    if (c.turned) turn_chunk<T>(a.turn.adjacent, cs, u, v);
+    store16(out + h * a.out_head + c.at0, u);
+    if (c.at1 >= 0) store16(out + h * a.out_head + c.at1, v);
+  }
+}
+
+// A pair, or a channel that is copied, at a time: any alignment and size.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void rotate_any_kernel(const RotateArgs a) {
+  extern __shared__ float2 angles[];
+  const long long row0 = static_cast<long long>(blockIdx.x) * a.each;
+  const long long left = a.turn.tokens - row0;
+  const int count = left < a.each ? static_cast<int>(left) : a.each;
+  make_angles(angles, a.turn, row0, 0, count);
+  __syncthreads();
+  const int pairs = a.turn.pairs, items = a.D - pairs;  // of a head
+  for (long long i = threadIdx.x; i < static_cast<long long>(count) * a.heads * items; i += kThreads) {
+    const int c = static_cast<int>(i % items);
+    const long long th = i / items;
+    const int h = static_cast<int>(th % a.heads), t = static_cast<int>(th / a.heads);
+    const uint16_t* x = a.x + (row0 + t) * a.x_token + h * a.x_head;
+    uint16_t* out = a.out + (row0 + t) * a.out_token + h * a.out_head;
+    if (c < pairs) {
+      const int c0 = a.turn.adjacent ? 2 * c : c, c1 = a.turn.adjacent ? 2 * c + 1 : pairs + c;
+      float x0 = T::value(x[c0]), x1 = T::value(x[c1]);
+      turn_pair<T>(angles[t * pairs + c], x0, x1);
+      const uint32_t y = T::pack(x0, x1);
+      out[c0] = static_cast<uint16_t>(y);
+      out[c1] = static_cast<uint16_t>(y >> 16);
+    } else {
+      out[pairs + c] = x[pairs + c];
+    }
+  }
+}
+
+struct RotaryAppendArgs {
+  Turn turn;
+  PagedView kv;
+  uint16_t* ck;
+  uint16_t* cv;
+  float* weights;
+  const uint16_t* k;
+  const uint16_t* v;
+  const uint16_t* q;
+  uint16_t* out;
+  long long k_token, k_head, v_token, v_head, q_token, q_head, out_token, out_head;
+  const int32_t* cu;
+  int each, heads;  // each: new tokens of every sequence where cu is NULL
+};
+
+// One workgroup per eight positions (aligned: one interleaved group of values) of a
+// sequence; units are numbered as in paged_append_kernel. Positions before the first
+// place count here too, since their queries are rotated.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void rotary_append_kernel(const RotaryAppendArgs a) {
+  extern __shared__ float2 angles[];
+  int b, begin, n, g;
+  if (a.cu) {
+    b = sequence_of(a.cu, a.kv.batch, blockIdx.x, 1, 8, 2);
+    if (b < 0) return;
+    begin = a.cu[b];
+    const int end = a.cu[b + 1];
+    n = begin >= 0 && end > begin ? end - begin : 0;
+    g = static_cast<int>(blockIdx.x) - (begin / 8 + 2 * b);
+  } else {
+    const int units = a.each / 8 + 2;
+    b = blockIdx.x / units;
+    begin = b * a.each;
+    n = a.each;
+    g = blockIdx.x % units;
+  }
+  if (n < 1 || n > a.turn.tokens - begin || g < 0) return;  // (g < 0 where cu does not ascend)
+  const int length = a.kv.length(b), first = length - n;  // position of row `begin`
+  const int p0 = ((first >> 3) + g) * 8;
+  if (p0 >= length) return;
+  const int lo = first > p0 ? first - p0 : 0, hi = length - p0 < 8 ? length - p0 : 8;
+  const long long row0 = static_cast<long long>(begin) + p0 + lo - first;  // of token lo
+  const int count = hi - lo;
+  make_angles(angles, a.turn, row0, p0 + lo, count);
+  const int page = p0 >= 0 ? a.kv.page(b, p0 >> a.kv.page_shift) : -1;
+  const int P = 1 << a.kv.page_shift, off = p0 & (P - 1);
+  __syncthreads();
+  // queries and keys: tokens x 16-channel chunks x heads
+  constexpr int kChunks = D / 16;
+  const int items = count * kChunks, together = kThreads / items;
+  const int start = threadIdx.x / items, item = threadIdx.x - start * items;
+  const int t = item / kChunks;
+  if (start < together) {
+    const Chunk c = chunk_of(a.turn, item % kChunks, D);
+    float2 cs[8];
+    if (c.turned)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) cs[e] = angles[t * a.turn.pairs + 8 * (item % kChunks) + e];
+    const int last = a.heads + (page >= 0 ? a.kv.kv_heads : 0);
+    for (int h = start; h < last; h += together) {
+      const uint16_t* src;
+      uint16_t* dst;
+      if (h < a.heads) {
+        src = a.q + (row0 + t) * a.q_token + h * a.q_head;
+        dst = a.out + (row0 + t) * a.out_token + h * a.out_head;
+      } else {
+        src = a.k + (row0 + t) * a.k_token + (h - a.heads) * a.k_head;
+        dst = a.ck + ((static_cast<size_t>(page) * a.kv.kv_heads + h - a.heads) * P + off + lo + t) * D;
+      }
+      u32x4_t u = load16(src + c.at0), v = load16(src + c.at1);
+      if (c.turned) turn_chunk<T>(a.turn.adjacent, cs, u, v);
+      store16(dst + c.at0, u);
+      store16(dst + c.at1, v);
+    }
+  }
+  if (page < 0) return;
+  // values: two channels of the group's tokens, and the weights
+  for (int i = threadIdx.x; i < a.kv.kv_heads * (D / 2); i += kThreads) {
+    const int h = i / (D / 2), d = 2 * (i % (D / 2));
+    const size_t place = (static_cast<size_t>(page) * a.kv.kv_heads + h) * P + off;
+    if (a.weights && d < 16 && d / 2 >= lo && d / 2 < hi) a.weights[place + d / 2] = 0.0f;
+    uint16_t* cv = a.cv + place * D;
+    uint32_t pair[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e >= lo && e < hi)
+        pair[e] = *reinterpret_cast<const uint32_t*>(a.v + (row0 + e - lo) * a.v_token + h * a.v_head + d);
+    if (lo == 0 && hi == 8) {
+      u32x4_t even, odd;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        even[e] = (pair[2 * e] & 0xFFFFu) | (pair[2 * e + 1] << 16);
+        odd[e] = (pair[2 * e] >> 16) | (pair[2 * e + 1] & 0xFFFF0000u);
+      }
+      store16(cv + 8 * d, even);
+      store16(cv + 8 * d + 8, odd);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e >= lo && e < hi) {
+          cv[8 * d + e] = static_cast<uint16_t>(pair[e]);
+          cv[8 * d + 8 + e] = static_cast<uint16_t>(pair[e] >> 16);
+        }
+    }
+  }
+}
+
+// Checks a rotary plan and lays it out for the kernels.
+int turn_of(const cudalm_rotary* r, const int32_t* positions, long long tokens, Turn* turn) {
+  if (!r) return CUDALM_W4A16_ENULL;
+  if (r->pairs < 1 || r->pairs > CUDALM_ROTARY_MAX_PAIRS || r->axes < 1 ||
+      r->axes > CUDALM_ROTARY_MAX_AXES || !(r->adjacent == 0 || r->adjacent == 1) ||
+      !(r->turns == 0 || r->turns == 1))
+    return CUDALM_W4A16_EINVAL;
+  int left[CUDALM_ROTARY_MAX_AXES] = {};
+  long long sum = 0;
+  for (int i = 0; i < r->axes; ++i) {
+    left[i] = r->axes == 1 ? r->pairs : r->sections[i];
+    if (left[i] < 0) return CUDALM_W4A16_EINVAL;
+    sum += left[i];
+  }
+  if (sum != r->pairs) return CUDALM_W4A16_EINVAL;
+  if (!r->freqs) return CUDALM_W4A16_ENULL;
+  if (!aligned(r->freqs, 4) || !aligned(positions, 4)) return CUDALM_W4A16_EALIGN;
+  *turn = {};
+  turn->freqs = r->freqs;
+  turn->positions = positions;
+  turn->tokens = tokens;
+  turn->pairs = r->pairs;
+  turn->adjacent = r->adjacent;
+  turn->scale = r->scale;
+  int axis = 0;
+  for (int i = 0; i < r->pairs; ++i) {
+    while (left[axis] == 0) axis = (axis + 1) % r->axes;
+    --left[axis];
+    turn->axis[i >> 4] |= static_cast<uint32_t>(axis) << (2 * (i & 15));
+    if (r->turns) axis = (axis + 1) % r->axes;
+  }
+  return CUDALM_W4A16_OK;
+}
+
+bool wide_rows(const cudalm_rotary_rows* q) {
+  return aligned(q->x, 16) && aligned(q->out, 16) && q->x_token_stride % 8 == 0 &&
+         q->x_head_stride % 8 == 0 && q->out_token_stride % 8 == 0 && q->out_head_stride % 8 == 0;
+}
+
+// In place, an element's place has to be the same for reading and writing.
+bool in_place_as_it_is(const cudalm_rotary_rows* q) {
+  return q->x != q->out ||
+         (q->x_token_stride == q->out_token_stride && q->x_head_stride == q->out_head_stride);
+}
+
+template <typename T>
+int launch_append(int D, const RotaryAppendArgs& a, unsigned units, hipStream_t stream) {
+  const size_t lds = sizeof(float2) * kTokens * a.turn.pairs;
+  if (D == 64)
+    rotary_append_kernel<T, 64><<<units, kThreads, lds, stream>>>(a);
+  else if (D == 128)
+    rotary_append_kernel<T, 128><<<units, kThreads, lds, stream>>>(a);
+  else
+    rotary_append_kernel<T, 256><<<units, kThreads, lds, stream>>>(a);
+  return launch_status();
+}
+
+}  // namespace
+}  // namespace cudalm_hip
+
+using namespace cudalm_hip;
+
+extern "C" int cudalm_rotary_rotate(const cudalm_rotary* rotary, const cudalm_rotary_rows* rows,
+                                    int tokens, int head_dim, int type, const int32_t* positions,
+                                    hipStream_t stream) {
+  RotateArgs a;
+  if (const int rc = turn_of(rotary, positions, tokens, &a.turn)) return rc;
+  if (!rows) return CUDALM_W4A16_ENULL;
+  if (tokens < 0 || rows->heads < 0 || head_dim < 2 * rotary->pairs ||
+      head_dim > 2 * CUDALM_ROTARY_MAX_PAIRS ||
+      (type != CUDALM_PAGED_BF16 && type != CUDALM_PAGED_F16) || !in_place_as_it_is(rows))
+    return CUDALM_W4A16_EINVAL;
+  if (tokens == 0 || rows->heads == 0) return CUDALM_W4A16_OK;
+  if (!rows->x || !rows->out || !positions) return CUDALM_W4A16_ENULL;
+  if (!aligned(rows->x, 2) || !aligned(rows->out, 2)) return CUDALM_W4A16_EALIGN;
+  a.x = static_cast<const uint16_t*>(rows->x);
+  a.out = static_cast<uint16_t*>(rows->out);
+  a.x_token = rows->x_token_stride;
+  a.x_head = rows->x_head_stride;
+  a.out_token = rows->out_token_stride;
+  a.out_head = rows->out_head_stride;
+  a.heads = rows->heads;
+  a.D = head_dim;
+  // Fewer tokens per workgroup until the chip has some for every CU.
+  a.each = kTokens;
+  while (a.each > 1 && (static_cast<long long>(tokens) + a.each - 1) / a.each < 2LL * cu_count()) a.each /= 2;
+  const long long groups = (static_cast<long long>(tokens) + a.each - 1) / a.each;
+  if (groups >= kMaxGemmTiles) return CUDALM_W4A16_ERANGE;
+  const size_t lds = sizeof(float2) * a.each * rotary->pairs;
+  const bool wide = wide_rows(rows) && rotary->pairs % 8 == 0 && head_dim % 8 == 0;
+  const bool bf16 = type == CUDALM_PAGED_BF16;
+  auto kernel = wide ? (bf16 ? rotate_kernel<PagedBf16> : rotate_kernel<PagedF16>)
+                     : (bf16 ? rotate_any_kernel<PagedBf16> : rotate_any_kernel<PagedF16>);
+  kernel<<<static_cast<unsigned>(groups), kThreads, lds, stream>>>(a);
+  return launch_status();
+}
+
+extern "C" int cudalm_rotary_append(const cudalm_rotary* rotary, const cudalm_paged_kv* kv,
+                                    const void* k, const void* v, int64_t k_token_stride,
+                                    int64_t k_head_stride, int64_t v_token_stride,
+                                    int64_t v_head_stride, const cudalm_rotary_rows* queries,
+                                    const int32_t* positions, const int32_t* cu_new, int tokens,
+                                    hipStream_t stream) {
+  if (const int rc = paged_check(kv)) return rc;
+  RotaryAppendArgs a = {};
+  if (const int rc = turn_of(rotary, positions, tokens, &a.turn)) return rc;
+  if (tokens < 0 || (!cu_new && tokens % kv->batch) || rotary->pairs % 8 ||
+      2 * rotary->pairs > kv->head_dim)
+    return CUDALM_W4A16_EINVAL;
+  if (queries && (queries->heads < 1 || !in_place_as_it_is(queries))) return CUDALM_W4A16_EINVAL;
+  if (tokens == 0) return CUDALM_W4A16_OK;
+  if (!k || !v || (queries && (!queries->x || !queries->out))) return CUDALM_W4A16_ENULL;
+  if (!aligned(k, 16) || !aligned(v, 16) || !aligned(cu_new, 4) || k_token_stride % 8 ||
+      k_head_stride % 8 || v_token_stride % 8 || v_head_stride % 8 || (queries && !wide_rows(queries)))
+    return CUDALM_W4A16_EALIGN;
+  const long long units = cu_new ? static_cast<long long>(tokens) / 8 + 2LL * kv->batch
+                                 : static_cast<long long>(kv->batch) * (tokens / kv->batch / 8 + 2);
+  if (units >= kMaxGemmTiles || kv->kv_heads >= (1 << 22) || (queries && queries->heads >= (1 << 22)))
+    return CUDALM_W4A16_ERANGE;
+  a.kv = view_of(kv);
+  a.ck = static_cast<uint16_t*>(kv->k);
+  a.cv = static_cast<uint16_t*>(kv->v);
+  a.weights = kv->weights;
+  a.k = static_cast<const uint16_t*>(k);
+  a.v = static_cast<const uint16_t*>(v);
+  a.k_token = k_token_stride;
+  a.k_head = k_head_stride;
+  a.v_token = v_token_stride;
+  a.v_head = v_head_stride;
+  if (queries) {
+    a.q = static_cast<const uint16_t*>(queries->x);
+    a.out = static_cast<uint16_t*>(queries->out);
+    a.q_token = queries->x_token_stride;
+    a.q_head = queries->x_head_stride;
+    a.out_token = queries->out_token_stride;
+    a.out_head = queries->out_head_stride;
+    a.heads = queries->heads;
+  }
+  a.cu = cu_new;
+  a.each = cu_new ? 0 : tokens / kv->batch;
+  return kv->type == CUDALM_PAGED_BF16
+             ? launch_append<PagedBf16>(kv->head_dim, a, static_cast<unsigned>(units), stream)
+             : launch_append<PagedF16>(kv->head_dim, a, static_cast<unsigned>(units), stream);
+}
