@@ -49,6 +49,11 @@ struct PagedF16 {
   }
 };
 
+__device__ __forceinline__ u32x4_t load16(const uint16_t* p) {
+  return *reinterpret_cast<const u32x4_t*>(p);
+}
+__device__ __forceinline__ void store16(uint16_t* p, u32x4_t v) { *reinterpret_cast<u32x4_t*>(p) = v; }
+
 // Running maxima start here and not at -inf, so that differences of maxima
 // are never inf - inf; no finite score is below it.
 constexpr float kLowest = -3.402823466e38f;

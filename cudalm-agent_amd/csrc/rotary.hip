@@ -107,11 +107,6 @@ __device__ __forceinline__ void turn_chunk(bool adjacent, const float2* cs, u32x
   }
 }
 
-__device__ __forceinline__ u32x4_t load16(const uint16_t* p) {
-  return *reinterpret_cast<const u32x4_t*>(p);
-}
-__device__ __forceinline__ void store16(uint16_t* p, u32x4_t v) { *reinterpret_cast<u32x4_t*>(p) = v; }
-
 struct RotateArgs {
   Turn turn;
   const uint16_t* x;
