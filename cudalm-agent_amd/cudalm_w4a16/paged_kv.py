@@ -33,6 +33,8 @@ _SIGS = {
     "cudalm_paged_append": ([_P, _P, _P, _L, _L, _L, _L, _P, _I, _P], _I),
     "cudalm_paged_decode_workspace_bytes": ([_P, _P, _I, _I], _SZ),
     "cudalm_paged_decode": ([_P, _P, _I, _I, _P, _SZ, _P], _I),
+    "cudalm_paged_decode_shared_workspace_bytes": ([_P, _P, _P, _I], _SZ),
+    "cudalm_paged_decode_shared": ([_P, _P, _P, _I, _P, _SZ, _P], _I),
     "cudalm_paged_prefill_workspace_bytes": ([_P, _P, _I], _SZ),
     "cudalm_paged_prefill": ([_P, _P, _P, _I, _P, _SZ, _P], _I),
     "cudalm_paged_evict_workspace_bytes": ([_P, _I], _SZ),
@@ -88,9 +90,16 @@ class Query(ctypes.Structure):
                 ("window", ctypes.c_int), ("sinks", ctypes.c_int), ("max_len", ctypes.c_int)]
 
 
+class Groups(ctypes.Structure):
+    """struct cudalm_paged_groups."""
+    _fields_ = [("cu", ctypes.c_void_p), ("shared", ctypes.c_void_p), ("count", ctypes.c_int),
+                ("max_shared", ctypes.c_int)]
+
+
 # the same as bytes: one pack instead of a ctypes store per field
 _pack_kv = struct.Struct("5P7i4x").pack
 _pack_query = struct.Struct("2P2qifiii4x").pack
+_pack_groups = struct.Struct("2P2i").pack
 
 
 def _need(ok, what):
@@ -193,6 +202,12 @@ def _empty(shape, dtype, index, stream):
         return torch.empty(shape, dtype=dtype, device=_devices(index))
 
 
+def _current_device() -> int:
+    import torch
+
+    return torch.cuda.current_device()
+
+
 def _workspace(nbytes, workspace, index, stream):
     """(address, bytes) of the caller's workspace or of a new one, with what holds it."""
     if workspace is not None:
@@ -284,6 +299,43 @@ def decode(q, k, v, tables, lens, scale=None, window: int = 0, sinks: int = 0, w
     at, size, held = _workspace(need, workspace, index, stream)
     rc = _lib.cudalm_paged_decode(kv, query, Q, mode, at, size, _stream(stream))
     _check(rc, "cudalm_paged_decode")
+    return out
+
+
+def decode_shared(q, k, v, tables, lens, cu_groups, shared, scale=None, window: int = 0, sinks: int = 0,
+                  max_len=None, max_shared=None, out=None, workspace=None, stream=None):
+    """decode() for a batch in which groups of sequences begin with the same tokens,
+    which are read once for all of a group's queries. Group g is sequences cu_groups[g] ..
+    cu_groups[g + 1] - 1 (int32 [G + 1], G at most the batch; the others share nothing); its
+    first shared[g] tokens (int32 [G], any number) are those in the pages of its first
+    sequence, whatever the other sequences' tables hold there. max_shared is what the
+    caller knows of the longest prefix. Other arguments as in decode()."""
+    kv, index = _cache(k, v, tables, lens, None)
+    if index != _current_device():
+        import torch
+
+        with torch.cuda.device(index):
+            return decode_shared(q, k, v, tables, lens, cu_groups, shared, scale, window, sinks, max_len, max_shared,
+                                 out, workspace, stream)
+    one = q.dim() == 3
+    ts, hs = _rows(q, 1 if one else 2, None, k, index, "q")
+    if q.shape[0] != tables.shape[0]:
+        raise ValueError("paged_kv: q has one entry per sequence")
+    G = shared.shape[0] if shared.dim() == 1 else -1
+    _int32(shared, (G,), "shared", index)
+    _int32(cu_groups, (G + 1,), "cu_groups", index)
+    if max_shared is not None:
+        _need_ints(max_shared=max_shared)
+    Q = 1 if one else q.shape[1]
+    out = _out_like(q, out, index, stream)
+    query = _query(q, out, ts, hs, scale, window, sinks, max_len)
+    groups = _pack_groups(cu_groups.data_ptr(), shared.data_ptr(), G, max_shared or 0)
+    need = 0
+    if workspace is None:
+        need = _lib.cudalm_paged_decode_shared_workspace_bytes(kv, query, groups, Q)
+    at, size, held = _workspace(need, workspace, index, stream)
+    rc = _lib.cudalm_paged_decode_shared(kv, query, groups, Q, at, size, _stream(stream))
+    _check(rc, "cudalm_paged_decode_shared")
     return out
 
 

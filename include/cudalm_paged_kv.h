@@ -114,6 +114,30 @@ int cudalm_paged_decode(const cudalm_paged_kv* kv, const cudalm_paged_query* q, 
                         int weights_mode, void* workspace, size_t workspace_bytes,
                         hipStream_t stream);
 
+/* The same, without weights, where groups of sequences begin with the same tokens, whose
+ * pages are read once for all of a group's queries. Group g is sequences cu[g] .. cu[g + 1] - 1
+ * (device, [count + 1], ascending within 0 .. batch; sequences of no group share
+ * nothing); its first shared[g] tokens (device, [count]; any number, below zero counts as
+ * zero) are those in the pages of its first sequence, and what the other sequences'
+ * tables hold for them does not count (of a page that is shared in part they hold the
+ * rest). A sequence need not have them all: it sees those of its length. Where every
+ * table names the same pages, results are those of cudalm_paged_decode but for rounding.
+ * (Bounds that do not ascend make their sequences' results unspecified; nothing outside of the
+ * tensors is touched.) Every sequence's row of out is written. */
+typedef struct cudalm_paged_groups {
+  const int32_t* cu;
+  const int32_t* shared;
+  int count;      /* 1 .. batch */
+  int max_shared; /* no group is expected to share more (<= 0: max_pages * page_size); only
+                     speed goes by it */
+} cudalm_paged_groups;
+size_t cudalm_paged_decode_shared_workspace_bytes(const cudalm_paged_kv* kv,
+                                                  const cudalm_paged_query* q,
+                                                  const cudalm_paged_groups* groups, int new_tokens);
+int cudalm_paged_decode_shared(const cudalm_paged_kv* kv, const cudalm_paged_query* q,
+                               const cudalm_paged_groups* groups, int new_tokens, void* workspace,
+                               size_t workspace_bytes, hipStream_t stream);
+
 /* Attention of a chunk: rows cu_new[b] .. cu_new[b + 1] - 1 (device,
  * [batch + 1], ascending from 0 to `tokens`) of q and out are the last tokens
  * of sequence b; their keys and values are in the cache. Rows that belong to no
