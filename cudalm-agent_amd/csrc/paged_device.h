@@ -54,9 +54,6 @@ __device__ __forceinline__ u32x4_t load16(const uint16_t* p) {
 }
 __device__ __forceinline__ void store16(uint16_t* p, u32x4_t v) { *reinterpret_cast<u32x4_t*>(p) = v; }
 
-constexpr int kTile = 32;  // tokens per step of an attention kernel
-constexpr int kTileShift = 5;
-
 // Running maxima start here and not at -inf, so that differences of maxima
 // are never inf - inf; no finite score is below it.
 constexpr float kLowest = -3.402823466e38f;

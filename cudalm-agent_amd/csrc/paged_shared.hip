@@ -2,156 +2,990 @@
 // begin with the same tokens.
 //
 // A group's queries, those of all its sequences, are the rows of one product over its
-// shared tokens (prefill's tiles, positions row by row), so a shared key or value is
-// fetched once for 128 of them. Every sequence's own tokens are decode's. Both leave
+// shared tokens, so a shared key or value is fetched once for 128 of them; every
+// sequence's own tokens are multiplied with its own queries. Both kinds of work leave
 // sums under a running maximum in parts, which a last kernel joins:
 //
 //   out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s     over the parts of both kinds
+//
+// They share one launch. The products are those of prefill and decode: which token a row
+// of the first one stands for is free, so that a lane's scores are its operand of the
+// second one.
 
-#include "paged_decode_body.h"
-#include "paged_prefill_body.h"
+#include <cmath>
+
+#include "paged_device.h"
 
 namespace cudalm_hip {
 namespace {
 
+constexpr int kTile = 32;  // tokens per step
+constexpr int kTileShift = 5;
+constexpr int kWaves = 4;  // of a workgroup
+constexpr int kRows = 32 * kWaves;
+constexpr int kMaxRows = 1024;  // new tokens x query heads of a key-value head
+
+// Workgroups of a CU, and the tiles of keys or values that one has room for.
+template <int D>
+constexpr int kPerCu = D == 256 ? 2 : D == 128 ? 3 : 4;
+template <int D>
+constexpr int kRing = D == 256 ? 5 : D == 128 ? 6 : 8;
+template <int D>
+constexpr size_t kLdsBytes = static_cast<size_t>(kRing<D>) * kTile * D * 2;
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Group g is sequences cu[g] .. cu[g + 1] - 1; its first tokens, shared[g] of them, are
+// those in the pages of sequence cu[g].
+struct SharedGroups {
+  const int32_t* cu;
+  const int32_t* shared;
+  int count;
+
+  // Where group g's sequences begin and end; false where they are none or not there.
+  __device__ __forceinline__ bool sequences(int g, int batch, int* begin, int* end) const {
+    *begin = load_uniform(cu + g);
+    *end = load_uniform(cu + g + 1);
+    return *begin >= 0 && *end > *begin && *end <= batch;
+  }
+  __device__ __forceinline__ int tokens(const PagedView& kv, int g) const {
+    const int n = load_uniform(shared + g), cap = kv.max_pages << kv.page_shift;
+    return n < 0 ? 0 : n < cap ? n : cap;
+  }
+};
+
+// The tiles of the tokens lo .. hi - 1 that some query of positions first .. last sees:
+// those of the sinks, then those from the earliest window's first token on.
+struct PagedRange {
+  int base, sink_tiles, from, count;
+
+  __device__ __forceinline__ PagedRange(int lo, int hi, int first, int last, int window, int sinks) {
+    const int mask = kTile - 1, top = last + 1 < hi ? last + 1 : hi;
+    base = lo >> kTileShift;
+    const int end = top > lo ? (top + mask) >> kTileShift : base;
+    sink_tiles = 0;
+    from = base;
+    if (window > 0 && first - window + 1 > 0) {
+      int st = ((sinks < hi ? sinks : hi) + mask) >> kTileShift, w = (first - window + 1) >> kTileShift;
+      st = st < base ? base : st < end ? st : end;
+      w = w < end ? w : end;
+      if (w > st) sink_tiles = st - base, from = w - sink_tiles;
+    }
+    count = end - from;
+  }
+  __device__ __forceinline__ int tile(int i) const { return i < sink_tiles ? i + base : i + from; }
+};
+
+// Into how many parts a prefix of `tiles` tiles is cut: at most `splits`, of `least` tiles
+// or more.
+__device__ __forceinline__ int prefix_parts(int tiles, int splits, int least) {
+  const int per = tiles_per_split(tiles, splits, least);
+  return (tiles + per - 1) / per;
+}
+
+struct SharedArgs {
+  PagedView kv;
+  SharedGroups sharing;
+  const uint16_t* k;
+  const uint16_t* v;
+  const uint16_t* q;
+  uint16_t* out;
+  long long token_stride, head_stride;
+  float scale_log2;
+  int negate;  // scale is negative: queries are negated and it is taken positive
+  int new_tokens, heads, group, rows, window, sinks;
+  // Prefixes: rows of all groups by kRows, a group's beginning a new unit; parts by blocks
+  // of 32 rows, [splits][units * kWaves][kv_heads], in the order of the registers.
+  f32x4_t* prefix_o;   // .. [D / 8][64 lanes]
+  float2* prefix_ml;   // .. [32]
+  int units, splits, least;
+  // Own tokens: (sequence, head, 16 RT rows) are segments, their tiles in a row are cut into
+  // equal ranges. Part 2 w + x is range w's; whole segments follow, one each.
+  float* own_o;        // [parts][part_rows][D]
+  float2* own_ml;      // [parts][part_rows]
+  int4* places;        // per segment: first part, how many, parts of its prefix, row in prefixes
+  int zrows, part_rows, ranges, own_least;
+};
+
+// --- prefixes ---------------------------------------------------------------------
+
+// N times 16 bytes per lane from base (wave-uniform) + offset to LDS: lane i's of load x
+// land at dst + 4096 x + 16 i. The compiler's builtin for it makes every later LDS read
+// wait for all such loads, those of later tiles among them; here loads_landed() does the
+// waiting.
+template <int N>
+__device__ __forceinline__ void load_lds16(const uint16_t* const* base, const uint32_t* offset, uint32_t dst) {
+  uint32_t saved;  // m0 holds the LDS address for the instruction
+  if constexpr (N == 1) {
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "s"(dst), "v"(offset[0]), "s"(base[0])
+        : "memory");
+  } else {
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\t"
+        "s_mov_b32 m0, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %5, %6\n\ts_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "s"(dst), "v"(offset[0]), "s"(base[0]), "s"(dst + 4096), "v"(offset[1]), "s"(base[1])
+        : "memory");
+    if constexpr (N > 2) load_lds16<N - 2>(base + 2, offset + 2, dst + 8192);
+  }
+}
+
+// This wave's loads have landed but for the last N; a barrier after it speaks for all waves.
+template <int N>
+__device__ __forceinline__ void loads_landed() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// All waves have read what they read from LDS, and come here.
+__device__ __forceinline__ void barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+__device__ __forceinline__ int swap_bits_2_3(int r) {
+  return (r & ~12) | ((r & 4) << 1) | ((r & 8) >> 1);
+}
+
+// Key row r has chunk c at place c ^ chunk_exchange(r): 16 rows of 64 channels lie in
+// eight lines of 64 banks, two to a line, wider ones in one line or more each.
+template <int D>
+__device__ __forceinline__ int chunk_exchange(int r) {
+  return D == 64 ? (r >> 1) & 7 : r & 15;
+}
+
+// kRows rows of a group (a wave has 32 of them as the columns of 32x32x16 products) against
+// a part of its shared tokens:
+//
+//   S^T = K Q^T     (A = 32 tokens x 16 channels, B = 16 channels x 32 rows)
+//   O^T += V^T P^T  (A = 32 channels x 16 tokens, B = 16 tokens x 32 rows)
+//
+// Tiles of keys and of values take turns in a ring of kRing places in LDS, which they
+// reach from the pages without passing registers: unit 2 i is the keys of tile i, unit 2 i +
+// 1 its values. A place is loaded again as soon as all waves have read it, so that kRing - 1 units
+// are on their way or waiting at any time.
+// Row r of a tile of 32 keys in LDS is token r with bits 2 and 3 exchanged: then the
+// eight scores that a lane holds of a row after the first product are those of eight
+// consecutive tokens, which is its operand of the second.
 template <typename T, int D>
-__global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : D == 128 ? 3 : 4) void paged_prefix_kernel(const PrefixArgs a) {
-  extern __shared__ uint16_t lds[];
-  paged_prefill_body<T, D>(a, lds, blockIdx.x);
+__device__ __forceinline__ void prefix_body(const SharedArgs& a, uint16_t* lds, unsigned block) {
+  constexpr int KT = kTile, KK = D / 16, DT = D / 32;
+  constexpr int C = D / 8;              // 16-byte chunks of a key row
+  constexpr int kUnit = KT * D;         // elements of a unit
+  constexpr int kLoads = D / 64;        // 1 KB loads of a unit per wave
+  constexpr int R = kRing<D>;
+  const int wave = wave_id(), lane = threadIdx.x & 63;
+  const int n = lane & 31, half = lane >> 5;
+
+  // The row tiles of the same keys and values stand 8 workgroups apart, in one XCD, one
+  // after the other.
+  const int hs = static_cast<int>(block) / 8 / a.units * 8 + static_cast<int>(block) % 8;
+  const int unit = static_cast<int>(block) / 8 % a.units;
+  if (hs >= a.kv.kv_heads * a.splits) return;
+  const int h = hs % a.kv.kv_heads, split = hs / a.kv.kv_heads;
+  const int g = sequence_of(a.sharing.cu, a.sharing.count, unit, a.rows, kRows, 1);
+  int b, b_end;
+  if (g < 0 || !a.sharing.sequences(g, a.kv.batch, &b, &b_end)) return;
+  const int row0 = (unit - (b * a.rows / kRows + g)) * kRows, rows = (b_end - b) * a.rows;
+  if (row0 < 0 || row0 >= rows) return;  // (below 0 where cu does not ascend)
+  const int length = a.sharing.tokens(a.kv, g);
+  const int parts = prefix_parts((length + KT - 1) >> kTileShift, a.splits, a.least);
+  if (split >= parts) return;
+
+  // this lane's row (one past the last stands for it, and sees nothing), and the positions
+  // of the wave's and the workgroup's first and last
+  const int wave_row = row0 + 32 * wave, row = wave_row + n;
+  const bool real = row < rows;
+  const int token = (real ? row : rows - 1) / a.group;
+  const int seq = b + token / a.new_tokens;
+  int pos = a.kv.length(seq) - a.new_tokens + token % a.new_tokens;
+  u32x4_t qf[KK];
+  {
+    const uint16_t* qp = a.q + (static_cast<long long>(b) * a.new_tokens + token) * a.token_stride +
+                         (static_cast<long long>(h) * a.group + (real ? row - token * a.group : 0)) * a.head_stride +
+                         8 * half;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      qf[kk] = load16(qp + 16 * kk);
+      if (a.negate) qf[kk] ^= 0x80008000u;
+    }
+  }
+  int wave_first = pos, wave_last = pos;
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1) {
+    wave_first = min(wave_first, __shfl_xor(wave_first, x));
+    wave_last = max(wave_last, __shfl_xor(wave_last, x));
+  }
+  wave_first = uniform(wave_first);
+  wave_last = uniform(wave_last);
+  int wg_first = wave_first, wg_last = wave_last;
+  {
+    int* seen = reinterpret_cast<int*>(lds);
+    if (lane == 0) seen[2 * wave] = wave_first, seen[2 * wave + 1] = wave_last;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) wg_first = min(wg_first, seen[2 * w]), wg_last = max(wg_last, seen[2 * w + 1]);
+    wg_first = uniform(wg_first);
+    wg_last = uniform(wg_last);
+    __syncthreads();
+  }
+  if (!real) pos = -1;
+  if (wave_row >= rows) wave_last = -1;  // nothing to multiply
+  const PagedRange tiles(0, length, wg_first, wg_last, a.window, a.sinks);
+  const int per = tiles_per_split(tiles.count, parts, 1);
+  const int begin = split * per, end = begin + per < tiles.count ? begin + per : tiles.count;
+
+  f32x16_t o[DT];
+  float m = kLowest, l = 0;
+
+  const int P = 1 << a.kv.page_shift;
+  const size_t page_elems = static_cast<size_t>(P) * D * a.kv.kv_heads;
+  const size_t head_elems = static_cast<size_t>(P) * D * h;
+  // A wave loads 1 KB pieces wave, wave + 4, .. of a unit. Key row r of piece 4 x + wave is r0
+  // + x kStep: its token is that of r0 plus a number that all lanes share, and the exchange of its
+  // chunks is the same for every x (but for chunk bit 3 where D = 256). So one or two offsets
+  // per lane serve all loads.
+  constexpr int kStep = 2048 / D;
+  const int r0 = wave * (512 / D) + lane / C;
+  const uint32_t k_lane = 2 * (swap_bits_2_3(r0) % 16 * D + 8 * ((lane % C) ^ chunk_exchange<D>(r0)));
+  const int v_piece = wave * 64;  // in channels of the tile's groups of eight tokens
+  const uint32_t v_lane = 16 * (v_piece % D + lane);
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)) + wave * 1024;
+
+  // every row from position `from` to `to` sees all of the tile at t
+  auto seen_whole = [&](int t, int from, int to) {
+    return t + KT <= length && t + KT - 1 <= from && (a.window <= 0 || t > to - a.window || t + KT - 1 < a.sinks);
+  };
+  const bool wg_full = row0 + kRows <= rows, wave_full = wave_row + 32 <= rows;
+  // Places, pages and visibility of 32 tiles: lanes 2 i and 2 i + 1 hold the halves of tile
+  // i, masks a bit each, and those of the 32 before, since loads run ahead of products.
+  uint64_t half_at = 0;  // of the half's first key, and value, in its cache
+  struct Masks {
+    uint64_t absent, whole, wg_whole;
+  } masks = {0, 0, 0}, old_masks = masks;
+  int ahead = begin;  // the first tile of the 32
+  auto look_ahead = [&](int i) {
+    old_masks = masks;
+    ahead = i;
+    const int first_token = tiles.tile(i + lane / 2) << kTileShift, t = first_token + 16 * (lane & 1);
+    int page = -1;
+    if (i + lane / 2 < end) page = a.kv.page(b, t >> a.kv.page_shift);
+    // absent pages are hidden below; any page will do
+    half_at = max(page, 0) * page_elems + head_elems + static_cast<uint64_t>(t & (P - 1)) * D;
+    masks.absent = __ballot(page < 0);
+    masks.whole = __ballot(wave_full && seen_whole(first_token, wave_first, wave_last));
+    masks.wg_whole = __ballot(wg_full && seen_whole(first_token, wg_first, wg_last));
+  };
+  auto half_place = [&](int x) { return readlane64(half_at, x); };
+  const int units = 2 * (end - begin);
+  int into = 0;  // the place of the next unit
+  auto issue = [&](int u) {
+    const int x = u & 63;
+    if (x == 0 && u > 0) look_ahead(begin + u / 2);
+    const uint64_t at0 = half_place(x & ~1), at1 = half_place(x | 1);
+    const uint16_t* base[kLoads];
+    uint32_t offset[kLoads];
+    if (x & 1) {
+#pragma unroll
+      for (int y = 0; y < kLoads; ++y) {
+        const int group = y * (2048 / (8 * D)) + v_piece / D;
+        base[y] = a.v + (group & 2 ? at1 : at0) + (group & 1) * 8 * D;
+        offset[y] = v_lane;
+      }
+    } else {
+#pragma unroll
+      for (int y = 0; y < kLoads; ++y) {
+        // rows of the piece: tokens of 16-token half r / 16, bit 3 of r is bit 2 of the token
+        const int r = y * kStep + wave * (512 / D);
+        const bool odd = D == 256 && (y & 1);
+        base[y] = a.k + (r & 16 ? at1 : at0) + (odd ? 4 * D : 0);
+        offset[y] = odd ? k_lane ^ 128 : k_lane;
+      }
+    }
+    load_lds16<kLoads>(base, offset, lds0 + into * (2 * kUnit));
+    into = into + 1 == R ? 0 : into + 1;
+  };
+  // Unit u is there for all waves, and all have read unit u - 1.
+  auto arrive = [&](int u) {
+    const int after = units - 1 - u;  // those issued by now but for the last R - 2
+    if (after >= R - 2)
+      loads_landed<(R - 2) * kLoads>();
+    else if (after >= 2)
+      loads_landed<2 * kLoads>();
+    else if (after == 1)
+      loads_landed<kLoads>();
+    else
+      loads_landed<0>();
+    barrier();
+  };
+  // Zero weights times Inf or NaN are NaN. So in a tile that some row sees only
+  // part of, values past the end or of absent pages (which may be anything) are
+  // cleared, and Inf and NaN among the others taken out; the rows that do see
+  // those get them at the end.
+  uint32_t special = 0;
+  auto clean = [&](u32x4_t* vt, int t0, uint32_t absent) {
+#pragma unroll 2
+    for (int u = threadIdx.x; u < KT / 8 * D; u += 64 * kWaves) {
+      const int group = u / D, t = t0 + 8 * group;
+      const bool gone = (absent >> (group >> 1)) & 1;
+      u32x4_t w = vt[u];
+      if (gone || t + 8 > length) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (gone || t + 2 * e >= length) w[e] &= 0xFFFF0000u;
+          if (gone || t + 2 * e + 1 >= length) w[e] &= 0x0000FFFFu;
+        }
+        vt[u] = w;
+      }
+      const uint32_t bad = special_bits<T>(w);
+      special |= bad;
+      if (bad) vt[u] = finite_part<T>(w);
+    }
+  };
+
+  constexpr int kAhead = D == 256 ? 3 : 4;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[dt][e] = 0;
+  // (Its wait for the table is one for the queries too: the compiler, which does not see the
+  // loads to LDS, would else have the products of every tile wait for all of those.)
+  look_ahead(begin);
+  for (int u = 0; u < R - 1 && u < units; ++u) issue(u);
+  int from = 0;  // the place of the next unit to be read
+#pragma unroll 1
+  for (int u = 0; u < units; u += 2) {
+    const int tile = begin + u / 2, t0 = tiles.tile(tile) << kTileShift;
+    arrive(u);
+    if (u - 1 + R < units) issue(u - 1 + R);
+    const Masks& now = tile < ahead ? old_masks : masks;
+    const int bit = u & 63;
+    const uint32_t absent = static_cast<uint32_t>(now.absent >> bit) & 3;
+    const bool whole = !absent && ((now.whole >> bit) & 1), wg_whole = !absent && ((now.wg_whole >> bit) & 1);
+    const bool work = t0 <= wave_last;  // not above the wave's rows
+    f32x16_t s;
+    u32x4_t pf[2];
+    if (work) {
+      const uint16_t* kt = lds + from * kUnit;
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = 0;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+        s = T::mfma32(load16(kt + n * D + 8 * ((2 * kk + half) ^ chunk_exchange<D>(n))), qf[kk], s);
+      __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+      for (int kk = 0; kk < KK - kAhead; ++kk) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+      __builtin_amdgcn_s_setprio(0);
+      // s[e] is the score of token t0 + 16 (e / 8) + 8 half + e % 8
+      if (!whole) {
+        // token t is seen from p if 0 <= p - t < window, or if t is a sink up to p
+        const uint32_t reach = a.window > 0 ? a.window : 0x7FFFFFFF;
+        const int back = pos - t0 - 8 * half, room = length - t0 - 8 * half;
+        const int sunk = t0 < a.sinks ? min(a.sinks - t0 - 8 * half, back + 1) : -1;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int i = 16 * (e >> 3) + (e & 7);
+          const bool sees = (static_cast<uint32_t>(back - i) < reach || i < sunk) && i < room &&
+                            !((absent >> (e >> 3)) & 1);
+          s[e] = sees ? s[e] : -__builtin_inff();
+        }
+      }
+      float top = s[0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
+      top = max_across_32(top) * a.scale_log2;
+      // The maximum may lag by up to 2^8: weights stay below 256, which neither fp32 sums nor
+      // 16-bit weights mind, and most tiles rescale nothing.
+      if (__any(top > m + 8.0f)) {
+        const float next = fmaxf(m, top), r = exp2_fast(m - next);
+        l *= r;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[dt][e] *= r;
+        m = next;
+      }
+      float sum = 0;
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        const float p0 = exp2_fast(__builtin_fmaf(s[e], a.scale_log2, -m));
+        const float p1 = exp2_fast(__builtin_fmaf(s[e + 1], a.scale_log2, -m));
+        sum += p0 + p1;
+        // rounded to the values' type, as the matrix unit takes them; l sums the unrounded ones
+        pf[e / 8][e % 8 / 2] = T::pack(p0, p1);
+      }
+      l += sum;
+    }
+    from = from + 1 == R ? 0 : from + 1;
+    arrive(u + 1);
+    if (u + R < units) issue(u + R);
+    uint16_t* vt = lds + from * kUnit;
+    if (!wg_whole) {
+      clean(reinterpret_cast<u32x4_t*>(vt), t0, absent);
+      barrier();
+    }
+    if (work) {
+      __builtin_amdgcn_s_setprio(1);
+      constexpr int kFirst = 1 + D / 128;
+      const u32x4_t* vp = reinterpret_cast<const u32x4_t*>(vt) + half * D + n;
+#pragma unroll
+      for (int x = 0; x < 2 * DT; ++x)
+        o[x % DT] = T::mfma32(vp[(x / DT) * 2 * D + 32 * (x % DT)], pf[x / DT], o[x % DT]);
+      __builtin_amdgcn_sched_group_barrier(0x100, kFirst, 0);
+#pragma unroll
+      for (int x = 0; x < 2 * DT - kFirst; ++x) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, kFirst, 0);
+      __builtin_amdgcn_s_setprio(0);
+    }
+    from = from + 1 == R ? 0 : from + 1;
+  }
+  // Inf or NaN for the sums of channels 32 dt .. whose rows see such a value: how many
+  // tokens hold +Inf or NaN, -Inf or NaN. In tiles that were not cleaned a weight that
+  // underflows has made NaN of Inf, so what the sums hold there does not count.
+  auto add_special = [&](f32x16_t& r, int dt) {
+    f32x16_t up, down;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) up[e] = down[e] = 0;
+#pragma unroll 1
+    for (int i = begin; i < end; ++i) {
+      const int place = tiles.tile(i) << kTileShift;
+#pragma unroll 1
+      for (int y = 0; y < KT / 16; ++y) {
+        const int t = place + 16 * y + 8 * half;
+        const int page = a.kv.page(b, t >> a.kv.page_shift);
+        uint32_t seen = 0;
+        u32x4_t w = {0, 0, 0, 0};
+        if (page >= 0) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            seen |= t + e < length && paged_sees(t + e, pos, a.window, a.sinks) ? 1u << e : 0u;
+          w = load16(a.v + page * page_elems + head_elems + static_cast<size_t>(t & (P - 1)) * D + 8 * (32 * dt + n));
+        }
+        const u32x4_t ones = seen_operand<T>(seen);
+        up = T::mfma32(special_part<T>(w, ~0u), ones, up);
+        down = T::mfma32(special_part<T>(w, 0), ones, down);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (up[e] > 0 || down[e] > 0)
+        r[e] = (up[e] > 0 ? __builtin_inff() : 0.0f) + (down[e] > 0 ? -__builtin_inff() : 0.0f);
+  };
+  f32x16_t most = o[0];  // of the sums' sizes, NaN if one of them is
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) most[e] = __builtin_elementwise_maximum(fabsf(most[e]), fabsf(o[dt][e]));
+#pragma unroll
+  for (int x = 8; x > 0; x >>= 1)
+#pragma unroll
+    for (int e = 0; e < x; ++e) most[e] = __builtin_elementwise_maximum(most[e], most[e + x]);
+  barrier();  // the ring has been read: its first words hold the waves' votes
+  uint32_t* votes = reinterpret_cast<uint32_t*>(lds);
+  votes[wave] = __any(special != 0 || !(most[0] < __builtin_inff()));
+  __syncthreads();
+  special = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) special |= votes[w];
+  special = uniform(special);
+  if (wave_row >= rows) return;
+  l += __shfl_xor(l, 32);
+  const size_t at = (static_cast<size_t>(split) * (a.units * kWaves) + unit * kWaves + wave) * a.kv.kv_heads + h;
+  // -inf tells the join that there is nothing to read: no weight here, nor Inf or NaN
+  if (half == 0) a.prefix_ml[at * 32 + n] = float2{l == 0.0f && !special ? -__builtin_inff() : m, l};
+  if (begin >= end) return;
+  f32x4_t* p = a.prefix_o + at * (D / 8 * 64) + lane;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) {
+    f32x16_t r = o[dt];
+    if (special) add_special(r, dt);
+#pragma unroll
+    for (int y = 0; y < 4; ++y)
+      p[(4 * dt + y) * 64] = f32x4_t{r[4 * y], r[4 * y + 1], r[4 * y + 2], r[4 * y + 3]};
+  }
+}
+
+// --- own tokens ---------------------------------------------------------------------
+
+// 16 bytes; `once`: nothing else of the call reads them, so the caches need not keep them.
+template <bool once>
+__device__ __forceinline__ u32x4_t load_once(const uint16_t* p) {
+  const u32x4_t* q = reinterpret_cast<const u32x4_t*>(p);
+  return once ? __builtin_nontemporal_load(q) : *q;
+}
+
+// Sequences' own tokens in the row of all tiles (fewer than 2^31), 64 sequences at a time, a
+// lane each.
+struct Segments {
+  int block, base;   // first sequence of the 64, tiles before it
+  int length, from;  // this lane's sequence: tokens, and how many of them are its group's
+  int row;           // its first row among those of prefixes
+  int count, end;    // tiles of a segment, end of its last one
+
+  // All lanes look at all groups: their bounds are wave-uniform loads that do not wait
+  // for each other, where a search would be a chain of them.
+  __device__ __forceinline__ void load(const SharedArgs& a, int lane) {
+    const int b = block + lane, per_seq = a.kv.kv_heads * a.zrows;
+    length = b < a.kv.batch ? a.kv.length(b) : 0;
+    from = row = 0;
+#pragma unroll 2
+    for (int g = 0; g < a.sharing.count; ++g) {
+      int first, last;
+      const bool real = a.sharing.sequences(g, a.kv.batch, &first, &last);
+      const int tokens = a.sharing.tokens(a.kv, g);
+      if (real && b >= first && b < last) {
+        from = tokens;
+        row = (first * a.rows / kRows + g) * kRows + (b - first) * a.rows;
+      }
+    }
+    const PagedRange tiles(from, length, length - a.new_tokens, length - 1, a.window, a.sinks);
+    count = b < a.kv.batch ? max(tiles.count, 1) : 0;  // (a place for the row's zeros)
+    end = count * per_seq;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) {
+      const int o = __shfl_up(end, x);
+      if (lane >= x) end += o;
+    }
+  }
+  // The tiles of all sequences; leaves the first 64 loaded.
+  __device__ __forceinline__ int total(const SharedArgs& a, int lane) {
+    int all = 0;
+    base = 0;
+    for (block = (a.kv.batch - 1) / 64 * 64;; block -= 64) {
+      load(a, lane);
+      all += __builtin_amdgcn_readlane(end, 63);
+      if (block == 0) return all;
+    }
+  }
+  // The lane whose sequence has tile g (not before the block, and before the last).
+  __device__ __forceinline__ int find(const SharedArgs& a, int lane, int g) {
+    for (;;) {
+      const uint64_t after = __ballot(base + end > g);
+      if (after) return __builtin_ctzll(after);
+      base += __builtin_amdgcn_readlane(end, 63);
+      block += 64;
+      load(a, lane);
+    }
+  }
+};
+
+// The rows of a (sequence, head), its new tokens times the group's query heads, are the 16
+// columns of 16x16x32 products; keys and values come straight from the pages into
+// registers. RT tiles of 16 rows have a wave each, which walk over the same tokens; beside them
+// 4 / RT ranges. No wave waits for another.
+template <typename T, int D, int RT>
+__device__ __forceinline__ void own_body(const SharedArgs& a, uint16_t* lds, unsigned block) {
+  constexpr int KK = D / 32, DT = D / 16, SL = kWaves / RT;
+  const int wave = wave_id(), lane = threadIdx.x & 63;
+  const int n = lane & 15, quarter = lane >> 4;
+  const int rt = wave % RT, range = block * SL + wave / RT;
+  // The queries in the order of the operands (registers are for what is on its way from
+  // memory).
+  u32x4_t* q_lds = reinterpret_cast<u32x4_t*>(lds) + wave * (KK * 64) + lane;
+
+  const int P = 1 << a.kv.page_shift;
+  const size_t page_elems = (static_cast<size_t>(P) * D) * a.kv.kv_heads;
+  const int ktok = 8 * (n >> 2) + (n & 3);  // token of K row n in half 0
+
+  Segments segments;
+  const int total = segments.total(a, lane);
+  int per = uniform((total + a.ranges - 1) / a.ranges);
+  per = per > a.own_least ? per : a.own_least;
+  if (static_cast<long long>(range) * per >= total) return;
+  int g = range * per;
+  const int stop = g + per < total ? g + per : total, per_seq = a.kv.kv_heads * a.zrows;
+#pragma unroll 1
+  while (g < stop) {
+    const int x0 = segments.find(a, lane, g), b = segments.block + x0;
+    const int all = __builtin_amdgcn_readlane(segments.count, x0);
+    const int start = segments.base + __builtin_amdgcn_readlane(segments.end, x0) - all * per_seq;
+    const int hz = uniform((g - start) / all), h = hz / a.zrows, zr = hz % a.zrows;
+    const int begin = g - start - hz * all, end = stop - g < all - begin ? begin + stop - g : all;
+    const int length = __builtin_amdgcn_readlane(segments.length, x0), from = __builtin_amdgcn_readlane(segments.from, x0);
+    const PagedRange tiles(from, length, length - a.new_tokens, length - 1, a.window, a.sinks);
+    const int segment = b * per_seq + hz;
+    const int slot = end - begin == all ? 2 * a.ranges + segment : 2 * range + (begin == 0);
+    if (begin == 0 && rt == 0 && lane == 0)
+      a.places[segment] = int4{slot, (g + all - 1) / per - range + 1,
+                               prefix_parts((from + kTile - 1) >> kTileShift, a.splits, a.least),
+                               __builtin_amdgcn_readlane(segments.row, x0)};
+    // this lane's row
+    const int row = (zr * RT + rt) * 16 + n;
+    const bool real = row < a.rows;
+    const int j = real ? row / a.group : 0;
+    const int pos = real ? length - a.new_tokens + j : -1;
+    const size_t head_elems = static_cast<size_t>(P) * D * h;
+    auto row_sees = [&](int t) { return t >= from && paged_sees(t, pos, a.window, a.sinks); };
+    // Pages of the next 32 tiles: lanes 2 i and 2 i + 1 hold the halves of tile i.
+    int tile = 0, page = -1;  // first token
+    uint64_t half_at = 0;     // of the half's first key, and value, in its cache
+    auto look_up = [&](int c) {
+      const int mine = c + (lane >> 1);
+      tile = tiles.tile(mine) << kTileShift;
+      page = -1;
+      if (mine < end) page = a.kv.page(b, (tile + 16 * (lane & 1)) >> a.kv.page_shift);
+    };
+    look_up(begin);
+    {
+      const uint16_t* qp = a.q + (static_cast<long long>(b) * a.new_tokens + j) * a.token_stride +
+                           (static_cast<long long>(h) * a.group + (real ? row - j * a.group : 0)) * a.head_stride +
+                           8 * quarter;
+      u32x4_t qf[KK];
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) qf[kk] = load16(qp + 32 * kk);
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        if (!real) qf[kk] = u32x4_t{0, 0, 0, 0};
+        if (a.negate) qf[kk] ^= 0x80008000u;
+        q_lds[kk * 64] = qf[kk];
+      }
+    }
+    f32x4_t o[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4_t{0, 0, 0, 0};
+    float m = kLowest, l = 0;
+    uint32_t bad = 0;
+    u32x4_t kf[2][KK], vf[DT];
+    auto place = [&](int x) { return readlane64(half_at, x); };
+    auto load_k = [&](int x) {
+      const uint64_t at0 = place(x), at1 = place(x + 1), at = n < 8 ? at0 : at1;
+      const uint16_t* kp = a.k + at + static_cast<uint32_t>((ktok & 15) * D + 8 * quarter);
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+        for (int f = 0; f < 2; ++f) kf[f][kk] = load_once<RT == 1>(kp + 4 * f * D + 32 * kk);
+    };
+    auto load_v = [&](int x) {
+      const uint64_t at0 = place(x), at1 = place(x + 1), at = quarter < 2 ? at0 : at1;
+      const uint16_t* vp = a.v + at + static_cast<uint32_t>(8 * (quarter & 1) * D + 8 * n);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) vf[dt] = load_once<RT == 1>(vp + 128 * dt);
+    };
+#pragma unroll 1
+    for (int c = begin; c < end; c += 32) {
+      if (c > begin) look_up(c);
+      half_at = static_cast<uint64_t>(page < 0 ? 0 : page) * page_elems + head_elems +
+                static_cast<uint64_t>((tile + 16 * (lane & 1)) & (P - 1)) * D;
+      const uint64_t here = __ballot(page >= 0);
+      const int last = end - c < 32 ? end - c : 32;
+      // The next tile's keys load while this one's weights are made, its values while the
+      // scores are.
+      load_k(0);
+      wave_lds_sync();
+#pragma unroll 1
+      for (int x = 0; x < last; ++x) {
+        load_v(2 * x);
+        const int t0 = __builtin_amdgcn_readlane(tile, 2 * x);
+        float t[8];  // this lane's scores: its row, tokens 8 quarter .. 8 quarter + 7
+        {
+          f32x4_t s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
+          asm volatile("" ::: "memory");  // the queries stay in LDS between tiles
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk) {
+            const u32x4_t qf = q_lds[kk * 64];
+            s0 = T::mfma(kf[0][kk], qf, s0);
+            s1 = T::mfma(kf[1][kk], qf, s1);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            t[e] = s0[e] * a.scale_log2;
+            t[4 + e] = s1[e] * a.scale_log2;
+          }
+        }
+        if (x + 1 < last) load_k(2 * x + 2);
+        const bool has = (here >> (2 * x + (quarter >> 1))) & 1;
+        uint32_t sees = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const bool one = has && row_sees(t0 + 8 * quarter + e);
+          sees |= one ? 1u << e : 0u;
+          t[e] = one ? t[e] : -__builtin_inff();
+        }
+        float top = t[0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) top = fmaxf(top, t[e]);
+        top = max_across_32(max_across_16(top));
+        if (__any(top > m + 8.0f)) {  // (a lagging maximum, as above)
+          const float next = fmaxf(m, top), r = exp2_fast(m - next);
+          l *= r;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) o[dt] *= r;
+          m = next;
+        }
+        u32x4_t pf;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float p0 = exp2_fast(t[e] - m), p1 = exp2_fast(t[e + 1] - m);
+          l += p0 + p1;
+          pf[e / 2] = T::pack(p0, p1);
+        }
+        // Zero weights times Inf or NaN are NaN: values of tokens that no row here
+        // sees, which may be anything, are cleared, and Inf and NaN taken out of the
+        // others; the rows that do see those get them at the end.
+        uint32_t some = sees;
+#pragma unroll
+        for (int y = 1; y < 16; y <<= 1) some |= __shfl_xor(static_cast<int>(some), y);
+        uint32_t keep[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          keep[w] = ((some >> (2 * w)) & 1 ? 0xFFFFu : 0u) | ((some >> (2 * w + 1)) & 1 ? 0xFFFF0000u : 0u);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) vf[dt][w] &= keep[w];
+          bad |= special_bits<T>(vf[dt]);
+          o[dt] = T::mfma(finite_part<T>(vf[dt]), pf, o[dt]);
+        }
+      }
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    // Inf and NaN that were taken out, for the rows that see them: how many tokens hold
+    // +Inf or NaN, -Inf or NaN.
+    if (__any(bad != 0)) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        f32x4_t up = {0, 0, 0, 0}, down = {0, 0, 0, 0};
+#pragma unroll 1
+        for (int i = begin; i < end; ++i) {
+          const int t0 = (tiles.tile(i) << kTileShift) + 8 * quarter;
+          const int at = a.kv.page(b, t0 >> a.kv.page_shift);
+          uint32_t sees = 0;
+          u32x4_t v = {0, 0, 0, 0};
+          if (at >= 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sees |= row_sees(t0 + e) ? 1u << e : 0u;
+            v = load16(a.v + at * page_elems + head_elems + static_cast<size_t>(t0 & (P - 1)) * D + 8 * n + 128 * dt);
+          }
+          const u32x4_t ones = seen_operand<T>(sees);
+          up = T::mfma(special_part<T>(v, ~0u), ones, up);
+          down = T::mfma(special_part<T>(v, 0), ones, down);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          o[dt][e] += (up[e] > 0 ? __builtin_inff() : 0.0f) + (down[e] > 0 ? -__builtin_inff() : 0.0f);
+      }
+    }
+    if (real) {
+      const size_t at = static_cast<size_t>(slot) * a.part_rows + rt * 16 + n;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        *reinterpret_cast<f32x4_t*>(a.own_o + at * D + 16 * dt + 4 * quarter) = o[dt];
+      if (quarter == 0) a.own_ml[at] = float2{m, l};
+    }
+    wave_lds_sync();  // the queries have been read
+    g += end - begin;
+  }
 }
 
 template <typename T, int D, int RT>
-__global__ __launch_bounds__(256, 2) void paged_own_kernel(const OwnDecodeArgs a) {
-  __shared__ DecodeLds<D, RT, 4> lds;
-  paged_decode_body<T, D, RT, 4, true>(a, lds, blockIdx.x);
+__global__ __launch_bounds__(64 * kWaves, kPerCu<D>) void paged_shared_kernel(const SharedArgs a, unsigned prefix_blocks) {
+  extern __shared__ uint16_t shared_lds[];
+  if (blockIdx.x < prefix_blocks)
+    prefix_body<T, D>(a, shared_lds, blockIdx.x);
+  else
+    own_body<T, D, RT>(a, shared_lds, blockIdx.x - prefix_blocks);
 }
 
-// A workgroup of four waves per row, a quarter of its parts each: out = the join.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void paged_shared_join_kernel(const OwnDecodeArgs a, const float* prefix_o,
-                                                                const float* prefix_ml, int splits) {
-  constexpr int E = D / 64;
-  __shared__ float sums[4][D], weights[4];
-  const int lane = threadIdx.x & 63, wave = wave_id();
-  const int heads = a.group * a.kv.kv_heads;
-  const size_t rows = static_cast<size_t>(a.kv.batch) * a.new_tokens * heads, row = blockIdx.x;
-  const int token = static_cast<int>(row / heads), head = static_cast<int>(row - static_cast<size_t>(token) * heads);
-  const int b = token / a.new_tokens, h = head / a.group;
-  const int r = (token - b * a.new_tokens) * a.group + head - h * a.group, zr = r / a.part_rows;
-  const Parts own(a, b, h, zr, lane);
-  const int before = uniform(a.sharing.shared_of(a.kv, b)) > 0 ? splits : 0, count = before + own.count;
-  auto ml = [&](int s) {
-    return s < before ? prefix_ml + 2 * (s * rows + row)
-                      : a.part_ml + 2 * (own.at(s - before) * a.part_rows + r - zr * a.part_rows);
-  };
-  float M = kLowest;
-  for (int s = lane; s < count; s += 64) M = fmaxf(M, ml(s)[0]);
+// --- the join -------------------------------------------------------------------------
+
+// 32 rows of a key-value head, PC pieces of eight channels; the waves of a workgroup take
+// every fourth part. A lane has the row n of a prefix's register order and four channels of a
+// piece, so that a part's piece is one load of 1 KB. The maximum runs along, which saves a pass
+// over the parts' maxima.
+template <typename T, int D, int PC>
+__global__ __launch_bounds__(256) void paged_shared_join_kernel(const SharedArgs a, int chunks) {
+  constexpr int kAtOnce = 8 / PC;
+  __shared__ f32x4_t sums[kWaves][PC][64];
+  __shared__ float2 tops[kWaves][32];
+  const int lane = threadIdx.x & 63, wave = wave_id(), n = lane & 31, half = lane >> 5;
+  const int chunk = blockIdx.x % chunks, h = blockIdx.x / chunks % a.kv.kv_heads;
+  const int R = static_cast<int>(blockIdx.x / chunks / a.kv.kv_heads) * 32 + n;
+  const bool real = R < a.kv.batch * a.rows;
+  const int b = (real ? R : 0) / a.rows, r = (real ? R : 0) - b * a.rows, zr = r / a.part_rows;
+  const int4 place = a.places[(b * a.kv.kv_heads + h) * a.zrows + zr];
+  const int before = place.z, count = real ? before + place.y : 0, prow = place.w + r;
+  f32x4_t acc[PC];
 #pragma unroll
-  for (int x = 1; x < 64; x <<= 1) M = fmaxf(M, __shfl_xor(M, x));
-  float acc[E] = {}, l = 0;
-#pragma unroll 4
-  for (int s = wave; s < count; s += 4) {
-    const float* at = ml(s);
-    const float m = at[0];
-    if (m == -__builtin_inff()) continue;  // nothing to read (prefill's parts say so)
-    const float w = exp2_fast(m - M);
-    l += w * at[1];
-    const float* p = (s < before ? prefix_o + (s * rows + row) * D
-                                 : a.part_o + (own.at(s - before) * a.part_rows + r - zr * a.part_rows) * D) + lane * E;
+  for (int x = 0; x < PC; ++x) acc[x] = f32x4_t{0, 0, 0, 0};
+  float m = kLowest, l = 0;
+  for (int s0 = wave; __any(s0 < count); s0 += kWaves * kAtOnce) {
+    float2 ml[kAtOnce];
+    f32x4_t o[kAtOnce][PC];
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] += joined(w, p[e]);
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int s = s0 + kWaves * i;
+      ml[i] = float2{-__builtin_inff(), 0};
+      if (s < before) {
+        const size_t at = (static_cast<size_t>(s) * (a.units * kWaves) + prow / 32) * a.kv.kv_heads + h;
+        ml[i] = a.prefix_ml[at * 32 + prow % 32];
+#pragma unroll
+        for (int x = 0; x < PC; ++x)
+          o[i][x] = a.prefix_o[(at * (D / 8) + chunk * PC + x) * 64 + half * 32 + prow % 32];
+      } else if (s < count) {
+        const int y = s - before;
+        const size_t at = (static_cast<size_t>(place.x) + (y ? 2 * y - 1 : 0)) * a.part_rows + r - zr * a.part_rows;
+        ml[i] = a.own_ml[at];
+#pragma unroll
+        for (int x = 0; x < PC; ++x)
+          o[i][x] = *reinterpret_cast<const f32x4_t*>(a.own_o + at * D + 8 * (chunk * PC + x) + 4 * half);
+      }
+    }
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) top = fmaxf(top, ml[i].x);
+    const float again = exp2_fast(m - top);
+    m = top;
+    l *= again;
+#pragma unroll
+    for (int x = 0; x < PC; ++x)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[x][e] = joined(again, acc[x][e]);
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (ml[i].x == -__builtin_inff()) continue;  // nothing there
+      const float w = exp2_fast(ml[i].x - m);
+      l += w * ml[i].y;
+#pragma unroll
+      for (int x = 0; x < PC; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[x][e] += joined(w, o[i][x][e]);
+    }
   }
 #pragma unroll
-  for (int e = 0; e < E; ++e) sums[wave][lane * E + e] = acc[e];
-  if (lane == 0) weights[wave] = l;
+  for (int x = 0; x < PC; ++x) sums[wave][x][lane] = acc[x];
+  if (half == 0) tops[wave][n] = float2{m, l};
   __syncthreads();
-  if (threadIdx.x >= D / 2) return;
-  l = weights[0] + weights[1] + weights[2] + weights[3];
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  float y[2];
+  if (wave >= PC) return;
+  float M = kLowest;
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int c = 2 * threadIdx.x + e;
-    const float v = sums[0][c] + sums[1][c] + sums[2][c] + sums[3][c];
-    y[e] = l == 0.0f ? 0.0f : v * inv;  // (no weight at all: zeros, whatever the values)
+  for (int w = 0; w < kWaves; ++w) M = fmaxf(M, tops[w][n].x);
+  l = 0;
+  f32x4_t y = {0, 0, 0, 0};
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const float weight = exp2_fast(tops[w][n].x - M);
+    l += weight * tops[w][n].y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] += joined(weight, sums[w][wave][lane][e]);
   }
-  reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + row * D)[threadIdx.x] = T::pack(y[0], y[1]);
+  if (!real) return;
+  const float inv = 1.0f / l;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = l == 0.0f ? 0.0f : y[e] * inv;  // (no weight at all: zeros)
+  const int j = r / a.group;
+  const size_t to = (static_cast<size_t>(b) * a.new_tokens + j) * a.heads + h * a.group + r - j * a.group;
+  *reinterpret_cast<u32x2_t*>(a.out + to * D + 8 * (chunk * PC + wave) + 4 * half) =
+      u32x2_t{T::pack(y[0], y[1]), T::pack(y[2], y[3])};
 }
+
+// --- host -----------------------------------------------------------------------------
 
 // How a call is cut.
 struct SharedPlan {
-  int rows, rt, zrows, part_rows, groups, least, splits;
-  long long units, segments;
-  size_t prefix_o, prefix_ml, own_o, own_ml;
-  size_t bytes() const { return prefix_o + prefix_ml + own_o + own_ml; }
+  int rows, rt, zrows, part_rows, splits, least, own_blocks, own_least;
+  long long units, segments, prefix_blocks;
+  size_t prefix_o, prefix_ml, own_o, own_ml, places;
+  size_t bytes() const { return prefix_o + prefix_ml + own_o + own_ml + places; }
+  int ranges() const { return own_blocks * (kWaves / rt); }
 };
+
+constexpr size_t padded(size_t bytes) { return (bytes + 15) / 16 * 16; }
 
 SharedPlan plan_of(const cudalm_paged_kv* kv, const cudalm_paged_query* q, const cudalm_paged_groups* g,
                    int new_tokens) {
   SharedPlan p;
-  const int group = q->heads / kv->kv_heads;
+  const int group = q->heads / kv->kv_heads, D = kv->head_dim, window = window_of(q);
+  const long long B = kv->batch;
   p.rows = new_tokens * group;
   const int row_tiles = (p.rows + 15) / 16;
   p.rt = row_tiles > 2 ? 4 : row_tiles;
   p.zrows = (row_tiles + p.rt - 1) / p.rt;
   p.part_rows = 16 * p.rt < p.rows ? 16 * p.rt : p.rows;
-  p.least = 4 / p.rt;
-  p.groups = (kv->head_dim == 64 ? 4 : 2) * cu_count();
-  p.segments = static_cast<long long>(kv->batch) * kv->kv_heads * p.zrows;
-  const size_t slots = (2 * static_cast<size_t>(p.groups) + p.segments) * p.part_rows;
-  p.own_o = slots * kv->head_dim * 4;
-  p.own_ml = (slots * 8 + 15) / 16 * 16;
-  // the prefixes: enough workgroups to fill the chip, of at least four tiles
-  const long long total = static_cast<long long>(kv->batch) * new_tokens * q->heads;
-  p.units = static_cast<long long>(kv->batch) * p.rows / kRows + g->count;
-  const int len = expected_len(kv, g->max_shared);
-  long long tiles = (len + kTile - 1) / kTile;
-  const long long groups = (static_cast<long long>(kv->batch) * p.rows + kRows - 1) / kRows * kv->kv_heads;
-  long long want = 2LL * cu_count() / groups;
-  want = want < tiles / 4 ? want : tiles / 4;
-  want = want < 32 ? want : 32;
-  p.splits = static_cast<int>(want < 1 ? 1 : want);
-  p.prefix_o = static_cast<size_t>(p.splits) * total * kv->head_dim * 4;
-  p.prefix_ml = (static_cast<size_t>(p.splits) * total * 8 + 15) / 16 * 16;
+  p.segments = B * kv->kv_heads * p.zrows;
+  const int at_once = (D == 256 ? kPerCu<256> : D == 128 ? kPerCu<128> : kPerCu<64>) * cu_count();
+  // What is expected: tiles of the longest prefix, and of all sequences' own tokens.
+  const int len = expected_len(kv, q->max_len), prefix = expected_len(kv, g->max_shared);
+  const long long near = window > 0 ? (window + sinks_of(q)) / kTile + 3LL : 1LL << 30;
+  long long tiles = (prefix + kTile - 1) / kTile;
+  tiles = tiles < near ? tiles : near;
+  long long own = ((len > prefix ? len - prefix : len) + kTile - 1) / kTile + 1;
+  own = p.segments * (own < near ? own : near);
+  // Prefixes: a workgroup per `least` tiles. Fewer tiles end sooner but leave more parts, whose
+  // bytes are written and read: t tiles cost t steps and all rows' parts 2 rows 4 D (tiles / t) at
+  // 5 TB/s, least where the two are equal; and half of what runs at once is left for the own
+  // tokens.
+  const long long units = (B * p.rows + kRows - 1) / kRows * kv->kv_heads;
+  const double bytes = 8.0 * B * p.rows * kv->kv_heads * D * tiles / 5e6, step = D == 256 ? 1.6 : D == 128 ? 1.0 : 0.7;
+  long long least = static_cast<long long>(std::sqrt(bytes / step) + 0.5);
+  const long long round = (units * tiles + at_once / 2 - 1) / (at_once / 2);
+  least = least < round ? round : least;
+  least = least < 1 ? 1 : least > tiles ? tiles : least;
+  p.least = static_cast<int>(least);
+  p.splits = static_cast<int>((tiles + least - 1) / least);
+  p.units = B * p.rows / kRows + g->count;
+  p.prefix_blocks = (static_cast<long long>(kv->kv_heads) * p.splits + 7) / 8 * 8 * p.units;
+  const size_t blocks = static_cast<size_t>(p.splits) * p.units * kWaves * kv->kv_heads;
+  p.prefix_o = blocks * 32 * D * 4;
+  p.prefix_ml = blocks * 32 * 8;
+  // Own tokens: what is left of a round of workgroups, a tile for a wave at least.
+  long long most = at_once - units * p.splits;
+  most = most > at_once / 4 ? most : at_once / 4;
+  const long long need = (own * p.rt + kWaves - 1) / kWaves;
+  p.own_blocks = static_cast<int>(need < most ? need : most);
+  p.own_least = 1;
+  const size_t slots = (2 * static_cast<size_t>(p.ranges()) + p.segments) * p.part_rows;
+  p.own_o = slots * D * 4;
+  p.own_ml = padded(slots * 8);
+  p.places = static_cast<size_t>(p.segments) * 16;
   return p;
 }
 
 template <typename T, int D>
-int launch(const PrefixArgs& a, const OwnDecodeArgs& o, const SharedPlan& p, hipStream_t stream) {
-  auto prefix = paged_prefix_kernel<T, D>;
-  if (!allow_lds(prefix, kPrefillLds<D>)) return CUDALM_W4A16_ELAUNCH;
-  prefix<<<static_cast<unsigned>(p.units * a.kv.kv_heads * a.splits), 64 * kWaves, kPrefillLds<D>, stream>>>(a);
+int launch(const SharedArgs& a, const SharedPlan& p, hipStream_t stream) {
+  auto kernel = p.rt == 1 ? paged_shared_kernel<T, D, 1> : p.rt == 2 ? paged_shared_kernel<T, D, 2>
+                                                                     : paged_shared_kernel<T, D, 4>;
+  if (!allow_lds(kernel, kLdsBytes<D>)) return CUDALM_W4A16_ELAUNCH;
+  const unsigned prefix = static_cast<unsigned>(p.prefix_blocks);
+  kernel<<<prefix + p.own_blocks, 64 * kWaves, kLdsBytes<D>, stream>>>(a, prefix);
   if (const int rc = launch_status()) return rc;
-  auto own = p.rt == 1 ? paged_own_kernel<T, D, 1> : p.rt == 2 ? paged_own_kernel<T, D, 2> : paged_own_kernel<T, D, 4>;
-  own<<<p.groups, 256, 0, stream>>>(o);
-  if (const int rc = launch_status()) return rc;
-  const unsigned rows = static_cast<unsigned>(a.tokens) * a.heads;
-  paged_shared_join_kernel<T, D><<<rows, 256, 0, stream>>>(o, a.part_o, a.part_ml, a.splits);
+  constexpr int PC = 2, kChunks = D / 8 / PC;
+  const unsigned tiles = static_cast<unsigned>((static_cast<long long>(a.kv.batch) * a.rows + 31) / 32);
+  paged_shared_join_kernel<T, D, PC><<<tiles * a.kv.kv_heads * kChunks, 256, 0, stream>>>(a, kChunks);
   return launch_status();
 }
 
 template <typename T>
-int launch_d(int D, const PrefixArgs& a, const OwnDecodeArgs& o, const SharedPlan& p, hipStream_t stream) {
-  return D == 64    ? launch<T, 64>(a, o, p, stream)
-         : D == 128 ? launch<T, 128>(a, o, p, stream)
-                    : launch<T, 256>(a, o, p, stream);
+int launch_d(int D, const SharedArgs& a, const SharedPlan& p, hipStream_t stream) {
+  return D == 64    ? launch<T, 64>(a, p, stream)
+         : D == 128 ? launch<T, 128>(a, p, stream)
+                    : launch<T, 256>(a, p, stream);
 }
 
 int check(const cudalm_paged_kv* kv, const cudalm_paged_query* q, const cudalm_paged_groups* g, int new_tokens) {
   if (const int rc = paged_check_query(kv, q)) return rc;
   if (!g) return CUDALM_W4A16_ENULL;
-  if (new_tokens < 1 || g->count < 1) return CUDALM_W4A16_EINVAL;
-  if (static_cast<long long>(new_tokens) * (q->heads / kv->kv_heads) > kMaxRows) return CUDALM_W4A16_EINVAL;
+  if (new_tokens < 1 || g->count < 1 || g->count > kv->batch ||
+      static_cast<long long>(new_tokens) * (q->heads / kv->kv_heads) > kMaxRows)
+    return CUDALM_W4A16_EINVAL;
   if (!g->cu || !g->shared) return CUDALM_W4A16_ENULL;
   if (!aligned(g->cu, 4) || !aligned(g->shared, 4)) return CUDALM_W4A16_EALIGN;
-  const long long rows = static_cast<long long>(kv->batch) * new_tokens * q->heads;
-  if (rows >= kMaxGemmTiles || g->count > kv->batch) return rows >= kMaxGemmTiles ? CUDALM_W4A16_ERANGE : CUDALM_W4A16_EINVAL;
+  // rows, blocks of 32 of them and own tiles (with where the last range would end) are
+  // numbered in 31 bits
+  if (static_cast<long long>(kv->batch) * new_tokens * q->heads >= kMaxGemmTiles) return CUDALM_W4A16_ERANGE;
   const SharedPlan p = plan_of(kv, q, g, new_tokens);
-  // own tiles are numbered in 31 bits, and where the last workgroup's range would end
   const long long cap = (static_cast<long long>(kv->max_pages) * kv->page_size + kTile - 1) / kTile;
-  const long long tiles = p.segments * (cap + 1);
-  if (tiles + tiles / p.groups + p.groups >= (1LL << 31)) return CUDALM_W4A16_ERANGE;
-  if (p.segments >= kMaxGemmTiles || p.units * kv->kv_heads * p.splits >= kMaxGemmTiles) return CUDALM_W4A16_ERANGE;
+  const long long tiles = p.segments * (cap + 1), ranges = p.ranges();
+  if (tiles + tiles / ranges + ranges >= (1LL << 31) || p.prefix_blocks + p.own_blocks >= kMaxGemmTiles ||
+      p.units * kRows >= (1LL << 31))
+    return CUDALM_W4A16_ERANGE;
   return CUDALM_W4A16_OK;
 }
 
@@ -177,50 +1011,41 @@ extern "C" int cudalm_paged_decode_shared(const cudalm_paged_kv* kv, const cudal
   const SharedPlan p = plan_of(kv, q, groups, new_tokens);
   if (workspace_bytes < p.bytes()) return CUDALM_W4A16_ERANGE;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  PrefixArgs a = {};
+  auto take = [&](size_t bytes) {
+    uint8_t* at = ws;
+    ws += bytes;
+    return at;
+  };
+  SharedArgs a = {};
   a.kv = view_of(kv);
+  a.sharing = {groups->cu, groups->shared, groups->count};
   a.k = static_cast<const uint16_t*>(kv->k);
   a.v = static_cast<const uint16_t*>(kv->v);
   a.q = static_cast<const uint16_t*>(q->q);
   a.out = static_cast<uint16_t*>(q->out);
-  a.part_o = reinterpret_cast<float*>(ws);
-  a.part_ml = reinterpret_cast<float*>(ws + p.prefix_o);
   a.token_stride = q->token_stride;
   a.head_stride = q->head_stride;
   a.negate = q->scale < 0;
-  a.scale_log2 = fmaxf((a.negate ? -q->scale : q->scale) * kLog2e, 1e-38f);  // (as in prefill)
-  a.tokens = kv->batch * new_tokens;
+  // Not zero: hidden scores of -inf are multiplied by it.
+  a.scale_log2 = fmaxf((a.negate ? -q->scale : q->scale) * kLog2e, 1e-38f);
+  a.new_tokens = new_tokens;
   a.heads = q->heads;
   a.group = q->heads / kv->kv_heads;
-  a.units = static_cast<int>(p.units);
-  a.splits = p.splits;
-  a.least = 1;
+  a.rows = p.rows;
   a.window = window_of(q);
   a.sinks = sinks_of(q);
-  a.sharing = {groups->cu, groups->shared, groups->count};
-  a.new_tokens = new_tokens;
-  OwnDecodeArgs o = {};
-  o.kv = a.kv;
-  o.k = a.k;
-  o.v = a.v;
-  o.q = a.q;
-  o.out = q->out;
-  o.part_o = reinterpret_cast<float*>(ws + p.prefix_o + p.prefix_ml);
-  o.part_ml = reinterpret_cast<float*>(ws + p.prefix_o + p.prefix_ml + p.own_o);
-  o.token_stride = q->token_stride;
-  o.head_stride = q->head_stride;
-  o.scale_log2 = q->scale * kLog2e;
-  o.new_tokens = new_tokens;
-  o.group = a.group;
-  o.rows = p.rows;
-  o.zrows = p.zrows;
-  o.part_rows = p.part_rows;
-  o.groups = p.groups;
-  o.splits = 0;
-  o.least = p.least;
-  o.window = a.window;
-  o.sinks = a.sinks;
-  o.sharing = a.sharing;
-  return kv->type == CUDALM_PAGED_BF16 ? launch_d<PagedBf16>(kv->head_dim, a, o, p, stream)
-                                       : launch_d<PagedF16>(kv->head_dim, a, o, p, stream);
+  a.prefix_o = reinterpret_cast<f32x4_t*>(take(p.prefix_o));
+  a.prefix_ml = reinterpret_cast<float2*>(take(p.prefix_ml));
+  a.units = static_cast<int>(p.units);
+  a.splits = p.splits;
+  a.least = p.least;
+  a.own_o = reinterpret_cast<float*>(take(p.own_o));
+  a.own_ml = reinterpret_cast<float2*>(take(p.own_ml));
+  a.places = reinterpret_cast<int4*>(take(p.places));
+  a.zrows = p.zrows;
+  a.part_rows = p.part_rows;
+  a.ranges = p.ranges();
+  a.own_least = p.own_least;
+  return kv->type == CUDALM_PAGED_BF16 ? launch_d<PagedBf16>(kv->head_dim, a, p, stream)
+                                       : launch_d<PagedF16>(kv->head_dim, a, p, stream);
 }
