@@ -13,6 +13,7 @@
 // second one.
 
 #include <cmath>
+#include <type_traits>
 
 #include "paged_device.h"
 
@@ -109,28 +110,35 @@ struct SharedArgs {
 
 // --- prefixes ---------------------------------------------------------------------
 
-// N times 16 bytes per lane from base (wave-uniform) + offset to LDS: lane i's of load x
-// land at dst + 4096 x + 16 i. The compiler's builtin for it makes every later LDS read
-// wait for all such loads, those of later tiles among them; here loads_landed() does the
-// waiting.
+// N times 16 bytes per lane from base[x / 2] (wave-uniform) + offset[x % 2] to LDS: lane
+// i's of load x land at dst + 4096 x + 16 i. The compiler's builtin for it makes every
+// later LDS read wait for all such loads, those of later tiles among them; here
+// loads_landed() does the waiting. (m0 holds the LDS address for the instruction.)
 template <int N>
-__device__ __forceinline__ void load_lds16(const uint16_t* const* base, const uint32_t* offset, uint32_t dst) {
-  uint32_t saved;  // m0 holds the LDS address for the instruction
-  if constexpr (N == 1) {
+__device__ __forceinline__ void load_lds16(const uint64_t* base, const uint32_t* offset, uint32_t dst) {
+  uint32_t saved;
+  if constexpr (N == 1)
     asm volatile(
         "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
         : "=&s"(saved)
         : "s"(dst), "v"(offset[0]), "s"(base[0])
         : "memory");
-  } else {
+  else if constexpr (N == 2)
     asm volatile(
         "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\t"
-        "s_mov_b32 m0, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %5, %6\n\ts_mov_b32 m0, %0"
+        "s_add_u32 m0, m0, 0x1000\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %4\n\ts_mov_b32 m0, %0"
         : "=&s"(saved)
-        : "s"(dst), "v"(offset[0]), "s"(base[0]), "s"(dst + 4096), "v"(offset[1]), "s"(base[1])
-        : "memory");
-    if constexpr (N > 2) load_lds16<N - 2>(base + 2, offset + 2, dst + 8192);
-  }
+        : "s"(dst), "v"(offset[0]), "s"(base[0]), "s"(base[1])
+        : "memory", "scc");
+  else
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %4\n\t"
+        "s_add_u32 m0, m0, 0x1000\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %4\n\t"
+        "s_add_u32 m0, m0, 0x1000\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %5\n\t"
+        "s_add_u32 m0, m0, 0x1000\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %5\n\ts_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "s"(dst), "v"(offset[0]), "v"(offset[1]), "s"(base[0]), "s"(base[1])
+        : "memory", "scc");
 }
 
 // This wave's loads have landed but for the last N; a barrier after it speaks for all waves.
@@ -191,17 +199,17 @@ __device__ __forceinline__ void prefix_body(const SharedArgs& a, uint16_t* lds, 
   const int parts = prefix_parts((length + KT - 1) >> kTileShift, a.splits, a.least);
   if (split >= parts) return;
 
-  // this lane's row (one past the last stands for it, and sees nothing), and the positions
-  // of the wave's and the workgroup's first and last
+  // this lane's row (rows past the last are copies of it), and the positions of the wave's
+  // and the workgroup's first and last
   const int wave_row = row0 + 32 * wave, row = wave_row + n;
   const bool real = row < rows;
   const int token = (real ? row : rows - 1) / a.group;
   const int seq = b + token / a.new_tokens;
-  int pos = a.kv.length(seq) - a.new_tokens + token % a.new_tokens;
+  const int pos = a.kv.length(seq) - a.new_tokens + token % a.new_tokens;
   u32x4_t qf[KK];
   {
     const uint16_t* qp = a.q + (static_cast<long long>(b) * a.new_tokens + token) * a.token_stride +
-                         (static_cast<long long>(h) * a.group + (real ? row - token * a.group : 0)) * a.head_stride +
+                         (static_cast<long long>(h) * a.group + (real ? row : rows - 1) - token * a.group) * a.head_stride +
                          8 * half;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
@@ -228,8 +236,6 @@ __device__ __forceinline__ void prefix_body(const SharedArgs& a, uint16_t* lds, 
     wg_last = uniform(wg_last);
     __syncthreads();
   }
-  if (!real) pos = -1;
-  if (wave_row >= rows) wave_last = -1;  // nothing to multiply
   const PagedRange tiles(0, length, wg_first, wg_last, a.window, a.sinks);
   const int per = tiles_per_split(tiles.count, parts, 1);
   const int begin = split * per, end = begin + per < tiles.count ? begin + per : tiles.count;
@@ -240,79 +246,68 @@ __device__ __forceinline__ void prefix_body(const SharedArgs& a, uint16_t* lds, 
   const int P = 1 << a.kv.page_shift;
   const size_t page_elems = static_cast<size_t>(P) * D * a.kv.kv_heads;
   const size_t head_elems = static_cast<size_t>(P) * D * h;
-  // A wave loads 1 KB pieces wave, wave + 4, .. of a unit. Key row r of piece 4 x + wave is r0
-  // + x kStep: its token is that of r0 plus a number that all lanes share, and the exchange of its
-  // chunks is the same for every x (but for chunk bit 3 where D = 256). So one or two offsets
-  // per lane serve all loads.
-  constexpr int kStep = 2048 / D;
+  // A wave loads 1 KB pieces wave, wave + 4, .. of a unit; of a half's 16 tokens, two (D =
+  // 256: one with each offset), one, or half of one. Key row r of piece 4 x + wave is r0 + x
+  // 2048 / D: its token is that of r0 plus a number that all lanes share, and the exchange of its
+  // chunks is the same for every x but for chunk bit 3 where D = 256.
   const int r0 = wave * (512 / D) + lane / C;
-  const uint32_t k_lane = 2 * (swap_bits_2_3(r0) % 16 * D + 8 * ((lane % C) ^ chunk_exchange<D>(r0)));
   const int v_piece = wave * 64;  // in channels of the tile's groups of eight tokens
-  const uint32_t v_lane = 16 * (v_piece % D + lane);
+  // bytes from the half's first key, value
+  const uint32_t k_lane = 2 * (swap_bits_2_3(r0) % 16 * D + 8 * ((lane % C) ^ chunk_exchange<D>(r0)));
+  const uint32_t v_lane = 16 * (v_piece % D + lane) + (v_piece / D % 2) * 16 * D;
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)) + wave * 1024;
+  const uint32_t k_lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)) +
+                         2 * (n * D + 8 * (half ^ chunk_exchange<D>(n)));
 
   // every row from position `from` to `to` sees all of the tile at t
   auto seen_whole = [&](int t, int from, int to) {
     return t + KT <= length && t + KT - 1 <= from && (a.window <= 0 || t > to - a.window || t + KT - 1 < a.sinks);
   };
-  const bool wg_full = row0 + kRows <= rows, wave_full = wave_row + 32 <= rows;
   // Places, pages and visibility of 32 tiles: lanes 2 i and 2 i + 1 hold the halves of tile
-  // i, masks a bit each, and those of the 32 before, since loads run ahead of products.
-  uint64_t half_at = 0;  // of the half's first key, and value, in its cache
+  // i, masks a bit each; and those of the 32 before, since loads run ahead of products.
+  uint64_t k_at = 0;  // of the half's first key; its first value is as far from the first of all
+  const uint64_t to_v = reinterpret_cast<uint64_t>(a.v) - reinterpret_cast<uint64_t>(a.k);
   struct Masks {
     uint64_t absent, whole, wg_whole;
-  } masks = {0, 0, 0}, old_masks = masks;
+    bool plain;  // all here, and seen by all rows
+  } masks = {0, 0, 0, false}, old_masks = masks;
   int ahead = begin;  // the first tile of the 32
   auto look_ahead = [&](int i) {
     old_masks = masks;
     ahead = i;
     const int first_token = tiles.tile(i + lane / 2) << kTileShift, t = first_token + 16 * (lane & 1);
+    const bool in = i + lane / 2 < end;
     int page = -1;
-    if (i + lane / 2 < end) page = a.kv.page(b, t >> a.kv.page_shift);
+    if (in) page = a.kv.page(b, t >> a.kv.page_shift);
     // absent pages are hidden below; any page will do
-    half_at = max(page, 0) * page_elems + head_elems + static_cast<uint64_t>(t & (P - 1)) * D;
+    k_at = reinterpret_cast<uint64_t>(a.k) +
+           2 * (max(page, 0) * page_elems + head_elems + static_cast<uint64_t>(t & (P - 1)) * D);
     masks.absent = __ballot(page < 0);
-    masks.whole = __ballot(wave_full && seen_whole(first_token, wave_first, wave_last));
-    masks.wg_whole = __ballot(wg_full && seen_whole(first_token, wg_first, wg_last));
+    masks.whole = __ballot(seen_whole(first_token, wave_first, wave_last));
+    masks.wg_whole = __ballot(seen_whole(first_token, wg_first, wg_last));
+    masks.plain = !__any(in && (page < 0 || !seen_whole(first_token, wg_first, wg_last)));
   };
-  auto half_place = [&](int x) { return readlane64(half_at, x); };
   const int units = 2 * (end - begin);
   int into = 0;  // the place of the next unit
   auto issue = [&](int u) {
     const int x = u & 63;
     if (x == 0 && u > 0) look_ahead(begin + u / 2);
-    const uint64_t at0 = half_place(x & ~1), at1 = half_place(x | 1);
-    const uint16_t* base[kLoads];
-    uint32_t offset[kLoads];
-    if (x & 1) {
-#pragma unroll
-      for (int y = 0; y < kLoads; ++y) {
-        const int group = y * (2048 / (8 * D)) + v_piece / D;
-        base[y] = a.v + (group & 2 ? at1 : at0) + (group & 1) * 8 * D;
-        offset[y] = v_lane;
-      }
-    } else {
-#pragma unroll
-      for (int y = 0; y < kLoads; ++y) {
-        // rows of the piece: tokens of 16-token half r / 16, bit 3 of r is bit 2 of the token
-        const int r = y * kStep + wave * (512 / D);
-        const bool odd = D == 256 && (y & 1);
-        base[y] = a.k + (r & 16 ? at1 : at0) + (odd ? 4 * D : 0);
-        offset[y] = odd ? k_lane ^ 128 : k_lane;
-      }
-    }
+    const uint64_t more = x & 1 ? to_v : 0;
+    uint64_t base[2];
+    // (of 64 channels a wave has half of one half)
+    base[0] = readlane64(k_at, kLoads == 1 ? (x & ~1) + wave / 2 : x & ~1) + more;
+    base[1] = kLoads == 1 ? 0 : readlane64(k_at, x | 1) + more;
+    uint32_t offset[2] = {x & 1 ? v_lane : k_lane, 0};
+    asm volatile("" : "+v"(offset[0]));  // (the other is made here, not held in a register)
+    offset[1] = x & 1 ? offset[0] + 16 * D : (offset[0] ^ 128) + 8 * D;
     load_lds16<kLoads>(base, offset, lds0 + into * (2 * kUnit));
     into = into + 1 == R ? 0 : into + 1;
   };
-  // Unit u is there for all waves, and all have read unit u - 1.
+  // Unit u is there for all waves, and all have read unit u - 1. (The last ones wait for
+  // all that is on its way.)
   auto arrive = [&](int u) {
-    const int after = units - 1 - u;  // those issued by now but for the last R - 2
-    if (after >= R - 2)
+    if (u + R <= units + 1)
       loads_landed<(R - 2) * kLoads>();
-    else if (after >= 2)
-      loads_landed<2 * kLoads>();
-    else if (after == 1)
-      loads_landed<kLoads>();
     else
       loads_landed<0>();
     barrier();
@@ -352,26 +347,33 @@ __device__ __forceinline__ void prefix_body(const SharedArgs& a, uint16_t* lds, 
   look_ahead(begin);
   for (int u = 0; u < R - 1 && u < units; ++u) issue(u);
   int from = 0;  // the place of the next unit to be read
+  auto walk = [&](auto multiplies) {
 #pragma unroll 1
   for (int u = 0; u < units; u += 2) {
-    const int tile = begin + u / 2, t0 = tiles.tile(tile) << kTileShift;
+    const int tile = begin + u / 2;
     arrive(u);
     if (u - 1 + R < units) issue(u - 1 + R);
-    const Masks& now = tile < ahead ? old_masks : masks;
-    const int bit = u & 63;
-    const uint32_t absent = static_cast<uint32_t>(now.absent >> bit) & 3;
-    const bool whole = !absent && ((now.whole >> bit) & 1), wg_whole = !absent && ((now.wg_whole >> bit) & 1);
-    const bool work = t0 <= wave_last;  // not above the wave's rows
+    int t0 = 0;
+    uint32_t absent = 0;
+    bool whole = true, wg_whole = true;
+    if (!(tile < ahead ? old_masks.plain : masks.plain)) {
+      const Masks now = tile < ahead ? old_masks : masks;
+      const int bit = u & 63;
+      t0 = tiles.tile(tile) << kTileShift;
+      absent = static_cast<uint32_t>(now.absent >> bit) & 3;
+      whole = !absent && ((now.whole >> bit) & 1);
+      wg_whole = !absent && ((now.wg_whole >> bit) & 1);
+    }
     f32x16_t s;
-    u32x4_t pf[2];
-    if (work) {
-      const uint16_t* kt = lds + from * kUnit;
+    if constexpr (multiplies) {
+      // chunk (2 kk + half) ^ chunk_exchange of row n: kk only flips bits 5 .. of the place
+      const uint32_t key = k_lds + from * (2 * kUnit);
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = 0;
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk)
-        s = T::mfma32(load16(kt + n * D + 8 * ((2 * kk + half) ^ chunk_exchange<D>(n))), qf[kk], s);
+        s = T::mfma32(*reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(key ^ (32 * kk)), qf[kk], s);
       __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
       for (int kk = 0; kk < KK - kAhead; ++kk) {
@@ -380,6 +382,16 @@ __device__ __forceinline__ void prefix_body(const SharedArgs& a, uint16_t* lds, 
       }
       __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
       __builtin_amdgcn_s_setprio(0);
+    }
+    from = from + 1 == R ? 0 : from + 1;
+    arrive(u + 1);
+    if (u + R < units) issue(u + R);
+    uint16_t* vt = lds + from * kUnit;
+    if (!wg_whole) {
+      clean(reinterpret_cast<u32x4_t*>(vt), t0, absent);
+      barrier();
+    }
+    if constexpr (multiplies) {
       // s[e] is the score of token t0 + 16 (e / 8) + 8 half + e % 8
       if (!whole) {
         // token t is seen from p if 0 <= p - t < window, or if t is a sink up to p
@@ -410,6 +422,8 @@ __device__ __forceinline__ void prefix_body(const SharedArgs& a, uint16_t* lds, 
         m = next;
       }
       float sum = 0;
+      const u32x4_t* vp = reinterpret_cast<const u32x4_t*>(vt) + half * D + n;
+      u32x4_t pf[2];
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
         const float p0 = exp2_fast(__builtin_fmaf(s[e], a.scale_log2, -m));
@@ -419,33 +433,30 @@ __device__ __forceinline__ void prefix_body(const SharedArgs& a, uint16_t* lds, 
         pf[e / 8][e % 8 / 2] = T::pack(p0, p1);
       }
       l += sum;
-    }
-    from = from + 1 == R ? 0 : from + 1;
-    arrive(u + 1);
-    if (u + R < units) issue(u + R);
-    uint16_t* vt = lds + from * kUnit;
-    if (!wg_whole) {
-      clean(reinterpret_cast<u32x4_t*>(vt), t0, absent);
-      barrier();
-    }
-    if (work) {
       __builtin_amdgcn_s_setprio(1);
-      constexpr int kFirst = 1 + D / 128;
-      const u32x4_t* vp = reinterpret_cast<const u32x4_t*>(vt) + half * D + n;
 #pragma unroll
       for (int x = 0; x < 2 * DT; ++x)
         o[x % DT] = T::mfma32(vp[(x / DT) * 2 * D + 32 * (x % DT)], pf[x / DT], o[x % DT]);
-      __builtin_amdgcn_sched_group_barrier(0x100, kFirst, 0);
+      if (D >= 128) {
+        constexpr int kFirst = 1 + D / 128;
+        __builtin_amdgcn_sched_group_barrier(0x100, kFirst, 0);
 #pragma unroll
-      for (int x = 0; x < 2 * DT - kFirst; ++x) {
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        for (int x = 0; x < 2 * DT - kFirst; ++x) {
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, kFirst, 0);
       }
-      __builtin_amdgcn_sched_group_barrier(0x008, kFirst, 0);
       __builtin_amdgcn_s_setprio(0);
     }
     from = from + 1 == R ? 0 : from + 1;
   }
+  };
+  const bool idle = wave_row >= rows;  // nothing to multiply
+  if (idle)
+    walk(std::false_type());
+  else
+    walk(std::true_type());
   // Inf or NaN for the sums of channels 32 dt .. whose rows see such a value: how many
   // tokens hold +Inf or NaN, -Inf or NaN. In tiles that were not cleaned a weight that
   // underflows has made NaN of Inf, so what the sums hold there does not count.
@@ -495,7 +506,7 @@ __device__ __forceinline__ void prefix_body(const SharedArgs& a, uint16_t* lds, 
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) special |= votes[w];
   special = uniform(special);
-  if (wave_row >= rows) return;
+  if (idle) return;
   l += __shfl_xor(l, 32);
   const size_t at = (static_cast<size_t>(split) * (a.units * kWaves) + unit * kWaves + wave) * a.kv.kv_heads + h;
   // -inf tells the join that there is nothing to read: no weight here, nor Inf or NaN
@@ -796,15 +807,15 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu<D>) void paged_shared_kernel(co
 
 // --- the join -------------------------------------------------------------------------
 
-// 32 rows of a key-value head, PC pieces of eight channels; the waves of a workgroup take
-// every fourth part. A lane has the row n of a prefix's register order and four channels of a
+// 32 rows of a key-value head, PC pieces of eight channels; the WV waves of a workgroup take
+// every WV-th part. A lane has the row n of a prefix's register order and four channels of a
 // piece, so that a part's piece is one load of 1 KB. The maximum runs along, which saves a pass
 // over the parts' maxima.
-template <typename T, int D, int PC>
-__global__ __launch_bounds__(256) void paged_shared_join_kernel(const SharedArgs a, int chunks) {
+template <typename T, int D, int PC, int WV>
+__global__ __launch_bounds__(64 * WV) void paged_shared_join_kernel(const SharedArgs a, int chunks) {
   constexpr int kAtOnce = 8 / PC;
-  __shared__ f32x4_t sums[kWaves][PC][64];
-  __shared__ float2 tops[kWaves][32];
+  __shared__ f32x4_t sums[WV][PC][64];
+  __shared__ float2 tops[WV][32];
   const int lane = threadIdx.x & 63, wave = wave_id(), n = lane & 31, half = lane >> 5;
   const int chunk = blockIdx.x % chunks, h = blockIdx.x / chunks % a.kv.kv_heads;
   const int R = static_cast<int>(blockIdx.x / chunks / a.kv.kv_heads) * 32 + n;
@@ -816,12 +827,12 @@ __global__ __launch_bounds__(256) void paged_shared_join_kernel(const SharedArgs
 #pragma unroll
   for (int x = 0; x < PC; ++x) acc[x] = f32x4_t{0, 0, 0, 0};
   float m = kLowest, l = 0;
-  for (int s0 = wave; __any(s0 < count); s0 += kWaves * kAtOnce) {
+  for (int s0 = wave; __any(s0 < count); s0 += WV * kAtOnce) {
     float2 ml[kAtOnce];
     f32x4_t o[kAtOnce][PC];
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
-      const int s = s0 + kWaves * i;
+      const int s = s0 + WV * i;
       ml[i] = float2{-__builtin_inff(), 0};
       if (s < before) {
         const size_t at = (static_cast<size_t>(s) * (a.units * kWaves) + prow / 32) * a.kv.kv_heads + h;
@@ -866,11 +877,11 @@ __global__ __launch_bounds__(256) void paged_shared_join_kernel(const SharedArgs
   if (wave >= PC) return;
   float M = kLowest;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) M = fmaxf(M, tops[w][n].x);
+  for (int w = 0; w < WV; ++w) M = fmaxf(M, tops[w][n].x);
   l = 0;
   f32x4_t y = {0, 0, 0, 0};
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
+  for (int w = 0; w < WV; ++w) {
     const float weight = exp2_fast(tops[w][n].x - M);
     l += weight * tops[w][n].y;
 #pragma unroll
@@ -958,7 +969,10 @@ int launch(const SharedArgs& a, const SharedPlan& p, hipStream_t stream) {
   if (const int rc = launch_status()) return rc;
   constexpr int PC = 2, kChunks = D / 8 / PC;
   const unsigned tiles = static_cast<unsigned>((static_cast<long long>(a.kv.batch) * a.rows + 31) / 32);
-  paged_shared_join_kernel<T, D, PC><<<tiles * a.kv.kv_heads * kChunks, 256, 0, stream>>>(a, kChunks);
+  // Sixteen waves where there are parts for them.
+  const long long parts = p.splits + p.ranges() / p.segments + 1;
+  auto join = parts > 16 ? paged_shared_join_kernel<T, D, PC, 16> : paged_shared_join_kernel<T, D, PC, 4>;
+  join<<<tiles * a.kv.kv_heads * kChunks, parts > 16 ? 1024 : 256, 0, stream>>>(a, kChunks);
   return launch_status();
 }
 
