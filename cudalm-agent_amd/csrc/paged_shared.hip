@@ -813,7 +813,7 @@ __global__ __launch_bounds__(64 * kWaves, kPerCu<D>) void paged_shared_kernel(co
 // over the parts' maxima.
 template <typename T, int D, int PC, int WV>
 __global__ __launch_bounds__(64 * WV) void paged_shared_join_kernel(const SharedArgs a, int chunks) {
-  constexpr int kAtOnce = 8 / PC;
+  constexpr int kAtOnce = 4;
   __shared__ f32x4_t sums[WV][PC][64];
   __shared__ float2 tops[WV][32];
   const int lane = threadIdx.x & 63, wave = wave_id(), n = lane & 31, half = lane >> 5;
@@ -921,7 +921,7 @@ SharedPlan plan_of(const cudalm_paged_kv* kv, const cudalm_paged_query* q, const
   p.zrows = (row_tiles + p.rt - 1) / p.rt;
   p.part_rows = 16 * p.rt < p.rows ? 16 * p.rt : p.rows;
   p.segments = B * kv->kv_heads * p.zrows;
-  const int at_once = (D == 256 ? kPerCu<256> : D == 128 ? kPerCu<128> : kPerCu<64>) * cu_count();
+  const int per_cu = D == 256 ? kPerCu<256> : D == 128 ? kPerCu<128> : kPerCu<64>, at_once = per_cu * cu_count();
   // What is expected: tiles of the longest prefix, and of all sequences' own tokens.
   const int len = expected_len(kv, q->max_len), prefix = expected_len(kv, g->max_shared);
   const long long near = window > 0 ? (window + sinks_of(q)) / kTile + 3LL : 1LL << 30;
@@ -931,12 +931,13 @@ SharedPlan plan_of(const cudalm_paged_kv* kv, const cudalm_paged_query* q, const
   own = p.segments * (own < near ? own : near);
   // Prefixes: a workgroup per `least` tiles. Fewer tiles end sooner but leave more parts, whose
   // bytes are written and read: t tiles cost t steps and all rows' parts 2 rows 4 D (tiles / t) at
-  // 5 TB/s, least where the two are equal; and half of what runs at once is left for the own
-  // tokens.
+  // 5 TB/s, least where the two are equal. And of the workgroups that run at once, one on every
+  // CU is for own tokens (128 samples behind 32768 tokens, 256 channels: 70 us with half of them
+  // for prefixes, 92 with two thirds; 5 documents, 128 channels: 39 and 35).
   const long long units = (B * p.rows + kRows - 1) / kRows * kv->kv_heads;
-  const double bytes = 8.0 * B * p.rows * kv->kv_heads * D * tiles / 5e6, step = D == 256 ? 1.6 : D == 128 ? 1.0 : 0.7;
+  const double bytes = 8.0 * B * p.rows * kv->kv_heads * D * tiles / 5e6, step = D == 256 ? 1.0 : D == 128 ? 0.8 : 0.6;
   long long least = static_cast<long long>(std::sqrt(bytes / step) + 0.5);
-  const long long round = (units * tiles + at_once / 2 - 1) / (at_once / 2);
+  const long long room = static_cast<long long>(per_cu - 1) * cu_count(), round = (units * tiles + room - 1) / room;
   least = least < round ? round : least;
   least = least < 1 ? 1 : least > tiles ? tiles : least;
   p.least = static_cast<int>(least);
@@ -967,12 +968,18 @@ int launch(const SharedArgs& a, const SharedPlan& p, hipStream_t stream) {
   const unsigned prefix = static_cast<unsigned>(p.prefix_blocks);
   kernel<<<prefix + p.own_blocks, 64 * kWaves, kLdsBytes<D>, stream>>>(a, prefix);
   if (const int rc = launch_status()) return rc;
-  constexpr int PC = 2, kChunks = D / 8 / PC;
-  const unsigned tiles = static_cast<unsigned>((static_cast<long long>(a.kv.batch) * a.rows + 31) / 32);
-  // Sixteen waves where there are parts for them.
+  // Four pieces per wave read whole lines of rows; eight waves where there are parts for them;
+  // where that makes few workgroups, more of both. (16 rows of 40 parts on 2 heads of 256: 5.2 us,
+  // 6.0 with eight waves; 5120 rows of 128, 9 parts: 8.5, 10.2 with two pieces, 21 with sixteen
+  // waves; 1024 rows of 256, 35 parts: 9.7, 10.2 with four waves, 13.6 with sixteen.)
   const long long parts = p.splits + p.ranges() / p.segments + 1;
-  auto join = parts > 16 ? paged_shared_join_kernel<T, D, PC, 16> : paged_shared_join_kernel<T, D, PC, 4>;
-  join<<<tiles * a.kv.kv_heads * kChunks, parts > 16 ? 1024 : 256, 0, stream>>>(a, kChunks);
+  const unsigned tiles = static_cast<unsigned>((static_cast<long long>(a.kv.batch) * a.rows + 31) / 32) * a.kv.kv_heads;
+  if (tiles * (D / 32) < static_cast<unsigned>(cu_count()) / 4)
+    paged_shared_join_kernel<T, D, 2, 16><<<tiles * (D / 16), 1024, 0, stream>>>(a, D / 16);
+  else if (parts > 16)
+    paged_shared_join_kernel<T, D, 4, 8><<<tiles * (D / 32), 512, 0, stream>>>(a, D / 32);
+  else
+    paged_shared_join_kernel<T, D, 4, 4><<<tiles * (D / 32), 256, 0, stream>>>(a, D / 32);
   return launch_status();
 }
 

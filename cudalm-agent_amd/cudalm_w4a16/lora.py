@@ -18,13 +18,12 @@ import struct
 
 from . import _I, _P, _SZ, _check, _lib, _stream
 from . import paged_kv as _kv
-from .paged_kv import _L, _empty, _type_of, _workspace
+from .paged_kv import _L, _elsewhere, _empty, _type_of
 
 _SIGS = {
     "cudalm_lora_plan_bytes": ([_I, _I], _SZ),
     "cudalm_lora_plan": ([_P, _I, _I, _P, _SZ, _P], _I),
-    "cudalm_lora_workspace_bytes": ([_I, _I, _I, _I], _SZ),
-    "cudalm_lora_add": ([_P, _I, _P, _L, _I, _I, _I, _I, _I, _P, _P, _P, _P, _SZ, _P], _I),
+    "cudalm_lora_add": ([_P, _I, _P, _L, _I, _I, _I, _I, _I, _P, _P, _P, _P], _I),
 }
 for _name, (_args, _ret) in _SIGS.items():
     _fn = getattr(_lib, _name)
@@ -35,13 +34,17 @@ EXPORTED_SYMBOLS = tuple(_SIGS)
 
 MAX_PROJ = 8
 MAX_RANK = 256
-MAX_ADAPTERS = 8192
+MAX_ADAPTERS = 4096
 
 
 class Proj(ctypes.Structure):
     """struct cudalm_lora_proj."""
     _fields_ = [("a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("y", ctypes.c_void_p), ("out", ctypes.c_void_p),
                 ("y_stride", ctypes.c_int64), ("out_stride", ctypes.c_int64), ("N", ctypes.c_int)]
+
+
+# an array of them as bytes, by their number
+_PACK = [struct.Struct("4P2qi4x" * n).pack for n in range(MAX_PROJ + 1)]
 
 
 def _need(ok, what):
@@ -54,12 +57,7 @@ class Plan:
 
     def __init__(self, memory, M, adapters):
         self.memory, self.M, self.adapters, self.index = memory, M, adapters, memory.get_device()
-
-
-def _elsewhere(index) -> bool:
-    import torch
-
-    return index >= 0 and index != torch.cuda.current_device()
+        self.at = memory.data_ptr()
 
 
 def plan(index, adapters: int, out: Plan | None = None, stream=None) -> Plan:
@@ -83,58 +81,68 @@ def plan(index, adapters: int, out: Plan | None = None, stream=None) -> Plan:
     return out
 
 
-def _matrix(t, M, N, dtype, gpu, name):
-    """Row stride of t [M, N]; N where there is one row."""
-    if (t.dim() != 2 or t.shape[0] != M or (N and t.shape[1] != N) or t.dtype != dtype or t.get_device() != gpu or
-            (t.stride(1) != 1 and t.shape[1] != 1)):
-        raise ValueError(f"lora: {name} is [{M}, {N or 'N'}] in x's type and on its GPU, a row's elements contiguous")
-    return t.stride(0) if M > 1 else t.shape[1]
+def _bad(name, shape):
+    raise ValueError(f"lora: {name} is {shape} in x's type and on its GPU, a row's elements contiguous")
 
 
-def add(x, ys, a, b, plan: Plan, scales=None, ranks=None, outs=None, workspace=None, stream=None):
+def add(x, ys, a, b, plan: Plan, scales=None, ranks=None, outs=None, stream=None):
     """out_j[m] = y_j[m] + scales[i] * B_j[i] (A_j[i] x[m]) with i the adapter of row m;
     rows of none keep y. x [M, K]; ys, a, b (and outs): one tensor, or a list of up to 8 for
     projections that share x: y [M, N], a [adapters, rank, K], b [adapters, N, rank]. The
     results replace ys, or go to outs. scales [adapters] float32 (None: 1); ranks
     [adapters] int32 (None: all the same): what adapter i uses of the rank, the rest is
     padding. Returns the results, as ys came."""
-    import torch
-
+    if not isinstance(ys, (list, tuple)):
+        return add(x, [ys], [a], [b], plan, scales, ranks, None if outs is None else [outs], stream)[0]
     gpu, dtype = x.get_device(), x.dtype
     kind = _type_of(dtype)
-    if gpu < 0 or x.dim() != 2 or plan.index != gpu or plan.M != x.shape[0]:
+    shape = x.shape
+    M = plan.M
+    if gpu < 0 or len(shape) != 2 or plan.index != gpu or shape[0] != M:
         raise ValueError("lora: x is [M, K] on the GPU of its plan")
     if _elsewhere(gpu):
+        import torch
+
         with torch.cuda.device(gpu):
-            return add(x, ys, a, b, plan, scales, ranks, outs, workspace, stream)
-    if isinstance(ys, torch.Tensor):
-        return add(x, [ys], [a], [b], plan, scales, ranks, None if outs is None else [outs], workspace, stream)[0]
+            return add(x, ys, a, b, plan, scales, ranks, outs, stream)
+    K = shape[1]
+    s = x.stride()
+    if s[1] != 1 and K != 1:
+        _bad("x", [M, K])
+    x_stride = s[0] if M > 1 else K
     if outs is None:
         outs = ys
     count, L = len(ys), plan.adapters
     if not 1 <= count <= MAX_PROJ or len(a) != count or len(b) != count or len(outs) != count:
         raise ValueError(f"lora: ys, a, b and outs are as many, 1 to {MAX_PROJ}")
-    M, K = x.shape
-    x_stride = _matrix(x, M, K, dtype, gpu, "x")
     R = a[0].shape[1] if a[0].dim() == 3 else 0
     fields = []
     for y, fa, fb, out in zip(ys, a, b, outs):
-        ysd = _matrix(y, M, 0, dtype, gpu, "y")
-        N = y.shape[1]
+        shape, s = y.shape, y.stride()
+        if len(shape) != 2 or shape[0] != M or y.dtype != dtype or y.get_device() != gpu or (s[1] != 1 and shape[1] != 1):
+            _bad("y", [M, "N"])
+        N = shape[1]
+        step = to = s[0] if M > 1 else N
+        if out is not y:
+            s = out.stride()
+            if out.shape != shape or out.dtype != dtype or out.get_device() != gpu or (s[1] != 1 and N != 1):
+                _bad("out", [M, N])
+            to = s[0] if M > 1 else N
         if (fa.shape != (L, R, K) or fb.shape != (L, N, R) or fa.dtype != dtype or fb.dtype != dtype or
                 fa.get_device() != gpu or fb.get_device() != gpu or not fa.is_contiguous() or not fb.is_contiguous()):
             raise ValueError(f"lora: a and b are contiguous [{L}, rank, {K}] and [{L}, {N}, rank] in x's type and on its GPU")
-        osd = ysd if out is y else _matrix(out, M, N, dtype, gpu, "out")
-        fields += (fa.data_ptr(), fb.data_ptr(), y.data_ptr(), out.data_ptr(), ysd, osd, N)
-    for t, want, name in ((scales, torch.float32, "scales"), (ranks, torch.int32, "ranks")):
-        if t is not None and (t.shape != (L,) or t.dtype != want or t.get_device() != gpu or not t.is_contiguous()):
-            raise ValueError(f"lora: {name} is a contiguous {want} tensor [{L}] on x's GPU")
-    need = 0
-    if workspace is None:
-        need = _lib.cudalm_lora_workspace_bytes(count, M, R, kind)
-    at, size, held = _workspace(need, workspace, gpu, stream)
-    rc = _lib.cudalm_lora_add(struct.pack("4P2qi4x" * count, *fields), count, x.data_ptr(), x_stride, K, M, R, L, kind,
-                              None if scales is None else scales.data_ptr(), None if ranks is None else ranks.data_ptr(),
-                              plan.memory.data_ptr(), at, size, _stream(stream))
-    _check(rc, "cudalm_lora_add")
+        fields += (fa.data_ptr(), fb.data_ptr(), y.data_ptr(), out.data_ptr(), step, to, N)
+    sp = rp = None
+    if scales is not None:
+        if scales.shape != (L,) or scales.dtype != _kv._float32_type or scales.get_device() != gpu or not scales.is_contiguous():
+            raise ValueError(f"lora: scales is a contiguous float32 tensor [{L}] on x's GPU")
+        sp = scales.data_ptr()
+    if ranks is not None:
+        if ranks.shape != (L,) or ranks.dtype != _kv._int32_type or ranks.get_device() != gpu or not ranks.is_contiguous():
+            raise ValueError(f"lora: ranks is a contiguous int32 tensor [{L}] on x's GPU")
+        rp = ranks.data_ptr()
+    rc = _lib.cudalm_lora_add(_PACK[count](*fields), count, x.data_ptr(), x_stride, K, M, R, L, kind, sp, rp, plan.at,
+                              _stream(stream))
+    if rc:
+        _check(rc, "cudalm_lora_add")
     return outs

@@ -202,10 +202,20 @@ def _empty(shape, dtype, index, stream):
         return torch.empty(shape, dtype=dtype, device=_devices(index))
 
 
-def _current_device() -> int:
-    import torch
+_current_device = None  # torch's accessor, once a call needs it
 
-    return torch.cuda.current_device()
+
+def _elsewhere(index) -> bool:
+    """Whether the GPU of a call's tensors is not the current one, which launches go to."""
+    global _current_device
+    if _current_device is None:
+        import torch
+
+        try:
+            _current_device = torch._C._cuda_getDevice
+        except AttributeError:  # a torch without GPUs, or without this accessor
+            _current_device = torch.cuda.current_device
+    return index >= 0 and index != _current_device()
 
 
 def _workspace(nbytes, workspace, index, stream):
@@ -311,7 +321,7 @@ def decode_shared(q, k, v, tables, lens, cu_groups, shared, scale=None, window: 
     sequence, whatever the other sequences' tables hold there. max_shared is what the
     caller knows of the longest prefix. Other arguments as in decode()."""
     kv, index = _cache(k, v, tables, lens, None)
-    if index != _current_device():
+    if _elsewhere(index):
         import torch
 
         with torch.cuda.device(index):

@@ -16,7 +16,7 @@ import struct
 
 from . import _I, _P, _check, _lib, _stream
 from . import paged_kv as _kv
-from .paged_kv import _L, _cache, _empty, _int32, _rows, _type_of
+from .paged_kv import _L, _cache, _elsewhere, _empty, _int32, _rows, _type_of
 
 _SIGS = {
     "cudalm_rotary_rotate": ([_P, _P, _I, _I, _I, _P, _P], _I),
@@ -94,51 +94,43 @@ def _positions(rot, positions, T, index):
     return positions.data_ptr()
 
 
-def _strides(t):
+def _strides(shape, s):
     """(token stride, head stride) of [T, heads, D]; 0 where a dimension has one entry."""
-    s = t.stride()
-    return s[0] if t.shape[0] != 1 else 0, s[1] if t.shape[1] != 1 else 0
+    return s[0] if shape[0] != 1 else 0, s[1] if shape[1] != 1 else 0
 
 
-def _out(x, out, stream):
+def _out(x, shape, dtype, index, out, stream):
+    """(out, its token and head strides)."""
     if out is None:
-        return _empty(x.shape, x.dtype, x.get_device(), stream)
-    if (out.shape != x.shape or out.dtype != x.dtype or out.get_device() != x.get_device() or
-            (out.stride(2) != 1 and x.shape[2] != 1)):
+        out = _empty(shape, dtype, index, stream)
+    s = out.stride()
+    if (out is not x and (out.shape != shape or out.dtype != dtype or out.get_device() != index)) or (
+            s[2] != 1 and shape[2] != 1):
         raise ValueError("rotary: out is like the rows, a head's elements contiguous")
-    return out
-
-
-def _on(index):
-    """The device of a call's tensors, where it is not the current one: launches go to it."""
-    import torch
-
-    return torch.cuda.device(index)
-
-
-def _elsewhere(index) -> bool:
-    import torch
-
-    return index >= 0 and index != torch.cuda.current_device()
+    return out, _strides(shape, s)
 
 
 def rotate(x, positions, rot: Rotary, out=None, stream=None):
     """x [T, heads, D] rotated by positions [axes, T] (or [T] for one axis), int32;
     into `out`, which may be x itself, or a new tensor. Any strides of tokens and
     heads."""
-    index = x.get_device()
-    kind = _type_of(x.dtype)
-    if x.dim() != 3 or (x.stride(2) != 1 and x.shape[2] != 1) or index < 0 or index != rot.index:
+    index, dtype = x.get_device(), x.dtype
+    kind = _type_of(dtype)
+    shape, s = x.shape, x.stride()
+    if len(shape) != 3 or (s[2] != 1 and shape[2] != 1) or index < 0 or index != rot.index:
         raise ValueError("rotary: x is [T, heads, D] on the GPU of the frequencies, a head's elements contiguous")
     if _elsewhere(index):
-        with _on(index):
+        import torch
+
+        with torch.cuda.device(index):
             return rotate(x, positions, rot, out, stream)
-    T, heads, D = x.shape
-    out = _out(x, out, stream)
+    T, heads, D = shape
+    out, to = _out(x, shape, dtype, index, out, stream)
     at = _positions(rot, positions, T, index)
-    rc = _lib.cudalm_rotary_rotate(rot._bytes, _pack_rows(x.data_ptr(), out.data_ptr(), *_strides(x), *_strides(out), heads),
+    rc = _lib.cudalm_rotary_rotate(rot._bytes, _pack_rows(x.data_ptr(), out.data_ptr(), *_strides(shape, s), *to, heads),
                                    T, D, kind, at, _stream(stream))
-    _check(rc, "cudalm_rotary_rotate")
+    if rc:
+        _check(rc, "cudalm_rotary_rotate")
     return out
 
 
@@ -153,7 +145,9 @@ def append(q, k_new, v_new, k, v, tables, lens, rot: Rotary, positions=None, cu_
     if index != rot.index:
         raise ValueError("rotary: the frequencies are on the cache's GPU")
     if _elsewhere(index):
-        with _on(index):
+        import torch
+
+        with torch.cuda.device(index):
             return append(q, k_new, v_new, k, v, tables, lens, rot, positions, cu_new, weights, out, stream)
     heads = k.shape[1]
     kt, kh = _rows(k_new, 1, heads, k, index, "k_new")
@@ -164,8 +158,8 @@ def append(q, k_new, v_new, k, v, tables, lens, rot: Rotary, positions=None, cu_
     rows = None
     if q is not None:
         qt, qh = _rows(q, 1, None, k, index, "q")
-        out = _out(q, out, stream)
-        rows = _pack_rows(q.data_ptr(), out.data_ptr(), qt, qh, *_strides(out), q.shape[1])
+        out, to = _out(q, q.shape, q.dtype, index, out, stream)
+        rows = _pack_rows(q.data_ptr(), out.data_ptr(), qt, qh, *to, q.shape[1])
     at = None if positions is None else _positions(rot, positions, T, index)
     cu = None
     if cu_new is not None:

@@ -20,10 +20,10 @@
  * Ownership, threading and errors are those of cudalm_w4a16.h: the caller owns every
  * buffer, calls keep no state, never synchronize and enqueue on `stream`; the same
  * CUDALM_W4A16_E* codes (EINVAL: a size or type that is not served; ENULL: a required
- * pointer is NULL; EALIGN: x, A, B or a workspace that is not 16-byte aligned, or x's
+ * pointer is NULL; EALIGN: x, A, B or a plan that is not 16-byte aligned, or x's
  * row stride no multiple of 8, other bases below their elements' alignment; ERANGE: more
- * work than one launch or index holds, or a buffer that is too small). A workspace
- * serves one call at a time; a plan may be read by any number.
+ * work than one launch or index holds, or a buffer that is too small). A plan may be
+ * read by any number of calls at a time.
  */
 #ifndef CUDALM_LORA_H
 #define CUDALM_LORA_H
@@ -43,7 +43,7 @@ extern "C" {
 #define CUDALM_LORA_F16 1
 #define CUDALM_LORA_MAX_PROJ 8
 #define CUDALM_LORA_MAX_RANK 256
-#define CUDALM_LORA_MAX_ADAPTERS 8192
+#define CUDALM_LORA_MAX_ADAPTERS 4096
 
 typedef struct cudalm_lora_proj {
   const void* a; /* [adapters][rank][K] */
@@ -65,10 +65,9 @@ int cudalm_lora_plan(const int32_t* index, int M, int adapters, void* plan, size
  * most 256). plan: made for the same M and adapters. scales: [adapters] fp32, device
  * (NULL: 1). ranks: [adapters] int32, device (NULL: `rank` each): how many rows of A and
  * columns of B adapter i uses; what stands in the others (padding) has no effect. */
-size_t cudalm_lora_workspace_bytes(int count, int M, int rank, int type);
 int cudalm_lora_add(const cudalm_lora_proj* projs, int count, const void* x, int64_t x_stride, int K,
                     int M, int rank, int adapters, int type, const float* scales, const int32_t* ranks,
-                    const void* plan, void* workspace, size_t workspace_bytes, hipStream_t stream);
+                    const void* plan, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -37,7 +37,7 @@ CASES = [(1, 1024, [4096, 512, 512], 16, 8, "bf16", "one"), (1, 128, [16], 8, 1,
          (21, 8, [7], 8, 4, "bf16", "each"), (50, 264, [33, 1, 130], 40, 7, "f16", "each"),
          (5, 128, [48], 256, 2, "bf16", "turn"), (18, 256, [96], 200, 2, "f16", "each"),
          (9, 128, [64], 16, 4, "bf16", "none"), (200, 128, [32], 16, 1, "f16", "one"),
-         (130, 128, [16] * 8, 16, 130, "bf16", "turn"), (400, 64, [40], 8, 8192, "bf16", "each")]
+         (130, 128, [16] * 8, 16, 130, "bf16", "turn"), (400, 64, [40], 8, 4096, "bf16", "each")]
 
 
 @pytest.mark.parametrize("M,K,Ns,R,L,dtype,index", CASES)
