@@ -46,9 +46,12 @@ __device__ __forceinline__ void make_angles(float2* cs, const Turn& a, long long
   }
 }
 
-// Eight pairs, or 16 channels that are copied, of one token: where they are in a head.
+// Twice eight channels of a token: eight pairs, or channels that are copied. The second
+// eight are half of the rotated (copied) channels further, so that threads side by side
+// have channels side by side.
 struct Chunk {
-  int at0, at1;  // channels; at1 < 0: none (eight channels are left to copy)
+  int at0, at1;      // channels; at1 < 0: none
+  int pair0, pair1;  // of the first four pairs and the others
   bool turned;
 };
 __device__ __forceinline__ Chunk chunk_of(const Turn& a, int c, int D) {
@@ -56,11 +59,15 @@ __device__ __forceinline__ Chunk chunk_of(const Turn& a, int c, int D) {
   Chunk r;
   r.turned = c < turned;
   if (r.turned) {
-    r.at0 = a.adjacent ? 16 * c : 8 * c;
-    r.at1 = a.adjacent ? 16 * c + 8 : a.pairs + 8 * c;
+    r.at0 = 8 * c;
+    r.at1 = a.pairs + 8 * c;
+    r.pair0 = a.adjacent ? 4 * c : 8 * c;
+    r.pair1 = a.adjacent ? a.pairs / 2 + 4 * c : 8 * c + 4;
   } else {
-    r.at0 = 16 * c;
-    r.at1 = r.at0 + 8 < D ? r.at0 + 8 : -1;
+    const int eights = (D - 2 * a.pairs) / 8, half = (eights + 1) / 2, i = c - turned;
+    r.at0 = 2 * a.pairs + 8 * i;
+    r.at1 = i + half < eights ? r.at0 + 8 * half : -1;
+    r.pair0 = r.pair1 = 0;
   }
   return r;
 }
@@ -81,8 +88,7 @@ __device__ __forceinline__ float lower(uint32_t w) {
   return T::value(static_cast<uint16_t>(w));
 }
 
-// Turns the pairs that u and v hold: of channels at0 .. and at1 .. (element e of both
-// is a pair), or pairs side by side.
+// Turns the pairs that u and v hold: element e of both is a pair, or those side by side.
 template <typename T>
 __device__ __forceinline__ void turn_chunk(bool adjacent, const float2* cs, u32x4_t& u, u32x4_t& v) {
   if (adjacent) {
@@ -107,6 +113,19 @@ __device__ __forceinline__ void turn_chunk(bool adjacent, const float2* cs, u32x
   }
 }
 
+// Results pass the caches by: nothing here reads them again (19201 rows of 16 heads of 128: 34
+// us with ordinary stores, 27 so; eight prompts 63 and 58).
+__device__ __forceinline__ void stream16(uint16_t* p, u32x4_t v) {
+  __builtin_nontemporal_store(v, reinterpret_cast<u32x4_t*>(p));
+}
+
+// The same for what is read once (eight prompts: 56 us; rotate_kernel is the slower one with
+// it, 30).
+template <typename V>
+__device__ __forceinline__ V load_once(const uint16_t* p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+}
+
 struct RotateArgs {
   Turn turn;
   const uint16_t* x;
@@ -115,7 +134,8 @@ struct RotateArgs {
   int heads, D, each;  // each: tokens of a workgroup
 };
 
-// 16 bytes at a time.
+// 16 bytes at a time. Bytes bound it: 19201 rows of 16 heads of 128 (158 MB) 27 us, 5.9 TB/s (with
+// four heads of a thread on their way before the angles are made 37, by ordinary stores).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void rotate_kernel(const RotateArgs a) {
   extern __shared__ float2 angles[];
@@ -132,15 +152,15 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(const RotateArgs a) {
   float2 cs[8];
   if (c.turned)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) cs[e] = angles[t * a.turn.pairs + 8 * (item - t * chunks) + e];
+    for (int e = 0; e < 8; ++e) cs[e] = angles[t * a.turn.pairs + (e < 4 ? c.pair0 + e : c.pair1 + e - 4)];
   const uint16_t* x = a.x + (row0 + t) * a.x_token;
   uint16_t* out = a.out + (row0 + t) * a.out_token;
   for (int h = first; h < a.heads; h += together) {
     u32x4_t u = load16(x + h * a.x_head + c.at0), v = {0, 0, 0, 0};
     if (c.at1 >= 0) v = load16(x + h * a.x_head + c.at1);
     if (c.turned) turn_chunk<T>(a.turn.adjacent, cs, u, v);
-    store16(out + h * a.out_head + c.at0, u);
-    if (c.at1 >= 0) store16(out + h * a.out_head + c.at1, v);
+    stream16(out + h * a.out_head + c.at0, u);
+    if (c.at1 >= 0) stream16(out + h * a.out_head + c.at1, v);
   }
 }
 
@@ -188,12 +208,17 @@ struct RotaryAppendArgs {
   int each, heads;  // each: new tokens of every sequence where cu is NULL
 };
 
-// One workgroup per eight positions (aligned: one interleaved group of values) of a
-// sequence; units are numbered as in paged_append_kernel. Positions before the first
-// place count here too, since their queries are rotated.
+// Two workgroups per eight positions (aligned: one interleaved group of values) of a
+// sequence, one for queries and keys and one for values; units are numbered as in
+// paged_append_kernel. Positions before the first place count here too, since their queries
+// are rotated. Bytes bound it for prompts: eight of up to 2001 tokens, 32 heads on 8 of 128
+// (265 MB): 56 us, 4.7 TB/s; with ordinary loads and stores 63, 68 with all three in one workgroup,
+// 72 with four heads of a thread on their way at once. A step of 32 sequences, 8 heads on 2 of 256, takes
+// 5 us, latency.
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads) void rotary_append_kernel(const RotaryAppendArgs a) {
   extern __shared__ float2 angles[];
+  const bool values = blockIdx.y == 1;
   int b, begin, n, g;
   if (a.cu) {
     b = sequence_of(a.cu, a.kv.batch, blockIdx.x, 1, 8, 2);
@@ -216,37 +241,35 @@ __global__ __launch_bounds__(kThreads) void rotary_append_kernel(const RotaryApp
   const int lo = first > p0 ? first - p0 : 0, hi = length - p0 < 8 ? length - p0 : 8;
   const long long row0 = static_cast<long long>(begin) + p0 + lo - first;  // of token lo
   const int count = hi - lo;
-  make_angles(angles, a.turn, row0, p0 + lo, count);
   const int page = p0 >= 0 ? a.kv.page(b, p0 >> a.kv.page_shift) : -1;
   const int P = 1 << a.kv.page_shift, off = p0 & (P - 1);
-  __syncthreads();
-  // queries and keys: tokens x 16-channel chunks x heads
-  constexpr int kChunks = D / 16;
-  const int items = count * kChunks, together = kThreads / items;
-  const int start = threadIdx.x / items, item = threadIdx.x - start * items;
-  const int t = item / kChunks;
-  if (start < together) {
+  if (!values) {
+    // tokens x twice eight channels x heads
+    constexpr int kChunks = D / 16;
+    const int items = count * kChunks, together = kThreads / items;
+    const int start = threadIdx.x / items, item = threadIdx.x - start * items;
+    const int t = item / kChunks;
     const Chunk c = chunk_of(a.turn, item % kChunks, D);
+    const int last = start < together ? a.heads + (page >= 0 ? a.kv.kv_heads : 0) : 0;
+    const uint16_t* q = a.q + (row0 + t) * a.q_token;
+    const uint16_t* k = a.k + (row0 + t) * a.k_token;
+    uint16_t* out = a.out + (row0 + t) * a.out_token;
+    make_angles(angles, a.turn, row0, p0 + lo, count);
+    __syncthreads();
     float2 cs[8];
-    if (c.turned)
+    if (c.turned && last)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) cs[e] = angles[t * a.turn.pairs + 8 * (item % kChunks) + e];
-    const int last = a.heads + (page >= 0 ? a.kv.kv_heads : 0);
+      for (int e = 0; e < 8; ++e) cs[e] = angles[t * a.turn.pairs + (e < 4 ? c.pair0 + e : c.pair1 + e - 4)];
+    uint16_t* ck = a.ck + ((static_cast<size_t>(page < 0 ? 0 : page) * a.kv.kv_heads) * P + off + lo + t) * D;
     for (int h = start; h < last; h += together) {
-      const uint16_t* src;
-      uint16_t* dst;
-      if (h < a.heads) {
-        src = a.q + (row0 + t) * a.q_token + h * a.q_head;
-        dst = a.out + (row0 + t) * a.out_token + h * a.out_head;
-      } else {
-        src = a.k + (row0 + t) * a.k_token + (h - a.heads) * a.k_head;
-        dst = a.ck + ((static_cast<size_t>(page) * a.kv.kv_heads + h - a.heads) * P + off + lo + t) * D;
-      }
-      u32x4_t u = load16(src + c.at0), v = load16(src + c.at1);
+      const uint16_t* src = h < a.heads ? q + h * a.q_head : k + (h - a.heads) * a.k_head;
+      uint16_t* dst = h < a.heads ? out + h * a.out_head : ck + static_cast<size_t>(h - a.heads) * P * D;
+      u32x4_t u = load_once<u32x4_t>(src + c.at0), v = load_once<u32x4_t>(src + c.at1);
       if (c.turned) turn_chunk<T>(a.turn.adjacent, cs, u, v);
-      store16(dst + c.at0, u);
-      store16(dst + c.at1, v);
+      stream16(dst + c.at0, u);
+      stream16(dst + c.at1, v);
     }
+    return;
   }
   if (page < 0) return;
   // values: two channels of the group's tokens, and the weights
@@ -259,7 +282,7 @@ __global__ __launch_bounds__(kThreads) void rotary_append_kernel(const RotaryApp
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (e >= lo && e < hi)
-        pair[e] = *reinterpret_cast<const uint32_t*>(a.v + (row0 + e - lo) * a.v_token + h * a.v_head + d);
+        pair[e] = load_once<uint32_t>(a.v + (row0 + e - lo) * a.v_token + h * a.v_head + d);
     if (lo == 0 && hi == 8) {
       u32x4_t even, odd;
 #pragma unroll
@@ -267,8 +290,8 @@ __global__ __launch_bounds__(kThreads) void rotary_append_kernel(const RotaryApp
         even[e] = (pair[2 * e] & 0xFFFFu) | (pair[2 * e + 1] << 16);
         odd[e] = (pair[2 * e] >> 16) | (pair[2 * e + 1] & 0xFFFF0000u);
       }
-      store16(cv + 8 * d, even);
-      store16(cv + 8 * d + 8, odd);
+      stream16(cv + 8 * d, even);
+      stream16(cv + 8 * d + 8, odd);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -328,12 +351,13 @@ bool in_place_as_it_is(const cudalm_rotary_rows* q) {
 template <typename T>
 int launch_append(int D, const RotaryAppendArgs& a, unsigned units, hipStream_t stream) {
   const size_t lds = sizeof(float2) * kTokens * a.turn.pairs;
+  const dim3 grid(units, 2);
   if (D == 64)
-    rotary_append_kernel<T, 64><<<units, kThreads, lds, stream>>>(a);
+    rotary_append_kernel<T, 64><<<grid, kThreads, lds, stream>>>(a);
   else if (D == 128)
-    rotary_append_kernel<T, 128><<<units, kThreads, lds, stream>>>(a);
+    rotary_append_kernel<T, 128><<<grid, kThreads, lds, stream>>>(a);
   else
-    rotary_append_kernel<T, 256><<<units, kThreads, lds, stream>>>(a);
+    rotary_append_kernel<T, 256><<<grid, kThreads, lds, stream>>>(a);
   return launch_status();
 }
 
@@ -397,7 +421,7 @@ extern "C" int cudalm_rotary_append(const cudalm_rotary* rotary, const cudalm_pa
     return CUDALM_W4A16_EALIGN;
   const long long units = cu_new ? static_cast<long long>(tokens) / 8 + 2LL * kv->batch
                                  : static_cast<long long>(kv->batch) * (tokens / kv->batch / 8 + 2);
-  if (units >= kMaxGemmTiles || kv->kv_heads >= (1 << 22) || (queries && queries->heads >= (1 << 22)))
+  if (units >= kMaxGemmTiles / 2 || kv->kv_heads >= (1 << 22) || (queries && queries->heads >= (1 << 22)))
     return CUDALM_W4A16_ERANGE;
   a.kv = view_of(kv);
   a.ck = static_cast<uint16_t*>(kv->k);
