@@ -484,9 +484,16 @@ extern "C" int cudalm_lora_add(const cudalm_lora_proj* projs, int count, const v
       rank > CUDALM_LORA_MAX_RANK || (type != CUDALM_LORA_BF16 && type != CUDALM_LORA_F16))
     return CUDALM_W4A16_EINVAL;
   if (!projs) return CUDALM_W4A16_ENULL;
-  for (int p = 0; p < count; ++p)
+  for (int p = 0; p < count; ++p) {
     if (projs[p].N < 1 || (projs[p].y == projs[p].out && projs[p].y_stride != projs[p].out_stride))
       return CUDALM_W4A16_EINVAL;
+    // workgroups read x and y while others write: a result's place is its own
+    const int64_t step = projs[p].out_stride < 0 ? -projs[p].out_stride : projs[p].out_stride;
+    if (M > 1 && step < projs[p].N) return CUDALM_W4A16_EINVAL;
+    if (projs[p].out && projs[p].out == x) return CUDALM_W4A16_EINVAL;
+    for (int o = 0; o < count && projs[p].out; ++o)
+      if (o != p && (projs[p].out == projs[o].out || projs[p].out == projs[o].y)) return CUDALM_W4A16_EINVAL;
+  }
   for (int p = 0; p < count; ++p)
     if (projs[p].N > (1 << 28)) return CUDALM_W4A16_ERANGE;
   if (M == 0) return CUDALM_W4A16_OK;

@@ -342,10 +342,14 @@ bool wide_rows(const cudalm_rotary_rows* q) {
          q->x_head_stride % 8 == 0 && q->out_token_stride % 8 == 0 && q->out_head_stride % 8 == 0;
 }
 
-// In place, an element's place has to be the same for reading and writing.
-bool in_place_as_it_is(const cudalm_rotary_rows* q) {
-  return q->x != q->out ||
-         (q->x_token_stride == q->out_token_stride && q->x_head_stride == q->out_head_stride);
+// In place, an element's place has to be the same for reading and writing; and no two rows
+// are written to the same one.
+bool written_apart(const cudalm_rotary_rows* q, int tokens, int D) {
+  if (q->x == q->out && (q->x_token_stride != q->out_token_stride || q->x_head_stride != q->out_head_stride))
+    return false;
+  const int64_t t = q->out_token_stride < 0 ? -q->out_token_stride : q->out_token_stride;
+  const int64_t h = q->out_head_stride < 0 ? -q->out_head_stride : q->out_head_stride;
+  return (tokens < 2 || t >= D) && (q->heads < 2 || h >= D);
 }
 
 template <typename T>
@@ -374,7 +378,7 @@ extern "C" int cudalm_rotary_rotate(const cudalm_rotary* rotary, const cudalm_ro
   if (!rows) return CUDALM_W4A16_ENULL;
   if (tokens < 0 || rows->heads < 0 || head_dim < 2 * rotary->pairs ||
       head_dim > 2 * CUDALM_ROTARY_MAX_PAIRS ||
-      (type != CUDALM_PAGED_BF16 && type != CUDALM_PAGED_F16) || !in_place_as_it_is(rows))
+      (type != CUDALM_PAGED_BF16 && type != CUDALM_PAGED_F16) || !written_apart(rows, tokens, head_dim))
     return CUDALM_W4A16_EINVAL;
   if (tokens == 0 || rows->heads == 0) return CUDALM_W4A16_OK;
   if (!rows->x || !rows->out || !positions) return CUDALM_W4A16_ENULL;
@@ -413,7 +417,7 @@ extern "C" int cudalm_rotary_append(const cudalm_rotary* rotary, const cudalm_pa
   if (tokens < 0 || (!cu_new && tokens % kv->batch) || rotary->pairs % 8 ||
       2 * rotary->pairs > kv->head_dim)
     return CUDALM_W4A16_EINVAL;
-  if (queries && (queries->heads < 1 || !in_place_as_it_is(queries))) return CUDALM_W4A16_EINVAL;
+  if (queries && (queries->heads < 1 || !written_apart(queries, tokens, kv->head_dim))) return CUDALM_W4A16_EINVAL;
   if (tokens == 0) return CUDALM_W4A16_OK;
   if (!k || !v || (queries && (!queries->x || !queries->out))) return CUDALM_W4A16_ENULL;
   if (!aligned(k, 16) || !aligned(v, 16) || !aligned(cu_new, 4) || k_token_stride % 8 ||

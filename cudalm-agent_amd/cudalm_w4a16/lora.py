@@ -89,7 +89,7 @@ def add(x, ys, a, b, plan: Plan, scales=None, ranks=None, outs=None, stream=None
     """out_j[m] = y_j[m] + scales[i] * B_j[i] (A_j[i] x[m]) with i the adapter of row m;
     rows of none keep y. x [M, K]; ys, a, b (and outs): one tensor, or a list of up to 8 for
     projections that share x: y [M, N], a [adapters, rank, K], b [adapters, N, rank]. The
-    results replace ys, or go to outs. scales [adapters] float32 (None: 1); ranks
+    results replace ys, or go to outs, which overlap neither x nor each other. scales [adapters] float32 (None: 1); ranks
     [adapters] int32 (None: all the same): what adapter i uses of the rank, the rest is
     padding. Returns the results, as ys came."""
     if not isinstance(ys, (list, tuple)):

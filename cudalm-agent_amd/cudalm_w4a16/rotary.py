@@ -160,6 +160,8 @@ def append(q, k_new, v_new, k, v, tables, lens, rot: Rotary, positions=None, cu_
         qt, qh = _rows(q, 1, None, k, index, "q")
         out, to = _out(q, q.shape, q.dtype, index, out, stream)
         rows = _pack_rows(q.data_ptr(), out.data_ptr(), qt, qh, *to, q.shape[1])
+    else:
+        out = None
     at = None if positions is None else _positions(rot, positions, T, index)
     cu = None
     if cu_new is not None:

@@ -49,7 +49,8 @@ typedef struct cudalm_lora_proj {
   const void* a; /* [adapters][rank][K] */
   const void* b; /* [adapters][N][rank] */
   const void* y; /* [M] rows of N, y_stride elements apart */
-  void* out;     /* the same, out_stride apart; may be y, with its stride */
+  void* out;     /* the same, out_stride apart; may be y, with its stride, and overlaps
+                    nothing else of the call: not x, no other projection's y or out */
   int64_t y_stride, out_stride;
   int N;
 } cudalm_lora_proj;

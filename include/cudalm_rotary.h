@@ -57,7 +57,8 @@ typedef struct cudalm_rotary {
 /* Rows of heads with any strides (in elements; a head's D channels are contiguous). */
 typedef struct cudalm_rotary_rows {
   const void* x;
-  void* out; /* may be x itself, with x's strides: rotated in place */
+  void* out; /* may be x itself, with x's strides: rotated in place; else it overlaps x nowhere.
+                Its rows are apart: strides of at least D where there are several */
   int64_t x_token_stride, x_head_stride, out_token_stride, out_head_stride;
   int heads;
 } cudalm_rotary_rows;

@@ -46,7 +46,8 @@ def test_struct_layout(tmp_path, lora):
 def _projs(lora, count=1, **bad):
     arr = (lora.Proj * count)()
     for i in range(count):
-        arr[i] = lora.Proj(**dict(a=FAKE, b=FAKE, y=FAKE, out=FAKE, y_stride=512, out_stride=512, N=512))
+        at = FAKE + (i << 20)
+        arr[i] = lora.Proj(**dict(a=FAKE, b=FAKE, y=at, out=at, y_stride=512, out_stride=512, N=512))
     for f, v in bad.items():
         setattr(arr[count - 1], f, v)
     return arr
@@ -78,7 +79,7 @@ def test_plan_bytes_hold_every_tile(w4):
 
 def test_add_refusals(lora, w4):
     lib = w4.lib()
-    good = dict(p=None, count=2, x=FAKE, xs=1024, K=1024, M=30, rank=16, L=7, type=0, scales=FAKE, ranks=FAKE, plan=FAKE,
+    good = dict(p=None, count=2, x=FAKE + (7 << 20), xs=1024, K=1024, M=30, rank=16, L=7, type=0, scales=FAKE, ranks=FAKE, plan=FAKE,
                 stream=None)
 
     def call(proj=(), **bad):
@@ -93,12 +94,16 @@ def test_add_refusals(lora, w4):
     for bad in (dict(p=None), dict(x=None), dict(plan=None), dict(proj=dict(a=None)), dict(proj=dict(b=None)),
                 dict(proj=dict(y=None)), dict(proj=dict(out=None))):
         assert call(**bad) == w4.ENULL, bad
-    for bad in (dict(x=FAKE + 8), dict(xs=1028), dict(plan=FAKE + 4), dict(scales=FAKE + 2),
+    for bad in (dict(x=FAKE + (7 << 20) + 8), dict(xs=1028), dict(plan=FAKE + 4), dict(scales=FAKE + 2),
                 dict(ranks=FAKE + 2), dict(proj=dict(a=FAKE + 2)), dict(proj=dict(b=FAKE + 8)),
                 dict(proj=dict(y=FAKE + 1)), dict(proj=dict(out=FAKE + 1))):
         assert call(**bad) == w4.EALIGN, bad
+    # results where others are read or written
+    for bad in (dict(out=FAKE + (7 << 20)), dict(out=FAKE), dict(out_stride=511, out=FAKE + (9 << 20)),
+                dict(out_stride=0, out=FAKE + (9 << 20))):
+        assert call(proj=bad, x=FAKE + (7 << 20)) == w4.EINVAL, bad
     assert call(L=4097) == w4.ERANGE and call(M=(1 << 22) + 1) == w4.ERANGE
-    assert call(proj=dict(N=(1 << 28) + 1)) == w4.ERANGE
+    assert call(proj=dict(N=(1 << 28) + 1, y_stride=1 << 29, out_stride=1 << 29)) == w4.ERANGE
     assert call(M=0) == w4.OK
 
 

@@ -89,6 +89,8 @@ def test_rotate_refusals(rot, w4):
     assert call(T=-1) == w4.EINVAL and call(D=63) == w4.EINVAL and call(D=513) == w4.EINVAL
     assert call(t=2) == w4.EINVAL and call(rows=_rows(rot, heads=-1)) == w4.EINVAL
     assert call(rows=_rows(rot, out=FAKE, out_head_stride=264)) == w4.EINVAL  # in place, elsewhere
+    # rows that would be written to one place
+    assert call(rows=_rows(rot, out_head_stride=0)) == w4.EINVAL and call(rows=_rows(rot, out_token_stride=255)) == w4.EINVAL
     assert call(T=0) == w4.OK and call(rows=_rows(rot, heads=0)) == w4.OK
     assert call(rows=_rows(rot, x=None)) == w4.ENULL and call(rows=_rows(rot, out=None)) == w4.ENULL
     assert call(p=None) == w4.ENULL and call(p=FAKE + 2) == w4.EALIGN
@@ -115,6 +117,7 @@ def test_append_refusals(rot, pk, w4):
     assert call(plan=_plan(rot, pairs=136, axes=1)) == w4.EINVAL  # more than the head has
     assert call(q=_rows(rot, heads=0)) == w4.EINVAL
     assert call(q=_rows(rot, out=FAKE, out_token_stride=0)) == w4.EINVAL
+    assert call(q=_rows(rot, out_head_stride=8)) == w4.EINVAL
     assert call(n=0) == w4.OK
     assert call(k=None) == w4.ENULL and call(v=None) == w4.ENULL
     assert call(q=_rows(rot, x=None)) == w4.ENULL and call(q=_rows(rot, out=None)) == w4.ENULL
