@@ -118,8 +118,8 @@ int cudalm_paged_decode(const cudalm_paged_kv* kv, const cudalm_paged_query* q, 
  * pages are read once for all of a group's queries. Group g is sequences cu[g] .. cu[g + 1] - 1
  * (device, [count + 1], ascending within 0 .. batch; sequences of no group share
  * nothing); its first shared[g] tokens (device, [count]; any number, below zero counts as
- * zero) are those in the pages of its first sequence, and what the other sequences'
- * tables hold for them does not count (of a page that is shared in part they hold the
+ * zero) are those in the pages of its first sequence, past its length too, and what the other
+ * sequences' tables hold for them does not count (of a page that is shared in part they hold the
  * rest). A sequence need not have them all: it sees those of its length. Where every
  * table names the same pages, results are those of cudalm_paged_decode but for rounding.
  * (Bounds that do not ascend make their sequences' results unspecified; nothing outside of the

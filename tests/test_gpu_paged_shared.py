@@ -27,7 +27,13 @@ class Shared:
                 self.k[b], self.v[b] = c.k[b].clone(), c.v[b].clone()
                 self.k[b][:n], self.v[b][:n] = c.k[lo][:n], c.v[lo][:n]
                 self.here[b][:n] = c.here[lo][:n]
-                self.here[b][n:min(S, lens[b])] = False  # past the first one's end, where it has no pages
+                # past the first one's end: what its last page holds there (the cache's pages are of NaN
+                # before tokens are written), and where it has no page, nothing
+                held = min(S, lens[b], -(-lens[lo] // page) * page)
+                if n < held:
+                    self.k[b][n:held] = self.v[b][n:held] = float("nan")
+                    self.here[b][n:held] = c.here[lo][n - 1]
+                self.here[b][max(n, held):min(S, lens[b])] = False
                 for w in range(W):
                     if (w + 1) * page <= S:
                         c.tables[b, w] = {"same": c.tables[lo, w], "none": -1, "nan": free[0]}[others]
@@ -89,6 +95,19 @@ def test_decode_shared(dev, case, window, sinks, others):
     for expect in (dict(max_shared=1), dict(max_shared=max(1, max(CASES[case]["shared"])), max_len=max(t.lens))):
         again = pk.decode_shared(q, k, v, tables, lens, t.cu, t.shared, window=window, sinks=sinks, **expect)
         t.check(again, t.c.D ** -0.5, window, sinks, (others, expect))
+
+
+def test_many_groups_some_of_them_empty(dev):
+    # bounds: runs of the same one around places 63, 64 and 128; sequences before the first group
+    # and behind the last
+    cu = [3] * 60 + [5, 8] + [9] * 10 + list(range(10, 66)) + [70] * 5 + list(range(90, 121, 2))
+    lens = [20 + b % 31 for b in range(150)]
+    shared = [5 + g % 23 for g in range(len(cu) - 1)]
+    from cudalm_w4a16 import paged_kv as pk
+
+    t = Shared(dev, 77, lens, cu, shared, 1, 2, 64, 16, "bf16")
+    k, v, tables, lens = t.c.upload()
+    t.check(pk.decode_shared(t.q.to(dev), k, v, tables, lens, t.cu, t.shared), 64 ** -0.5, 0, 0, "many groups")
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
