@@ -8,9 +8,12 @@
 //
 //   out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s     over the parts of both kinds
 //
-// They share one launch. The products are those of prefill and decode: which token a row
-// of the first one stands for is free, so that a lane's scores are its operand of the
-// second one.
+// They share one launch: prefixes are bound by the matrix unit and their waits, own tokens by
+// memory, so they run side by side on a CU (64 sequences behind 8192 tokens, 700 of their own each,
+// 8 heads on 2 of 256: 20 us of prefixes and 20 of own tokens take 27.5 together, 102 MB; in
+// launches of their own 22.6 and 24.3). The products are those of prefill and decode: which
+// token a row of the first one stands for is free, so that a lane's scores are its operand of
+// the second one.
 
 #include <cmath>
 #include <type_traits>
@@ -173,7 +176,11 @@ __device__ __forceinline__ int chunk_exchange(int r) {
 // Tiles of keys and of values take turns in a ring of kRing places in LDS, which they
 // reach from the pages without passing registers: unit 2 i is the keys of tile i, unit 2 i +
 // 1 its values. A place is loaded again as soon as all waves have read it, so that kRing - 1 units
-// are on their way or waiting at any time.
+// are on their way or waiting at any time. A tile takes 1.7 us where 256 channels have two
+// workgroups on a CU, of which the matrix unit works 30% for each: the rest is waiting for LDS and
+// the other wave's turn (32768 tokens, 128 samples, 8 heads on 2 of 256: 69 us beside 1024 own
+// tokens of every sample, 0.5 PFLOP/s of the prefix's products, 271 MB). Parts of more tiles would
+// save bytes and leave CUs idle.
 // Row r of a tile of 32 keys in LDS is token r with bits 2 and 3 exchanged: then the
 // eight scores that a lane holds of a row after the first product are those of eight
 // consecutive tokens, which is its operand of the second.
@@ -606,7 +613,9 @@ struct Segments {
 // The rows of a (sequence, head), its new tokens times the group's query heads, are the 16
 // columns of 16x16x32 products; keys and values come straight from the pages into
 // registers. RT tiles of 16 rows have a wave each, which walk over the same tokens; beside them
-// 4 / RT ranges. No wave waits for another.
+// 4 / RT ranges. No wave waits for another, since a range's end may be a wave's second part or
+// third (barriers for them took the 27.5 us above to 41). Alone they stream 45 MB in 20 us,
+// 128 x 1024 tokens 134 MB in 37: memory and the first loads' chain (lengths, groups, pages, keys).
 template <typename T, int D, int RT>
 __device__ __forceinline__ void own_body(const SharedArgs& a, uint16_t* lds, unsigned block) {
   constexpr int KK = D / 32, DT = D / 16, SL = kWaves / RT;
