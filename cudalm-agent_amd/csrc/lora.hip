@@ -49,28 +49,24 @@ struct PlanArgs {
 };
 
 // For every lane with a number a (a < 0: none): how much counter[a] was before the lanes
-// up to this one added one each, those of a wave in their order.
+// up to this one added one each. Lanes of one number, as prompts have them, add in one; others each for
+// themselves (64 rows of 48 adapters: 3.0 us, 7.1 with an addition of all of a number's lanes in turn).
 __device__ __forceinline__ int claim(int* counter, int a) {
-  int at = 0;
   const int lane = threadIdx.x & 63;
-  uint64_t left = __ballot(a >= 0);
-  while (left) {
-    const int leader = __builtin_ctzll(left);
-    const int one = __builtin_amdgcn_readlane(a, leader);
-    const uint64_t same = __ballot(a == one);
-    int base = 0;
-    if (lane == leader) base = atomicAdd(&counter[one], static_cast<int>(__popcll(same)));
-    base = __builtin_amdgcn_readlane(base, leader);
-    if (a == one) at = base + static_cast<int>(__popcll(same & ((1ULL << lane) - 1)));
-    left &= ~same;
-  }
-  return at;
+  const uint64_t real = __ballot(a >= 0);
+  if (real == 0) return 0;
+  const int leader = __builtin_ctzll(real), one = __builtin_amdgcn_readlane(a, leader);
+  if (__ballot(a == one) != real) return a >= 0 ? atomicAdd(&counter[a], 1) : 0;
+  int base = 0;
+  if (lane == leader) base = atomicAdd(&counter[one], static_cast<int>(__popcll(real)));
+  base = __builtin_amdgcn_readlane(base, leader);
+  return base + static_cast<int>(__popcll(real & ((1ULL << lane) - 1)));
 }
 
-// One workgroup: rows per adapter, the tiles of each, and their rows. Which of two waves adds
-// its rows first is open; no result depends on it, since every row is a column of its own
-// in the products. Latency: 3 us for one row, 7 for 64 rows of 48 adapters, 9 for 4001 rows; a step has
-// one for all of its layers.
+// One workgroup: rows per adapter, the tiles of each, and their rows. Which of two rows of an
+// adapter comes first is open; no result depends on it, since every row is a column of its own
+// in the products. Latency: 3 us for one row or 64 rows of 48 adapters, 9 for 4001 rows; a
+// step has one for all of its layers.
 __global__ __launch_bounds__(kPlanThreads) void lora_plan_kernel(const PlanArgs a) {
   extern __shared__ int counter[];  // [adapters + 1], the last for rows of none; and the first tiles
   __shared__ int tiles_of[kPlanThreads / 64];

@@ -10,7 +10,7 @@
 //
 // They share one launch: prefixes are bound by the matrix unit and their waits, own tokens by
 // memory, so they run side by side on a CU (64 sequences behind 8192 tokens, 700 of their own each,
-// 8 heads on 2 of 256: 20 us of prefixes and 20 of own tokens take 27.5 together, 102 MB; in
+// 8 heads on 2 of 256: 20 us of prefixes and 20 of own tokens take 26 together, 102 MB; in
 // launches of their own 22.6 and 24.3). The products are those of prefill and decode: which
 // token a row of the first one stands for is free, so that a lane's scores are its operand of
 // the second one.
@@ -551,8 +551,8 @@ struct Segments {
   int count, end;    // tiles of a segment, end of its last one
 
   // Sequence b's group, 64 bounds of groups at a time: each lane looks for its place among those
-  // that the others hold. (64 groups of four sequences, prefixes of 1024 of 128 channels: 41 us the
-  // call; a walk of all lanes over the groups took 86 there, and half a microsecond less with one.)
+  // that the others hold. (64 groups of four sequences, prefixes of 1024 of 128 channels: 37 us the
+  // call; a walk of all lanes over the groups took 86.)
   __device__ __forceinline__ int group_of(const SharedArgs& a, int lane, int b) {
     int g = -1;
     for (int g0 = 0; g0 <= a.sharing.count; g0 += 64) {
@@ -660,7 +660,7 @@ struct Segments {
 // columns of 16x16x32 products; keys and values come straight from the pages into
 // registers. RT tiles of 16 rows have a wave each, which walk over the same tokens; beside them
 // 4 / RT ranges. No wave waits for another, since a range's end may be a wave's second part or
-// third (barriers for them took the 27.5 us above to 41). Alone they stream 45 MB in 20 us,
+// third (barriers for them: 42 us above where there were 28 without). Alone they stream 45 MB in 20 us,
 // 128 x 1024 tokens 134 MB in 37: memory and the first loads' chain (lengths, groups, pages, keys).
 template <typename T, int D, int RT>
 __device__ __forceinline__ void own_body(const SharedArgs& a, uint16_t* lds, unsigned block) {

@@ -245,3 +245,26 @@ def test_offsets_past_32_bits(dev):
     rows = lambda a: torch.stack([a[:6], torch.cat([a[:3], a[6:9]])]).to(torch.int32).contiguous()  # noqa: E731
     far = rows(torch.tensor(ids, device=dev))
     assert torch.equal(pk.decode_shared(q, k, v, far, lens, cu, shared), pk.decode_shared(q, kc, vc, rows(small), lens, cu, shared))
+
+
+def test_more_sequences_than_one_list_holds(dev):
+    """64 x 4096 sequences and some: against plain decode, two roundings of each apart."""
+    from cudalm_w4a16 import paged_kv as pk
+
+    B, D, pages = 64 * 4096 + 130, 64, 40
+    g = torch.Generator(device=dev).manual_seed(9)
+    k, v = pk.empty_cache(pages, 16, 1, D, torch.bfloat16)
+    k.normal_(generator=g), v.normal_(generator=g)
+    tables = torch.randint(0, pages, (B, 2), dtype=torch.int32, device=dev, generator=g)
+    tables[1000:1040, 0] = tables[1000, 0]
+    tables[B - 90:B - 1, 0] = tables[B - 90, 0]
+    lens = torch.randint(1, 33, (B,), dtype=torch.int32, device=dev, generator=g)
+    q = torch.randn(B, 1, D, device=dev, generator=g).to(torch.bfloat16)
+    cu = torch.tensor([1000, 1040, B - 90, B - 1], dtype=torch.int32, device=dev)
+    shared = torch.tensor([16, 0, 13], dtype=torch.int32, device=dev)
+    got = pk.decode_shared(q, k, v, tables, lens, cu, shared).float()
+    want = pk.decode(q, k, v, tables, lens).float()
+    # an output's rounding (2^-8 of it) and the weights' (2^-8 of the largest value), of both; scores and
+    # exponentials in fp32 are 2^-18 of it or less
+    tol = 2 * (2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -17) * float(v.float().abs().max()))
+    assert (got - want).abs().le(tol).all()
