@@ -10,7 +10,7 @@
 //
 // They share one launch: prefixes are bound by the matrix unit and their waits, own tokens by
 // memory, so they run side by side on a CU (64 sequences behind 8192 tokens, 700 of their own each,
-// 8 heads on 2 of 256: 20 us of prefixes and 20 of own tokens take 26 together, 102 MB; in
+// 8 heads on 2 of 256: 20 us of prefixes and 20 of own tokens take 24.4 together, 102 MB; in
 // launches of their own 22.6 and 24.3). The products are those of prefill and decode: which
 // token a row of the first one stands for is free, so that a lane's scores are its operand of
 // the second one.
@@ -535,7 +535,10 @@ __device__ __forceinline__ void prefix_body(const SharedArgs& a, uint16_t* lds, 
 
 // --- own tokens ---------------------------------------------------------------------
 
-// 16 bytes; `once`: nothing else of the call reads them, so the caches need not keep them.
+// 16 bytes; `once`: nothing else of the call reads them, so the caches need not keep them. (For
+// values. Keys are read half a line at a time, and the caches have to keep the other half: 64
+// sequences of 2000 own tokens, 8 heads of 128, take 90 us so, 104 with streaming loads for both and
+// 113 with them for neither.)
 template <bool once>
 __device__ __forceinline__ u32x4_t load_once(const uint16_t* p) {
   const u32x4_t* q = reinterpret_cast<const u32x4_t*>(p);
@@ -551,7 +554,7 @@ struct Segments {
   int count, end;    // tiles of a segment, end of its last one
 
   // Sequence b's group, 64 bounds of groups at a time: each lane looks for its place among those
-  // that the others hold. (64 groups of four sequences, prefixes of 1024 of 128 channels: 37 us the
+  // that the others hold. (64 groups of four sequences, prefixes of 1024 of 128 channels: 35 us the
   // call; a walk of all lanes over the groups took 86.)
   __device__ __forceinline__ int group_of(const SharedArgs& a, int lane, int b) {
     int g = -1;
@@ -746,7 +749,7 @@ __device__ __forceinline__ void own_body(const SharedArgs& a, uint16_t* lds, uns
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-        for (int f = 0; f < 2; ++f) kf[f][kk] = load_once<RT == 1>(kp + 4 * f * D + 32 * kk);
+        for (int f = 0; f < 2; ++f) kf[f][kk] = load16(kp + 4 * f * D + 32 * kk);
     };
     auto load_v = [&](int x) {
       const uint64_t at0 = place(x), at1 = place(x + 1), at = quarter < 2 ? at0 : at1;
