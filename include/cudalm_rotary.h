@@ -66,7 +66,8 @@ typedef struct cudalm_rotary_rows {
 /* Rotates tokens x heads rows of head_dim channels (2 * pairs .. 512; type
  * CUDALM_PAGED_BF16 or _F16): row t by positions[axis * tokens + t] (device, int32, any
  * sign). Any alignment is served; 16-byte aligned bases, strides and head_dim that are
- * multiples of 8, and pairs that are, go 16 bytes at a time. */
+ * multiples of 8, and pairs that are, go 16 bytes at a time; the same of 8 bytes and
+ * 4, 8 bytes at a time; others 2. */
 int cudalm_rotary_rotate(const cudalm_rotary* rotary, const cudalm_rotary_rows* rows, int tokens,
                          int head_dim, int type, const int32_t* positions, hipStream_t stream);
 

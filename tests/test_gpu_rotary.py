@@ -68,6 +68,29 @@ def test_rotate(dev, T, heads, D, pairs, sections, turns, adjacent, dtype, layou
     assert torch.equal(got[:, :, 2 * pairs:].cpu(), copied)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("T,heads,D,pairs,adjacent,off", [
+    (4500, 3, 72, 36, True, 0), (4500, 3, 96, 20, False, 4), (9, 20, 76, 12, True, 4), (70, 2, 508, 252, False, 0),
+    (1, 1, 8, 4, True, 0), (2, 3, 64, 32, False, 4), (6, 2, 72, 36, False, 2)])
+def test_rotate_four_at_a_time(dev, T, heads, D, pairs, adjacent, off, dtype):
+    from cudalm_w4a16 import rotary
+
+    g = torch.Generator().manual_seed(T + D)
+    rot, f = _plan(dev, pairs, None, False, adjacent)
+    x = torch.randn(T, heads, D, generator=g).to(DT[dtype])
+    p = _positions(g, 1, T, 50000)
+    want, tol = rr.rotated(x, p, f, (pairs,), False, adjacent)
+    flat = torch.full((T * heads * D + 16,), 7.0, dtype=x.dtype, device=dev)
+    xd = flat[off:off + T * heads * D].view(T, heads, D)
+    xd.copy_(x)
+    out = torch.full_like(flat, 7.0)
+    got = rotary.rotate(xd, p.to(dev), rot, out=out[off:off + T * heads * D].view(T, heads, D))
+    rr.check(got, want, tol, "apart")
+    assert torch.equal(got[:, :, 2 * pairs:].cpu(), x[:, :, 2 * pairs:])
+    assert (out[:off] == 7).all() and (out[off + T * heads * D:] == 7).all(), "written beside the rows"
+    assert torch.equal(rotary.rotate(xd, p.to(dev), rot, out=xd), got)
+
+
 def test_far_positions_are_exact(dev):
     """Angles of positions up to 2^24 (2^31 where the angle's last places, 2^-22, allow for it)."""
     from cudalm_w4a16 import rotary
