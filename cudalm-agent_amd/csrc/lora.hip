@@ -326,6 +326,7 @@ __global__ __launch_bounds__(64 * kWaves, RT < 4 ? 4 : 2) void lora_kernel(const
         float v = 0, hi, lo;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) v += shared.sums[w][i / 256][i % 256];
+        if (r >= rank) v = 0;  // padding: its zeros times Inf of x are NaN
         split(v, hi, lo);
         uint16_t* h = hidden + row * pitch + r;
         h[0] = static_cast<uint16_t>(f32_to_bf16_rne(hi));
