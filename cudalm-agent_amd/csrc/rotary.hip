@@ -10,6 +10,7 @@
 #include "cudalm_rotary.h"
 
 #include "paged_device.h"
+#include "row_places.h"
 
 namespace cudalm_hip {
 namespace {
@@ -367,14 +368,27 @@ bool wide_rows(const cudalm_rotary_rows* q, int n) {
          q->x_head_stride % n == 0 && q->out_token_stride % n == 0 && q->out_head_stride % n == 0;
 }
 
-// In place, an element's place has to be the same for reading and writing; and no two rows
-// are written to the same one.
-bool written_apart(const cudalm_rotary_rows* q, int tokens, int D) {
+// In place, an element's place has to be the same for reading and writing; and strides are no
+// shorter than rows.
+bool strides_fit(const cudalm_rotary_rows* q, int tokens, int D) {
   if (q->x == q->out && (q->x_token_stride != q->out_token_stride || q->x_head_stride != q->out_head_stride))
     return false;
   const int64_t t = q->out_token_stride < 0 ? -q->out_token_stride : q->out_token_stride;
   const int64_t h = q->out_head_stride < 0 ? -q->out_head_stride : q->out_head_stride;
   return (tokens < 2 || t >= D) && (q->heads < 2 || h >= D);
+}
+
+RowGrid read_rows(const cudalm_rotary_rows* q, int tokens, int D) {
+  return {q->x, tokens, q->x_token_stride, q->heads, q->x_head_stride, D};
+}
+RowGrid written_rows(const cudalm_rotary_rows* q, int tokens, int D) {
+  return {q->out, tokens, q->out_token_stride, q->heads, q->out_head_stride, D};
+}
+
+// No two rows are written to the same place, nor one where others are read.
+bool written_apart(const cudalm_rotary_rows* q, int tokens, int D) {
+  const RowGrid out = written_rows(q, tokens, D);
+  return places_apart(out) && (q->x == q->out || !places_meet(out, read_rows(q, tokens, D)));
 }
 
 template <typename T>
@@ -403,7 +417,7 @@ extern "C" int cudalm_rotary_rotate(const cudalm_rotary* rotary, const cudalm_ro
   if (!rows) return CUDALM_W4A16_ENULL;
   if (tokens < 0 || rows->heads < 0 || head_dim < 2 * rotary->pairs ||
       head_dim > 2 * CUDALM_ROTARY_MAX_PAIRS ||
-      (type != CUDALM_PAGED_BF16 && type != CUDALM_PAGED_F16) || !written_apart(rows, tokens, head_dim))
+      (type != CUDALM_PAGED_BF16 && type != CUDALM_PAGED_F16) || !strides_fit(rows, tokens, head_dim))
     return CUDALM_W4A16_EINVAL;
   if (tokens == 0 || rows->heads == 0) return CUDALM_W4A16_OK;
   if (!rows->x || !rows->out || !positions) return CUDALM_W4A16_ENULL;
@@ -421,6 +435,7 @@ extern "C" int cudalm_rotary_rotate(const cudalm_rotary* rotary, const cudalm_ro
   while (a.each > 1 && (static_cast<long long>(tokens) + a.each - 1) / a.each < 2LL * cu_count()) a.each /= 2;
   const long long groups = (static_cast<long long>(tokens) + a.each - 1) / a.each;
   if (groups >= kMaxGemmTiles) return CUDALM_W4A16_ERANGE;
+  if (!written_apart(rows, tokens, head_dim)) return CUDALM_W4A16_EINVAL;
   const size_t lds = sizeof(float2) * a.each * rotary->pairs;
   auto served = [&](int n) { return wide_rows(rows, n) && rotary->pairs % n == 0 && head_dim % n == 0; };
   const bool bf16 = type == CUDALM_PAGED_BF16;
@@ -443,7 +458,7 @@ extern "C" int cudalm_rotary_append(const cudalm_rotary* rotary, const cudalm_pa
   if (tokens < 0 || (!cu_new && tokens % kv->batch) || rotary->pairs % 8 ||
       2 * rotary->pairs > kv->head_dim)
     return CUDALM_W4A16_EINVAL;
-  if (queries && (queries->heads < 1 || !written_apart(queries, tokens, kv->head_dim))) return CUDALM_W4A16_EINVAL;
+  if (queries && (queries->heads < 1 || !strides_fit(queries, tokens, kv->head_dim))) return CUDALM_W4A16_EINVAL;
   if (tokens == 0) return CUDALM_W4A16_OK;
   if (!k || !v || (queries && (!queries->x || !queries->out))) return CUDALM_W4A16_ENULL;
   if (!aligned(k, 16) || !aligned(v, 16) || !aligned(cu_new, 4) || k_token_stride % 8 ||
@@ -453,6 +468,13 @@ extern "C" int cudalm_rotary_append(const cudalm_rotary* rotary, const cudalm_pa
                                  : static_cast<long long>(kv->batch) * (tokens / kv->batch / 8 + 2);
   if (units >= kMaxGemmTiles / 2 || kv->kv_heads >= (1 << 22) || (queries && queries->heads >= (1 << 22)))
     return CUDALM_W4A16_ERANGE;
+  if (queries) {
+    const RowGrid out = written_rows(queries, tokens, kv->head_dim);
+    if (!written_apart(queries, tokens, kv->head_dim) ||
+        places_meet(out, {k, tokens, k_token_stride, kv->kv_heads, k_head_stride, kv->head_dim}) ||
+        places_meet(out, {v, tokens, v_token_stride, kv->kv_heads, v_head_stride, kv->head_dim}))
+      return CUDALM_W4A16_EINVAL;
+  }
   a.kv = view_of(kv);
   a.ck = static_cast<uint16_t*>(kv->k);
   a.cv = static_cast<uint16_t*>(kv->v);

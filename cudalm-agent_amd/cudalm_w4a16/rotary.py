@@ -112,8 +112,8 @@ def _out(x, shape, dtype, index, out, stream):
 
 def rotate(x, positions, rot: Rotary, out=None, stream=None):
     """x [T, heads, D] rotated by positions [axes, T] (or [T] for one axis), int32;
-    into `out`, which may be x itself, or a new tensor. Any strides of tokens and
-    heads."""
+    into `out`, which may be x itself (and else overlaps it nowhere), or a new tensor. Any
+    strides of tokens and heads; rows of `out` are apart."""
     index, dtype = x.get_device(), x.dtype
     kind = _type_of(dtype)
     shape, s = x.shape, x.stride()
@@ -137,8 +137,8 @@ def rotate(x, positions, rot: Rotary, out=None, stream=None):
 def append(q, k_new, v_new, k, v, tables, lens, rot: Rotary, positions=None, cu_new=None, weights=None,
            out=None, stream=None):
     """paged_kv.append with keys rotated on the way, and queries q [T, heads, D] (or
-    None) rotated by the same positions: into `out`, which may be q itself, or a new
-    tensor, which is returned. positions [axes, T] int32; None: a token's place in the
+    None) rotated by the same positions: into `out`, which may be q itself and overlaps no
+    other rows of the call, or a new tensor; it is returned. positions [axes, T] int32; None: a token's place in the
     cache (not its position any more after an eviction). Rows of no sequence are left
     as they are."""
     kv, index = _cache(k, v, tables, lens, weights)

@@ -57,8 +57,9 @@ typedef struct cudalm_rotary {
 /* Rows of heads with any strides (in elements; a head's D channels are contiguous). */
 typedef struct cudalm_rotary_rows {
   const void* x;
-  void* out; /* may be x itself, with x's strides: rotated in place; else it overlaps x nowhere.
-                Its rows are apart: strides of at least D where there are several */
+  void* out; /* may be x itself, with x's strides: rotated in place; else it overlaps x nowhere,
+                nor k or v of append. Its rows are apart. (EINVAL where rows of out share
+                places, or, if strides are the same, with rows that are read) */
   int64_t x_token_stride, x_head_stride, out_token_stride, out_head_stride;
   int heads;
 } cudalm_rotary_rows;
