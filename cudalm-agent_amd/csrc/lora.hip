@@ -18,6 +18,7 @@
 #include "cudalm_lora.h"
 
 #include "paged_device.h"
+#include "row_places.h"
 
 namespace cudalm_hip {
 namespace {
@@ -529,6 +530,16 @@ extern "C" int cudalm_lora_add(const cudalm_lora_proj* projs, int count, const v
     a.N[p] = q.N;
     if (aligned(q.y, 16) && aligned(q.out, 16) && q.y_stride % 8 == 0 && q.out_stride % 8 == 0 && q.N % 8 == 0)
       a.wide |= 1 << p;
+  }
+  // nor does a result lie over a part of what is read, or of another one
+  for (int p = 0; p < count; ++p) {
+    const RowGrid out = {projs[p].out, M, projs[p].out_stride, 1, 0, projs[p].N};
+    if (places_meet(out, {x, M, x_stride, 1, 0, K})) return CUDALM_W4A16_EINVAL;
+    for (int o = 0; o < count; ++o) {
+      const cudalm_lora_proj& q = projs[o];
+      if ((o != p || q.y != q.out) && places_meet(out, {q.y, M, q.y_stride, 1, 0, q.N})) return CUDALM_W4A16_EINVAL;
+      if (o > p && places_meet(out, {q.out, M, q.out_stride, 1, 0, q.N})) return CUDALM_W4A16_EINVAL;
+    }
   }
   return type == CUDALM_LORA_BF16 ? launch_rank<PagedBf16>(a, tiles, stream) : launch_rank<PagedF16>(a, tiles, stream);
 }

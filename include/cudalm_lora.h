@@ -50,7 +50,8 @@ typedef struct cudalm_lora_proj {
   const void* b; /* [adapters][N][rank] */
   const void* y; /* [M] rows of N, y_stride elements apart */
   void* out;     /* the same, out_stride apart; may be y, with its stride, and overlaps
-                    nothing else of the call: not x, no other projection's y or out */
+                    nothing else of the call: not x, no other projection's y or out (EINVAL
+                    where strides are the same, or M is 1; else the caller's part) */
   int64_t y_stride, out_stride;
   int N;
 } cudalm_lora_proj;
