@@ -19,6 +19,7 @@
 #include <type_traits>
 
 #include "paged_device.h"
+#include "paged_places.h"
 
 namespace cudalm_hip {
 namespace {
@@ -646,7 +647,7 @@ struct Segments {
     load(a, lane);
   }
   // The lane whose sequence has tile g, not before the block; -1: none, where lengths change under the
-  // call.
+  // call (the join then reads an entry of `places` that was not written, within its bounds).
   __device__ __forceinline__ int find(const SharedArgs& a, int lane, int g) {
     for (;;) {
       const uint64_t after = __ballot(base + end > g);
@@ -899,8 +900,11 @@ __global__ __launch_bounds__(64 * WV) void paged_shared_join_kernel(const Shared
   const int R = static_cast<int>(blockIdx.x / chunks / a.kv.kv_heads) * 32 + n;
   const bool real = R < a.kv.batch * a.rows;
   const int b = (real ? R : 0) / a.rows, r = (real ? R : 0) - b * a.rows, zr = r / a.part_rows;
-  const int4 place = a.places[(b * a.kv.kv_heads + h) * a.zrows + zr];
-  const int before = place.z, count = real ? before + place.y : 0, prow = place.w + r;
+  const int4 entry = a.places[(b * a.kv.kv_heads + h) * a.zrows + zr];
+  const SegmentParts place = parts_within({entry.x, entry.y, entry.z, entry.w},
+                                          2 * a.ranges + a.kv.batch * a.kv.kv_heads * a.zrows, a.splits,
+                                          a.units * kRows, a.rows);
+  const int before = place.prefix, count = real ? before + place.own : 0, prow = place.row + r;
   f32x4_t acc[PC];
 #pragma unroll
   for (int x = 0; x < PC; ++x) acc[x] = f32x4_t{0, 0, 0, 0};
@@ -920,7 +924,7 @@ __global__ __launch_bounds__(64 * WV) void paged_shared_join_kernel(const Shared
           o[i][x] = a.prefix_o[(at * (D / 8) + chunk * PC + x) * 64 + half * 32 + prow % 32];
       } else if (s < count) {
         const int y = s - before;
-        const size_t at = (static_cast<size_t>(place.x) + (y ? 2 * y - 1 : 0)) * a.part_rows + r - zr * a.part_rows;
+        const size_t at = static_cast<size_t>(own_part(place.first, y)) * a.part_rows + r - zr * a.part_rows;
         ml[i] = a.own_ml[at];
 #pragma unroll
         for (int x = 0; x < PC; ++x)
