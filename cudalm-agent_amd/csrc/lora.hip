@@ -428,7 +428,10 @@ int launch(LoraArgs& a, int tiles, hipStream_t stream) {
   // Columns per workgroup: 32 for every wave, then 64, then steps of them, until there are
   // no more than three workgroups for a CU, or two where h costs each of them more than 128 KB
   // (64 rows of 48 adapters, rank 16, K = 1024: 7.0 us with three, 8.3 with two; 4001 rows,
-  // rank 32, K = 3584: 20 and 15).
+  // rank 32, K = 3584: 528 workgroups, which three allow, 20; 264 of two steps, which is the next
+  // number below two's limit and one for a CU, 15). `tiles` is the most that a plan can have:
+  // adapters that no row has count in it and leave those in use fewer workgroups (1024 rows of one
+  // adapter, K = N = 4096, rank 16: 12.6 us among 8 adapters, 13.4 among 64, 20.2 among 512).
   const int limit = (static_cast<long long>(a.K) * (kRows + a.rank) > 65536 ? 2 : 3) * cu_count();
   long long chunks;
   int halves = 1;

@@ -440,7 +440,9 @@ __device__ __forceinline__ void prefix_body(const SharedArgs& a, uint16_t* lds, 
         const float p0 = exp2_fast(__builtin_fmaf(s[e], a.scale_log2, -m));
         const float p1 = exp2_fast(__builtin_fmaf(s[e + 1], a.scale_log2, -m));
         sum += p0 + p1;
-        // rounded to the values' type, as the matrix unit takes them; l sums the unrounded ones
+        // rounded to the values' type, as the matrix unit takes them; l sums the unrounded ones.
+        // (Two numbers for each would double the second product; against 64 bits the results' error is
+        // 0.0023 of their size in bf16, 0.0017 with exact weights: their own rounding.)
         pf[e / 8][e % 8 / 2] = T::pack(p0, p1);
       }
       l += sum;
@@ -814,7 +816,7 @@ __device__ __forceinline__ void own_body(const SharedArgs& a, uint16_t* lds, uns
         for (int e = 0; e < 8; e += 2) {
           const float p0 = exp2_fast(t[e] - m), p1 = exp2_fast(t[e + 1] - m);
           l += p0 + p1;
-          pf[e / 2] = T::pack(p0, p1);
+          pf[e / 2] = T::pack(p0, p1);  // (rounded as in prefixes)
         }
         // Zero weights times Inf or NaN are NaN: values of tokens that no row here
         // sees, which may be anything, are cleared, and Inf and NaN taken out of the

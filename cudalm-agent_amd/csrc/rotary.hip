@@ -3,9 +3,10 @@
 //
 // The cosines and sines of a token's pairs are those of all its heads: a workgroup takes
 // up to eight tokens, makes theirs once in LDS, and every thread keeps those of eight
-// pairs of one token in registers while it walks over heads. p f / pi is made in 64 bits
-// (31 bits of position times 24 of frequency), reduced there to [-1, 1], and only then
-// rounded to fp32 for the sine: positions of 10^6 are as exact as small ones.
+// pairs of one token in registers while it walks over heads. p f / pi is made in 64-bit floats
+// (three roundings: 31 bits of position times 24 of frequency are two more than a double has),
+// reduced there to [-1, 1], and only then rounded to fp32 for the sine. That last rounding, 2^-25, is
+// the larger one up to angles of 2^27.
 
 #include "cudalm_rotary.h"
 

@@ -91,7 +91,7 @@ def add(x, ys, a, b, plan: Plan, scales=None, ranks=None, outs=None, stream=None
     projections that share x: y [M, N], a [adapters, rank, K], b [adapters, N, rank]. The
     results replace ys, or go to outs, which overlap neither x nor each other. scales [adapters] float32 (None: 1); ranks
     [adapters] int32 (None: all the same): what adapter i uses of the rank, the rest is
-    padding. Returns the results, as ys came."""
+    padding. K and rank are multiples of 8. Returns the results, as ys came."""
     if not isinstance(ys, (list, tuple)):
         return add(x, [ys], [a], [b], plan, scales, ranks, None if outs is None else [outs], stream)[0]
     gpu, dtype = x.get_device(), x.dtype

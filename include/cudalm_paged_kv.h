@@ -32,7 +32,9 @@
  * -inf. Inf and NaN in the values that it sees count whatever their weights,
  * also ones that underflow or are zero next to others. Whatever stands in places
  * that no query sees (NaN included) has no effect. Query head h reads key-value head h / (heads / kv_heads). Scores,
- * statistics, sums and weights are fp32; outputs are rounded once.
+ * statistics and sums are fp32, and so is what kv->weights receives; a softmax weight
+ * is rounded to the values' type before it meets them (the matrix unit takes no wider
+ * ones), the sum that it is divided by is not; outputs are rounded once.
  *
  * Ownership, threading and errors are those of cudalm_w4a16.h: the caller
  * owns every buffer, calls keep no state, never synchronize and enqueue on

@@ -16,8 +16,9 @@
  * and the channels behind are copied. p is the token's position on the pair's axis:
  * 1 to 4 axes (one for text; time, height and width for video) share the pairs out,
  * axis 0 .. axes - 1 getting sections[0 .. axes - 1] of them. Frequencies are taken
- * as exact numbers, angles made in 64 bits, so that far positions lose nothing; the
- * rest is fp32, rounded once.
+ * as exact numbers, angles made and reduced in 64-bit floats: w is off by less than
+ * 2^-51 |w| (2^-27 at a position of 2^24 and a frequency of 1, 2^-20 at 2^31); the rest is
+ * fp32, rounded once.
  *
  * Ownership, threading and errors are those of cudalm_w4a16.h: the caller owns every
  * buffer, calls keep no state, never synchronize and enqueue on `stream`; the same
